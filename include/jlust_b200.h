@@ -67,9 +67,18 @@ enum jlb_sddmm_mode {
     JLB_SDDMM_MUL = 1  /* out[p] = (alpha*dot)*S[p] + beta*out[p] (sampled)   */
 };
 
+/* Activations of the grouped product's epilogue. */
+enum jlb_act {
+    JLB_ACT_NONE = 0,
+    JLB_ACT_RELU = 1, /* max(z, 0); NaN stays */
+    JLB_ACT_SILU = 2, /* z / (1 + exp(-z)) */
+    JLB_ACT_GELU = 3  /* z (1 + erf(z / sqrt 2)) / 2 */
+};
+
 typedef struct jlb_spmv_plan_s *jlb_spmv_plan;
 typedef struct jlb_spmm_plan_s *jlb_spmm_plan;
 typedef struct jlb_spgemm_plan_s *jlb_spgemm_plan;
+typedef struct jlb_mm_plan_s *jlb_mm_plan;
 
 /* ---------------------------------------------------------------- runtime */
 
@@ -449,6 +458,111 @@ JLB_API int jlb_sorted_compress_fill(void *stream, int dtype, int idx_base, int6
  * of a dense-over-compressed level, src/convert.jl:5-111). */
 JLB_API int jlb_positions_to_coordinates(void *stream, int idx_base, int64_t n_outer, int64_t nnz,
                                          const int32_t *ptr, int32_t *coords);
+
+/* ------------------------------------------------- routing to experts */
+
+/* The pattern of a T x E routing matrix R with k entries a row, compressed by
+ * column.  ids (T x k, origin idx_base) holds each entry's expert; an entry
+ * outside 0 .. E-1 is dropped.  Writes rowptr (E + 1): expert e's slots are
+ * rowptr[e] .. rowptr[e+1]-1; source (T * k): the token of each slot, origin
+ * idx_base, and idx_base - 1 in the slots past rowptr[E]; slot (T x k): the
+ * slot of each entry, idx_base - 1 where it is dropped.  An expert's slots
+ * follow the order of its entries (a stable sort), so the result is the same
+ * on every run.  E <= 2048.  Asynchronous: no host synchronisation, no atomics
+ * whose order shows.  No counterpart in the reference. */
+JLB_API size_t jlb_route_workspace_size(int64_t T, int64_t k, int64_t E);
+JLB_API int jlb_route(void *stream, int idx_base, int64_t T, int64_t k, int64_t E,
+                      const int32_t *ids, int32_t *rowptr, int32_t *source, int32_t *slot,
+                      void *workspace, size_t workspace_bytes);
+
+/* y[t] = sum over j of g[t, j] * z[slot[t, j]], in the order of j, for rows of
+ * N values (F32 or BF16; fp32 sums rounded once).  z has S rows; dropped
+ * entries add nothing and are not read, so a token all of whose entries are
+ * dropped gives a row of zeros.  g (T x k, fp32) may be NULL: all ones.  No
+ * counterpart in the reference. */
+JLB_API int jlb_combine(void *stream, int dtype, int idx_base, int64_t T, int64_t k, int64_t S,
+                        int64_t N, const int32_t *slot, const float *g, const void *z, int64_t ldz,
+                        void *y, int64_t ldy);
+
+/* Gradients of jlb_combine: dz[slot[t, j]] = g[t, j] * dy[t], rows of dz past
+ * rowptr[E] zero, and dg[t, j] = <dy[t], z[slot[t, j]]> (fp32, 0 for dropped
+ * entries; dg may be NULL).  Every slot belongs to one entry, as jlb_route
+ * leaves them. */
+JLB_API int jlb_combine_backward(void *stream, int dtype, int idx_base, int64_t T, int64_t k,
+                                 int64_t S, int64_t N, int64_t E, const int32_t *rowptr,
+                                 const int32_t *slot, const float *g, const void *z, int64_t ldz,
+                                 const void *dy, int64_t lddy, void *dz, int64_t lddz, float *dg);
+
+/* --------------------------------------- products grouped by expert */
+
+/* y[p] = act(z[p]) + res[p], z[p] = x[src(p)] * W[e] + bias[e] for the rows p
+ * of group e, rowptr[e] .. rowptr[e+1]-1 (origin idx_base, from the first row
+ * on): the product with a block-diagonal matrix whose blocks W[e] (K x N) have
+ * ragged row ranges.  src(p) = rows[p] (origin idx_base, a row of the T x K
+ * matrix x) or p itself when rows is NULL (then T == S).  Rows of y (S x N)
+ * past rowptr[E] belong to no group and are set to zero, their z too.  rowptr
+ * may be NULL when E == 1: all S rows are the one group (the dense product
+ * with its epilogue).
+ *
+ * F32 or BF16 values (one type for all operands) with fp32 sums rounded once
+ * to the value type.  x, res, z and y are row-major; W[e] starts at w + e *
+ * w_stride elements and is row-major (element (k, n) at k*ldw + n) or
+ * column-major (k + n*ldw).  bias (E x N, row stride ldb), res and z may be
+ * NULL; z, when given, receives the product before act.  y and z overlap no
+ * operand, except that y may be res itself.
+ *
+ * A row index outside x counts as a row of zeros, and row ranges that are not
+ * ascending inside [0, S] are cut to it; both are reported by
+ * jlb_device_status().  `workspace` holds the bytes the size query returns
+ * for the same operands (0: none needed).  Asynchronous.
+ *
+ * A plan keeps the weight's side of the call (the buffers stay the caller's
+ * and must outlive it; their values may change between calls). */
+JLB_API int jlb_mm_plan_create(jlb_mm_plan *plan, int dtype, int idx_base, int64_t E, int64_t K,
+                               int64_t N, const void *w, int64_t ldw, int64_t w_stride, int w_order,
+                               const void *bias, int64_t ldb, int act);
+JLB_API size_t jlb_mm_plan_workspace_size(jlb_mm_plan plan, int64_t S, int64_t T, const void *x,
+                                          int64_t ldx, int gather);
+JLB_API int jlb_mm_plan_execute(jlb_mm_plan plan, void *stream, int64_t S, int64_t T,
+                                const int32_t *rowptr, const int32_t *rows, const void *x,
+                                int64_t ldx, const void *res, int64_t ldr, void *z, int64_t ldz,
+                                void *y, int64_t ldy, void *workspace, size_t workspace_bytes);
+JLB_API int jlb_mm_plan_destroy(jlb_mm_plan plan);
+JLB_API size_t jlb_grouped_mm_workspace_size(int dtype, int64_t E, int64_t S, int64_t T, int64_t K,
+                                             int64_t N, const void *x, int64_t ldx, const void *w,
+                                             int64_t ldw, int64_t w_stride, int w_order,
+                                             int gather);
+JLB_API int jlb_grouped_mm(void *stream, int dtype, int idx_base, int64_t E, int64_t S, int64_t T,
+                           int64_t K, int64_t N, const int32_t *rowptr, const int32_t *rows,
+                           const void *x, int64_t ldx, const void *w, int64_t ldw,
+                           int64_t w_stride, int w_order, const void *bias, int64_t ldb, int act,
+                           const void *res, int64_t ldr, void *z, int64_t ldz, void *y,
+                           int64_t ldy, void *workspace, size_t workspace_bytes);
+
+/* dw[e] = sum over the rows p of group e of x[src(p)]^T * dz[p] (K x N, laid
+ * out as w in jlb_grouped_mm); zeros for a group without rows.  dz is S x N.
+ * The gradient with respect to x needs no entry point of its own: it is
+ * jlb_grouped_mm of dz with the weights in the other order and K and N
+ * exchanged. */
+JLB_API size_t jlb_grouped_mm_wgrad_workspace_size(int dtype, int64_t E, int64_t S, int64_t T,
+                                                   int64_t K, int64_t N, const void *x, int64_t ldx,
+                                                   const void *dz, int64_t lddz, int w_order,
+                                                   int gather);
+JLB_API int jlb_grouped_mm_wgrad(void *stream, int dtype, int idx_base, int64_t E, int64_t S,
+                                 int64_t T, int64_t K, int64_t N, const int32_t *rowptr,
+                                 const int32_t *rows, const void *x, int64_t ldx, const void *dz,
+                                 int64_t lddz, void *dw, int64_t lddw, int64_t dw_stride,
+                                 int w_order, void *workspace, size_t workspace_bytes);
+
+/* dz = dy * act'(z) for the rows of the groups (rows past rowptr[E] are not
+ * written), and db[e] = the sum of group e's rows of dz before their rounding
+ * (zeros for a group without rows).  dz or db may be NULL; z may be NULL when
+ * act is JLB_ACT_NONE.  dz may be dy itself. */
+JLB_API size_t jlb_act_backward_workspace_size(int64_t E, int64_t S, int64_t N, int need_db);
+JLB_API int jlb_act_backward(void *stream, int dtype, int idx_base, int64_t E, int64_t S, int64_t N,
+                             const int32_t *rowptr, int act, const void *dy, int64_t lddy,
+                             const void *z, int64_t ldz, void *dz, int64_t lddz, void *db,
+                             int64_t lddb, void *workspace, size_t workspace_bytes);
 
 /* ------------------------------------- row-partitioned SpMV (multi-GPU) */
 

@@ -6,7 +6,8 @@ bsr_tensor, ust), formats (Formats.CSR/COO/BSRRight/DensedRight), op tags
 (SpMVOp, SpMMOp, SDDMMOp, BlockSpMMOp), the backend boundary
 (B200Backend, supports_backend, execute, prepare, update_values,
 validate_storage, default_backend), convert_format and the reference's error
-types.  Every op runs on libjlust_b200.so (hand-written CUDA for sm_100a);
+types.  Beside them stand the operators of a layer of experts: route, combine,
+grouped_matmul, fused_matmul and their gradients (experts.py).  Every op runs on libjlust_b200.so (hand-written CUDA for sm_100a);
 there is no CPU fallback.
 """
 from . import errors, synth  # noqa: F401
@@ -18,9 +19,12 @@ from .block import BlockBandedMatrix, BlockSparseMatrix, mul, update_block_value
 from .errors import (DeviceMismatch, DeviceTimeout, IncompatibleExtents,  # noqa: F401
                      IndexOriginMismatch, InvalidLevelAccess, NonCanonicalStorage,
                      UnsupportedFormat, UnsupportedIndexType, UnsupportedValueType)
+from .experts import (B200ProductHandle, Routing, combine, combine_backward,  # noqa: F401
+                      fused_matmul, fused_matmul_backward, grouped_matmul,
+                      grouped_matmul_backward, route)
 from .formats import Formats, TensorFormat, dim2lvl, format_family, lvl2dim  # noqa: F401
-from .ops import (BBMSpMVOp, BlockSpMMOp, BlockSpMVOp, Op, SDDMMOp, SpGEMMOp, SpMMOp,  # noqa: F401
-                  SpMVOp, SpSMOp, SpSVOp, SparseToDenseOp)
+from .ops import (BBMSpMVOp, BlockSpMMOp, BlockSpMVOp, FusedMMOp, GroupedMMOp, Op,  # noqa: F401
+                  SDDMMOp, SpGEMMOp, SpMMOp, SpMVOp, SpSMOp, SpSVOp, SparseToDenseOp)
 from .tensor import (OneBased, USTensor, ZeroBased, bsr_tensor, coo_tensor, shifted_diag_tensor,  # noqa: F401
                      coordinates, csr_tensor, extents, has_coordinates, has_positions,
                      index_origin, nnz, nonzeros, positions, ust)

@@ -20,6 +20,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "jlust_b200.h")
 F32, F64, BF16 = 0, 1, 2
 ROW_MAJOR, COL_MAJOR = 0, 1
 SDDMM_ADD, SDDMM_MUL = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 
 _p, _i, _i64, _d, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_double, C.c_size_t
 _pi64 = C.POINTER(C.c_int64)
@@ -85,6 +86,28 @@ SIGNATURES = {
     "jlb_sorted_compress_fill": (_i, [_p, _i, _i, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p,
                                       _p, _sz]),
     "jlb_positions_to_coordinates": (_i, [_p, _i, _i64, _i64, _p, _p]),
+    "jlb_route_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "jlb_route": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _p, _p, _p, _sz]),
+    "jlb_combine": (_i, [_p, _i, _i, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64]),
+    "jlb_combine_backward": (_i, [_p, _i, _i, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64,
+                                  _p, _i64, _p, _i64, _p]),
+    "jlb_mm_plan_create": (_i, [C.POINTER(_p), _i, _i, _i64, _i64, _i64, _p, _i64, _i64, _i, _p,
+                                _i64, _i]),
+    "jlb_mm_plan_workspace_size": (_sz, [_p, _i64, _i64, _p, _i64, _i]),
+    "jlb_mm_plan_execute": (_i, [_p, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p,
+                                 _i64, _p, _sz]),
+    "jlb_mm_plan_destroy": (_i, [_p]),
+    "jlb_grouped_mm_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64,
+                                            _i64, _i, _i]),
+    "jlb_grouped_mm": (_i, [_p, _i, _i, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64,
+                            _i64, _i, _p, _i64, _i, _p, _i64, _p, _i64, _p, _i64, _p, _sz]),
+    "jlb_grouped_mm_wgrad_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p,
+                                                  _i64, _i, _i]),
+    "jlb_grouped_mm_wgrad": (_i, [_p, _i, _i, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p,
+                                  _i64, _p, _i64, _i64, _i, _p, _sz]),
+    "jlb_act_backward_workspace_size": (_sz, [_i64, _i64, _i64, _i]),
+    "jlb_act_backward": (_i, [_p, _i, _i, _i64, _i64, _i64, _p, _i, _p, _i64, _p, _i64, _p, _i64,
+                              _p, _i64, _p, _sz]),
     "jlb_halo_spmv_steps": (_i, [_p, _i, _i, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p,
                                  _p, _p, _i, _i, C.c_uint64]),
     "jlb_ipc_handle": (_i, [_p, _p, C.POINTER(C.c_uint64)]),

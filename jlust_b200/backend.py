@@ -69,6 +69,10 @@ def supports_backend(backend, op: Op) -> bool:
         return f[0].family == "BSR" and _dense_n(f[1], 2) and _dense_n(f[2], 2)
     if op.tag == "SpGEMM" and len(f) in (2, 3):
         return all(x.family == "CSR" for x in f)
+    if op.tag == "GroupedMM" and len(f) == 4:
+        return _dense_n(f[0], 2) and _dense_n(f[1], 3) and _dense_n(f[2], 1) and _dense_n(f[3], 2)
+    if op.tag == "FusedMM" and len(f) == 3:
+        return all(_dense_n(x, 2) for x in f)
     return False
 
 
@@ -296,6 +300,9 @@ _EXEC = {"SpMV": spmv, "SpMM": spmm, "SDDMM": sddmm, "BlockSpMM": bsr_spmm, "SpG
 def backend_execute(backend, op: Op, *tensors, **kw):
     if not supports_backend(backend, op):
         raise UnsupportedFormat(f"{op} not supported by {backend!r}")
+    if op.tag in ("GroupedMM", "FusedMM"):
+        from .experts import execute_product
+        return execute_product(op.tag, *(ust(t).val for t in tensors), **kw)
     return _EXEC[op.tag](*tensors, **kw)
 
 
@@ -481,6 +488,9 @@ def prepare(backend, op_type: OpType, A: USTensor, *more, **kw) -> AbstractKerne
         return B200SpMVHandle(A)
     if op_type.tag == "SpGEMM":
         return B200SpGEMMHandle(A, *more, **kw)
+    if op_type.tag in ("GroupedMM", "FusedMM"):
+        from .experts import B200ProductHandle
+        return B200ProductHandle(ust(A).val, grouped=op_type.tag == "GroupedMM", **kw)
     raise UnsupportedFormat(f"prepare: {op_type!r} has no prepared form on B200Backend")
 
 

@@ -62,6 +62,8 @@ int take_dev_error_halo();
 int take_dev_error_spmvfmt();
 int take_dev_error_bbm();
 int take_dev_error_spgemm();
+int take_dev_error_routing();
+int take_dev_error_emm();
 
 #define JLB_DEFINE_DEV_ERROR(unit)                                           \
     static __device__ int g_dev_error;                                       \

@@ -1,0 +1,545 @@
+// expert_mm.cu -- products grouped by expert over ragged row ranges, with
+// bias, activation and residual in the epilogue, and their gradients.  The
+// dense product is the same call with one group.
+//
+// This file holds the entry points and the kernels without tensor cores:
+// single precision, and shapes the tensor path does not take.
+#include "expert_mm.cuh"
+
+#include <new>
+
+namespace jlb {
+
+JLB_DEFINE_DEV_ERROR(emm)
+
+namespace emm {
+
+// ------------------------------------------------ tiled product, FFMA
+// out (M x N) = A (M x Kc) B (Kc x N) on 128 x 128 tiles, 16 of the inner
+// dimension a step, 256 threads with 8 x 8 sums each in fp32 registers.  An
+// operand is "k-contiguous" when neighbouring inner indices are neighbours in
+// memory, else its outer index is.
+constexpr int kTile = 128, kStep = 16, kSimtThreads = 256;
+constexpr int kPitch = kTile + 4;
+
+// Element source: outer index o (row of A or column of B), inner index i.
+template <typename T>
+struct Operand {
+    const T *p;
+    int64_t ld;
+    bool k_contig;
+    const int32_t *gather;   // maps the row index of the stored matrix, or null
+    int gbase;
+    int64_t glimit;          // rows the gathered matrix has
+    int row0;                // added to the row index of the stored matrix
+    // The stored matrix's row is the outer index when k_contig, else the inner.
+    __device__ __forceinline__ const T *row_ptr(int64_t r, bool &bad) const {
+        r += row0;
+        if (gather) {
+            r = (int64_t)__ldg(gather + r) - gbase;
+            if (r < 0 || r >= glimit) {
+                bad = true;
+                return nullptr;
+            }
+        }
+        return p + r * ld;
+    }
+};
+
+// Loads a kTile x kStep tile (outer x inner) into dst[inner][outer]; zeros
+// outside omax x imax.
+template <typename T>
+__device__ __forceinline__ void load_tile(const Operand<T> &op, int64_t o0, int64_t omax,
+                                          int64_t i0, int64_t imax, float (*dst)[kPitch]) {
+    const int tid = threadIdx.x;
+    bool bad = false;
+    if (op.k_contig) {
+        const int o = tid % kTile, ih = (tid / kTile) * 8;
+        const bool in = o0 + o < omax;
+        const T *r = in ? op.row_ptr(o0 + o, bad) : nullptr;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            dst[ih + c][o] = r && i0 + ih + c < imax ? to_f32(r[i0 + ih + c]) : 0.0f;
+    } else {
+        const int i = tid / 16, o8 = (tid % 16) * 8;
+        const bool in = i0 + i < imax;
+        const T *r = in ? op.row_ptr(i0 + i, bad) : nullptr;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            dst[i][o8 + c] = r && o0 + o8 + c < omax ? to_f32(r[o0 + o8 + c]) : 0.0f;
+    }
+    if (bad) dev_error(DEV_ERR_BOUNDS);
+}
+
+template <typename T>
+__device__ __forceinline__ void tile_product(const Operand<T> &A, int64_t m0, int64_t mmax,
+                                             const Operand<T> &B, int64_t n0, int64_t nmax,
+                                             int64_t kmax, float (&acc)[8][8]) {
+    __shared__ __align__(16) float sa[kStep][kPitch];
+    __shared__ __align__(16) float sb[kStep][kPitch];
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
+    for (int64_t k0 = 0; k0 < kmax; k0 += kStep) {
+        load_tile(A, m0, mmax, k0, kmax, sa);
+        load_tile(B, n0, nmax, k0, kmax, sb);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+            float a[8], b[8];
+            *reinterpret_cast<float4 *>(a) = *reinterpret_cast<const float4 *>(&sa[k][ty * 4]);
+            *reinterpret_cast<float4 *>(a + 4) = *reinterpret_cast<const float4 *>(&sa[k][64 + ty * 4]);
+            *reinterpret_cast<float4 *>(b) = *reinterpret_cast<const float4 *>(&sb[k][tx * 4]);
+            *reinterpret_cast<float4 *>(b + 4) = *reinterpret_cast<const float4 *>(&sb[k][64 + tx * 4]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ int tile_index(int t, int i) { return (i < 4 ? 0 : 64) + t * 4 + (i & 3); }
+
+// The group and first row of row tile `want`, tiles of `size` rows numbered
+// group by group; e = -1 past the last.  Warp 0 scans 32 groups at a time.
+struct Found {
+    int e, lo, hi, row0;
+};
+__device__ void find_row_tile(const int32_t *rowptr, int base, int64_t S, int64_t E, int size,
+                              int64_t want, Found *out) {
+    if (threadIdx.x >= kWarp) return;
+    const int lane = threadIdx.x;
+    int64_t before = 0;
+    if (lane == 0) out->e = -1;
+    for (int64_t e0 = 0; e0 < E; e0 += kWarp) {
+        int lo = 0, hi = 0;
+        if (e0 + lane < E) group_rows(rowptr, base, S, e0 + lane, lo, hi);
+        const int tiles = (int)ceil_div(hi - lo, size);
+        int inc = tiles;
+#pragma unroll
+        for (int o = 1; o < kWarp; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        const int64_t first = before + inc - tiles;
+        if (want >= first && want < first + tiles)
+            *out = Found{(int)(e0 + lane), lo, hi, lo + (int)(want - first) * size};
+        before += __shfl_sync(0xffffffffu, inc, 31);
+        if (want < before) break;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSimtThreads) product_simt(const Product P) {
+    __shared__ Found f;
+    find_row_tile(P.rowptr, P.base, P.S, P.E, kTile, blockIdx.y, &f);
+    if (blockIdx.x == 0 && P.rowptr) {
+        for (int64_t e = (int64_t)blockIdx.y * kSimtThreads + threadIdx.x; e < P.E;
+             e += (int64_t)gridDim.y * kSimtThreads)
+            if (group_bad(P.rowptr, P.base, P.S, e)) dev_error(DEV_ERR_BOUNDS);
+    }
+    // rows of no group are zero
+    if (P.rowptr) {
+        int lo, hi;
+        group_rows(P.rowptr, P.base, P.S, P.E - 1, lo, hi);
+        for (int64_t r = hi + blockIdx.y; r < P.S; r += gridDim.y)
+            for (int64_t c = (int64_t)blockIdx.x * kSimtThreads + threadIdx.x; c < P.N;
+                 c += (int64_t)gridDim.x * kSimtThreads) {
+                ((T *)P.y)[r * P.ldy + c] = from_f32<T>(0.0f);
+                if (P.z) ((T *)P.z)[r * P.ldz + c] = from_f32<T>(0.0f);
+            }
+    }
+    __syncthreads();
+    if (f.e < 0) return;
+    const int64_t n0 = (int64_t)blockIdx.x * kTile;
+    Operand<T> A{(const T *)P.x, P.ldx, true, P.rows, P.base, P.T, f.row0};
+    Operand<T> B{(const T *)P.w + f.e * P.w_stride, P.ldw, P.w_order == JLB_COL_MAJOR, nullptr, 0, 0, 0};
+    float acc[8][8];
+    tile_product<T>(A, 0, f.hi - f.row0, B, n0, P.N, P.K, acc);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t r = f.row0 + tile_index(ty, i);
+        if (r >= f.hi) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t n = n0 + tile_index(tx, j);
+            if (n >= P.N) continue;
+            float v = acc[i][j];
+            if (P.bias) v += to_f32(((const T *)P.bias)[f.e * P.ldb + n]);
+            if (P.z) ((T *)P.z)[r * P.ldz + n] = from_f32<T>(v);
+            v = act_value<T>(v, P.act);
+            if (P.res) v += to_f32(((const T *)P.res)[r * P.ldr + n]);
+            ((T *)P.y)[r * P.ldy + n] = from_f32<T>(v);
+        }
+    }
+}
+
+// dw[e] on 128 x 128 tiles; the inner dimension is the group's rows.  A
+// column-major dw is computed as its transpose, the operands swapped.
+template <typename T>
+__global__ void __launch_bounds__(kSimtThreads) gradient_simt(const Gradient G) {
+    const int64_t e = blockIdx.z;
+    int lo, hi;
+    group_rows(G.rowptr, G.base, G.S, e, lo, hi);
+    if (group_bad(G.rowptr, G.base, G.S, e) && threadIdx.x == 0) dev_error(DEV_ERR_BOUNDS);
+    Operand<T> X{(const T *)G.x, G.ldx, false, G.rows, G.base, G.T, lo};
+    Operand<T> D{(const T *)G.dz, G.lddz, false, nullptr, 0, 0, lo};
+    const bool col = G.w_order == JLB_COL_MAJOR;
+    const int64_t M = col ? G.N : G.K, N = col ? G.K : G.N;
+    const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
+    float acc[8][8];
+    tile_product<T>(col ? D : X, m0, M, col ? X : D, n0, N, hi - lo, acc);
+    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+    T *out = (T *)G.dw + e * G.dw_stride;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t r = m0 + tile_index(ty, i), c = n0 + tile_index(tx, j);
+            if (r < M && c < N) out[r * G.lddw + c] = from_f32<T>(acc[i][j]);
+        }
+}
+
+// ------------------------------------------------- activation's gradient
+// dz = dy * act'(z), and the column sums of each group's dz (the bias's
+// gradient) over kSumRows rows a CTA: 64 columns x 4 row lanes.  Sums of
+// unrounded products in fp32; a second kernel adds a group's parts in order.
+constexpr int kSumRows = 128, kSumCols = 64;
+template <typename T>
+__global__ void __launch_bounds__(256)
+act_backward(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__ rowptr, int act,
+             const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z, int64_t ldz,
+             T *__restrict__ dz, int64_t lddz, float *__restrict__ part) {
+    __shared__ Found f;
+    __shared__ float red[4][kSumCols];
+    find_row_tile(rowptr, base, S, E, kSumRows, blockIdx.y, &f);
+    __syncthreads();
+    if (f.e < 0) return;
+    const int cx = threadIdx.x % kSumCols, ry = threadIdx.x / kSumCols;
+    const int64_t c = (int64_t)blockIdx.x * kSumCols + cx;
+    float sum = 0.0f;
+    if (c < N)
+        for (int r = f.row0 + ry; r < f.hi && r < f.row0 + kSumRows; r += 4) {
+            float d = to_f32(dy[(int64_t)r * lddy + c]);
+            if (z) d *= act_slope<T>(to_f32(z[(int64_t)r * ldz + c]), act);
+            if (dz) dz[(int64_t)r * lddz + c] = from_f32<T>(d);
+            sum += d;
+        }
+    if (!part) return;
+    red[ry][cx] = sum;
+    __syncthreads();
+    if (ry == 0 && c < N)
+        part[(int64_t)blockIdx.y * N + c] = (red[0][cx] + red[1][cx]) + (red[2][cx] + red[3][cx]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+sum_parts(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__ rowptr,
+          const float *__restrict__ part, T *__restrict__ db, int64_t lddb) {
+    const int64_t e = blockIdx.y;
+    __shared__ int64_t first_s;
+    __shared__ int count_s;
+    if (threadIdx.x < kWarp) {                 // the group's parts: after those of the groups before
+        int64_t first = 0;
+        for (int64_t i = threadIdx.x; i < e; i += kWarp) {
+            int lo, hi;
+            group_rows(rowptr, base, S, i, lo, hi);
+            first += ceil_div(hi - lo, kSumRows);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
+        if (threadIdx.x == 0) {
+            int lo, hi;
+            group_rows(rowptr, base, S, e, lo, hi);
+            first_s = first;
+            count_s = (int)ceil_div(hi - lo, kSumRows);
+        }
+    }
+    __syncthreads();
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= N) return;
+    float s = 0.0f;
+    for (int i = 0; i < count_s; ++i) s += part[(first_s + i) * N + c];
+    db[e * lddb + c] = from_f32<T>(s);
+}
+
+static int64_t row_tiles_bound(int64_t E, int64_t S, bool ragged, int size) {
+    return ceil_div(S, size) + (ragged ? (E < S ? E : S) : 0);
+}
+
+static int check_types(int dtype, int idx_base) {
+    if (dtype != JLB_F32 && dtype != JLB_BF16)
+        return fail(JLB_ERR_UNSUPPORTED_VALUE_TYPE, "grouped products run on F32 and BF16 values");
+    if (idx_base != 0 && idx_base != 1) return fail(JLB_ERR_INVALID_ARGUMENT, "idx_base must be 0 or 1");
+    return JLB_OK;
+}
+
+static int check_extents(int64_t E, int64_t S, int64_t T, int64_t K, int64_t N,
+                         const int32_t *rowptr, const int32_t *rows) {
+    if (E < 0 || S < 0 || T < 0 || K < 0 || N < 0)
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "negative extent");
+    if (!rowptr && E != 1)
+        return fail(JLB_ERR_INVALID_ARGUMENT, "no row pointer: only one group has all the rows");
+    if (!rows && S != T)
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "x has %lld rows, the result %lld", (long long)T,
+                    (long long)S);
+    if (S > (int64_t)INT32_MAX - 1024 || T > (int64_t)INT32_MAX - 1024 ||
+        E > (int64_t)INT32_MAX - 1024 || K > (int64_t)INT32_MAX - 1024 || N > (int64_t)INT32_MAX - 1024)
+        return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent exceeds Int32 positions");
+    return JLB_OK;
+}
+
+static int check_weight(int order, int64_t E, int64_t K, int64_t N, int64_t ldw, int64_t stride) {
+    if (order != JLB_ROW_MAJOR && order != JLB_COL_MAJOR)
+        return fail(JLB_ERR_INVALID_ARGUMENT, "weight order must be row- or column-major");
+    if (ldw < (order == JLB_ROW_MAJOR ? N : K))
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "weight leading dimension too small");
+    if (E > 1 && stride < (order == JLB_ROW_MAJOR ? (K > 0 ? (K - 1) * ldw + N : 0)
+                                                   : (N > 0 ? (N - 1) * ldw + K : 0)))
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "experts' weights overlap");
+    return JLB_OK;
+}
+
+static int check_act(int act) {
+    return act < JLB_ACT_NONE || act > JLB_ACT_GELU
+               ? fail(JLB_ERR_INVALID_ARGUMENT, "unknown activation %d", act)
+               : JLB_OK;
+}
+
+static int run_product(cudaStream_t st, const Product &P) {
+    const int64_t ntiles = ceil_div(P.N, kTile), rtiles = row_tiles_bound(P.E, P.S, P.rowptr, kTile);
+    if (rtiles > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "too many rows (%lld)", (long long)P.S);
+    const dim3 grid((unsigned)ntiles, (unsigned)rtiles);
+    if (P.dtype == JLB_F32) product_simt<float><<<grid, kSimtThreads, 0, st>>>(P);
+    else product_simt<__nv_bfloat16><<<grid, kSimtThreads, 0, st>>>(P);
+    JLB_LAUNCH_CHECK("product_simt");
+    return ok();
+}
+
+static int run_gradient(cudaStream_t st, const Gradient &G) {
+    const bool col = G.w_order == JLB_COL_MAJOR;
+    const int64_t mt = ceil_div(col ? G.N : G.K, kTile), nt = ceil_div(col ? G.K : G.N, kTile);
+    if (mt > 65535 || G.E > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent too large");
+    const dim3 grid((unsigned)nt, (unsigned)mt, (unsigned)G.E);
+    if (G.dtype == JLB_F32) gradient_simt<float><<<grid, kSimtThreads, 0, st>>>(G);
+    else gradient_simt<__nv_bfloat16><<<grid, kSimtThreads, 0, st>>>(G);
+    JLB_LAUNCH_CHECK("gradient_simt");
+    return ok();
+}
+
+// Checks that need every argument of one call.
+static int check_call(const Product &P) {
+    int r = check_extents(P.E, P.S, P.T, P.K, P.N, P.rowptr, P.rows);
+    if (r) return r;
+    if (P.ldx < P.K || P.ldy < P.N || (P.z && P.ldz < P.N) || (P.res && P.ldr < P.N))
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "leading dimension too small");
+    if (P.S == 0 || P.N == 0) return JLB_OK;
+    if (P.E == 0 && P.S > 0)
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "rows without a group (E = 0)");
+    if (!P.y || (P.K > 0 && (!P.w || (P.T > 0 && !P.x))))
+        return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
+    return JLB_OK;
+}
+
+}  // namespace emm
+}  // namespace jlb
+
+using namespace jlb;
+
+struct jlb_mm_plan_s {
+    emm::Product p;
+};
+
+extern "C" JLB_API int jlb_mm_plan_create(jlb_mm_plan *plan, int dtype, int idx_base, int64_t E,
+                                          int64_t K, int64_t N, const void *w, int64_t ldw,
+                                          int64_t w_stride, int w_order, const void *bias,
+                                          int64_t ldb, int act) {
+    if (!plan) return fail(JLB_ERR_INVALID_ARGUMENT, "null plan");
+    *plan = nullptr;
+    int r = emm::check_types(dtype, idx_base);
+    if (!r) r = emm::check_act(act);
+    if (!r && (E < 0 || K < 0 || N < 0)) r = fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "negative extent");
+    if (!r) r = emm::check_weight(w_order, E, K, N, ldw, w_stride);
+    if (!r && bias && E > 1 && ldb < N)
+        r = fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "bias leading dimension too small");
+    if (!r && E * K * N > 0 && !w) r = fail(JLB_ERR_INVALID_ARGUMENT, "null weights");
+    if (r) return r;
+    jlb_mm_plan_s *h = new (std::nothrow) jlb_mm_plan_s();
+    if (!h) return fail(JLB_ERR_CUDA, "out of host memory");
+    emm::Product &p = h->p;
+    p = emm::Product{};
+    p.dtype = dtype;
+    p.base = idx_base;
+    p.act = act;
+    p.w_order = w_order;
+    p.E = E;
+    p.K = K;
+    p.N = N;
+    p.w = w;
+    p.ldw = ldw;
+    p.w_stride = w_stride;
+    p.bias = bias;
+    p.ldb = ldb;
+    *plan = h;
+    return ok();
+}
+
+extern "C" JLB_API int jlb_mm_plan_destroy(jlb_mm_plan plan) {
+    delete plan;
+    return ok();
+}
+
+extern "C" JLB_API size_t jlb_mm_plan_workspace_size(jlb_mm_plan plan, int64_t S, int64_t T,
+                                                     const void *x, int64_t ldx, int gather) {
+    (void)plan; (void)S; (void)T; (void)x; (void)ldx; (void)gather;
+    return 0;
+}
+
+extern "C" JLB_API int jlb_mm_plan_execute(jlb_mm_plan plan, void *stream, int64_t S, int64_t T,
+                                           const int32_t *rowptr, const int32_t *rows,
+                                           const void *x, int64_t ldx, const void *res,
+                                           int64_t ldr, void *z, int64_t ldz, void *y, int64_t ldy,
+                                           void *workspace, size_t workspace_bytes) {
+    (void)workspace; (void)workspace_bytes;
+    if (!plan) return fail(JLB_ERR_INVALID_ARGUMENT, "null plan");
+    emm::Product P = plan->p;
+    P.S = S;
+    P.T = T;
+    P.rowptr = rowptr;
+    P.rows = rows;
+    P.x = x;
+    P.ldx = ldx;
+    P.res = res;
+    P.ldr = ldr;
+    P.z = z;
+    P.ldz = ldz;
+    P.y = y;
+    P.ldy = ldy;
+    const int r = emm::check_call(P);
+    if (r) return r;
+    if (S == 0 || P.N == 0) return ok();
+    return emm::run_product(as_stream(stream), P);
+}
+
+extern "C" JLB_API size_t jlb_grouped_mm_workspace_size(int dtype, int64_t E, int64_t S, int64_t T,
+                                                        int64_t K, int64_t N, const void *x,
+                                                        int64_t ldx, const void *w, int64_t ldw,
+                                                        int64_t w_stride, int w_order, int gather) {
+    jlb_mm_plan_s h;
+    h.p = emm::Product{};
+    h.p.dtype = dtype;
+    h.p.E = E;
+    h.p.K = K;
+    h.p.N = N;
+    h.p.w = w;
+    h.p.ldw = ldw;
+    h.p.w_stride = w_stride;
+    h.p.w_order = w_order;
+    return jlb_mm_plan_workspace_size(&h, S, T, x, ldx, gather);
+}
+
+extern "C" JLB_API int jlb_grouped_mm(void *stream, int dtype, int idx_base, int64_t E, int64_t S,
+                                      int64_t T, int64_t K, int64_t N, const int32_t *rowptr,
+                                      const int32_t *rows, const void *x, int64_t ldx,
+                                      const void *w, int64_t ldw, int64_t w_stride, int w_order,
+                                      const void *bias, int64_t ldb, int act, const void *res,
+                                      int64_t ldr, void *z, int64_t ldz, void *y, int64_t ldy,
+                                      void *workspace, size_t workspace_bytes) {
+    jlb_mm_plan h = nullptr;
+    int r = jlb_mm_plan_create(&h, dtype, idx_base, E, K, N, w, ldw, w_stride, w_order, bias, ldb, act);
+    if (r) return r;
+    r = jlb_mm_plan_execute(h, stream, S, T, rowptr, rows, x, ldx, res, ldr, z, ldz, y, ldy,
+                            workspace, workspace_bytes);
+    delete h;
+    return r;
+}
+
+extern "C" JLB_API size_t jlb_grouped_mm_wgrad_workspace_size(int dtype, int64_t E, int64_t S,
+                                                              int64_t T, int64_t K, int64_t N,
+                                                              const void *x, int64_t ldx,
+                                                              const void *dz, int64_t lddz,
+                                                              int w_order, int gather) {
+    (void)dtype; (void)E; (void)S; (void)T; (void)K; (void)N; (void)x; (void)ldx; (void)dz;
+    (void)lddz; (void)w_order; (void)gather;
+    return 0;
+}
+
+extern "C" JLB_API int jlb_grouped_mm_wgrad(void *stream, int dtype, int idx_base, int64_t E,
+                                            int64_t S, int64_t T, int64_t K, int64_t N,
+                                            const int32_t *rowptr, const int32_t *rows,
+                                            const void *x, int64_t ldx, const void *dz,
+                                            int64_t lddz, void *dw, int64_t lddw,
+                                            int64_t dw_stride, int w_order, void *workspace,
+                                            size_t workspace_bytes) {
+    (void)workspace; (void)workspace_bytes;
+    int r = emm::check_types(dtype, idx_base);
+    if (!r) r = emm::check_extents(E, S, T, K, N, rowptr, rows);
+    if (!r) r = emm::check_weight(w_order, E, K, N, lddw, dw_stride);
+    if (!r && (ldx < K || lddz < N))
+        r = fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "leading dimension too small");
+    if (r) return r;
+    if (E == 0 || K == 0 || N == 0) return ok();
+    if (!dw || (S > 0 && (!dz || (T > 0 && !x)))) return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
+    const emm::Gradient G{dtype, idx_base, w_order, E, S, T, K, N, rowptr, rows,
+                          x, ldx, dz, lddz, dw, lddw, dw_stride};
+    return emm::run_gradient(as_stream(stream), G);
+}
+
+extern "C" JLB_API size_t jlb_act_backward_workspace_size(int64_t E, int64_t S, int64_t N,
+                                                          int need_db) {
+    if (!need_db || E <= 0 || S <= 0 || N <= 0) return 0;
+    return (size_t)(emm::row_tiles_bound(E, S, true, emm::kSumRows) * N * 4);
+}
+
+extern "C" JLB_API int jlb_act_backward(void *stream, int dtype, int idx_base, int64_t E, int64_t S,
+                                        int64_t N, const int32_t *rowptr, int act, const void *dy,
+                                        int64_t lddy, const void *z, int64_t ldz, void *dz,
+                                        int64_t lddz, void *db, int64_t lddb, void *workspace,
+                                        size_t workspace_bytes) {
+    int r = emm::check_types(dtype, idx_base);
+    if (!r) r = emm::check_act(act);
+    if (!r) r = emm::check_extents(E, S, S, 0, N, rowptr, nullptr);
+    if (r) return r;
+    if (lddy < N || (z && ldz < N) || (dz && lddz < N) || (db && E > 1 && lddb < N))
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "leading dimension too small");
+    if (act != JLB_ACT_NONE && !z && S > 0 && N > 0)
+        return fail(JLB_ERR_INVALID_ARGUMENT, "an activation's gradient needs the pre-activation");
+    if (N == 0 || E == 0 || (!dz && !db)) return ok();
+    if (S > 0 && !dy) return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
+    const size_t need = jlb_act_backward_workspace_size(E, S, N, db != nullptr);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(JLB_ERR_WORKSPACE, "act_backward needs %zu workspace bytes", need);
+    if (act == JLB_ACT_NONE) z = nullptr;
+    cudaStream_t st = as_stream(stream);
+    const int64_t tiles = emm::row_tiles_bound(E, S, rowptr, emm::kSumRows);
+    if (tiles > 65535 || E > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent too large");
+    float *part = db ? (float *)workspace : nullptr;
+    if (tiles > 0) {
+        const dim3 grid((unsigned)ceil_div(N, emm::kSumCols), (unsigned)tiles);
+        if (dtype == JLB_F32)
+            emm::act_backward<float><<<grid, 256, 0, st>>>(
+                E, S, N, idx_base, rowptr, act, (const float *)dy, lddy, (const float *)z, ldz,
+                (float *)dz, lddz, part);
+        else
+            emm::act_backward<__nv_bfloat16><<<grid, 256, 0, st>>>(
+                E, S, N, idx_base, rowptr, act, (const __nv_bfloat16 *)dy, lddy,
+                (const __nv_bfloat16 *)z, ldz, (__nv_bfloat16 *)dz, lddz, part);
+        JLB_LAUNCH_CHECK("act_backward");
+    }
+    if (db) {
+        const dim3 grid((unsigned)ceil_div(N, 256), (unsigned)E);
+        if (dtype == JLB_F32)
+            emm::sum_parts<float><<<grid, 256, 0, st>>>(E, S, N, idx_base, rowptr, part,
+                                                        (float *)db, lddb);
+        else
+            emm::sum_parts<__nv_bfloat16><<<grid, 256, 0, st>>>(E, S, N, idx_base, rowptr, part,
+                                                                (__nv_bfloat16 *)db, lddb);
+        JLB_LAUNCH_CHECK("sum_parts");
+    }
+    return ok();
+}

@@ -1,0 +1,118 @@
+// expert_mm.cuh -- what the translation units of the grouped and fused
+// products share: the call's operands, the row groups and the activations.
+#pragma once
+
+#include "common.cuh"
+
+namespace jlb {
+namespace emm {
+
+// One product y[p] = act(x[src(p)] W[e] + b[e]) + r[p], p in group e.
+struct Product {
+    int dtype, base, act;
+    int w_order;                       // JLB_ROW_MAJOR: element (k, n) at k*ldw + n
+    int64_t E, S, T, K, N;             // experts, output rows, rows of x, inner and output widths
+    const int32_t *rowptr;             // E + 1; null with E == 1: all S rows are one group
+    const int32_t *rows;               // S: the row of x of each output row; null: the row itself
+    const void *x;
+    int64_t ldx;
+    const void *w;
+    int64_t ldw, w_stride;             // leading dimension, elements from one expert to the next
+    const void *bias;                  // E x N, or null
+    int64_t ldb;
+    const void *res;                   // S x N, or null
+    int64_t ldr;
+    void *z;                           // S x N: the product before act, or null
+    int64_t ldz;
+    void *y;
+    int64_t ldy;
+};
+
+// dw[e] = sum over p in group e of x[src(p)]^T dz[p] (K x N each).
+struct Gradient {
+    int dtype, base;
+    int w_order;                       // layout of dw
+    int64_t E, S, T, K, N;
+    const int32_t *rowptr;
+    const int32_t *rows;
+    const void *x;
+    int64_t ldx;
+    const void *dz;
+    int64_t lddz;
+    void *dw;
+    int64_t lddw, dw_stride;
+};
+
+// Rows [lo, hi) of group e, kept inside [0, S] whatever rowptr holds.
+__device__ __forceinline__ void group_rows(const int32_t *__restrict__ rowptr, int base, int64_t S,
+                                           int64_t e, int &lo, int &hi) {
+    if (!rowptr) {
+        lo = 0;
+        hi = (int)S;
+        return;
+    }
+    lo = __ldg(rowptr + e) - base;
+    hi = __ldg(rowptr + e + 1) - base;
+    lo = lo < 0 ? 0 : lo > S ? (int)S : lo;
+    hi = hi < lo ? lo : hi > S ? (int)S : hi;
+}
+
+// Whether group e's row range is one that group_rows had to correct.
+__device__ __forceinline__ bool group_bad(const int32_t *__restrict__ rowptr, int base, int64_t S,
+                                          int64_t e) {
+    if (!rowptr) return false;
+    const int lo = __ldg(rowptr + e) - base, hi = __ldg(rowptr + e + 1) - base;
+    return lo < 0 || hi < lo || hi > S || (e == 0 && lo != 0);
+}
+
+// ------------------------------------------------------------ activations
+// relu keeps NaN.  silu = z / (1 + e^-z); gelu = z (1 + erf(z / sqrt 2)) / 2.
+// For BF16 results (T) the exponential and the quotient are the fast ones:
+// their error, a few units of 2^-22, is far below the rounding to 8 bits.
+template <typename T>
+__device__ __forceinline__ float exp_of(float v) {
+    return sizeof(T) == 2 ? __expf(v) : expf(v);
+}
+template <typename T>
+__device__ __forceinline__ float quotient(float a, float b) {
+    return sizeof(T) == 2 ? a * __frcp_rn(b) : a / b;
+}
+
+template <typename T>
+__device__ __forceinline__ float act_value(float z, int act) {
+    switch (act) {
+        case JLB_ACT_RELU: return z < 0.0f ? 0.0f : z;
+        case JLB_ACT_SILU: return quotient<T>(z, 1.0f + exp_of<T>(-z));
+        case JLB_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        default: return z;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case JLB_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+        case JLB_ACT_SILU: {
+            const float s = quotient<T>(1.0f, 1.0f + exp_of<T>(-z));
+            return s * (1.0f + z * (1.0f - s));
+        }
+        case JLB_ACT_GELU:
+            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
+                   z * (0.39894228040143268f * exp_of<T>(-0.5f * z * z));
+        default: return 1.0f;
+    }
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+}  // namespace emm
+}  // namespace jlb

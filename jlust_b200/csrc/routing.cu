@@ -1,0 +1,447 @@
+// routing.cu -- the routing pattern of a layer of experts and the products
+// with it.  A token's k expert indices are one row of a sparse T x E matrix R;
+// its pattern compressed by column (expert) gives each expert's rows, and
+// slot[t, j] is where entry (t, j) landed in that order.
+#include "common.cuh"
+
+namespace jlb {
+
+JLB_DEFINE_DEV_ERROR(routing)
+
+namespace routing {
+
+constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / kWarp;
+constexpr int kPer = 4;                       // entries a thread
+constexpr int kChunk = kThreads * kPer;       // entries a CTA
+constexpr int kMaxE = 2048;
+
+// The expert of entry i, or -1 when it is dropped (outside 0 .. E-1).
+__device__ __forceinline__ int expert_of(const int32_t *__restrict__ ids, int64_t i, int64_t n,
+                                         int base, int E) {
+    if (i >= n) return -1;
+    const int e = __ldg(ids + i) - base;
+    return e >= 0 && e < E ? e : -1;
+}
+
+// Entry order inside a CTA's chunk: warp w holds entries w*128 .. w*128+127,
+// lane l of round r entry w*128 + r*32 + l, so (warp, round, lane) ascends
+// with the entry index.
+__device__ __forceinline__ int64_t entry_index(int warp, int round, int lane) {
+    return (int64_t)blockIdx.x * kChunk + warp * (kWarp * kPer) + round * kWarp + lane;
+}
+
+// Entries per expert of each chunk: hist[chunk][e].
+__global__ void __launch_bounds__(kThreads) route_count(const int32_t *__restrict__ ids, int64_t n,
+                                                        int base, int E,
+                                                        int32_t *__restrict__ hist) {
+    extern __shared__ int32_t cnt[];
+    for (int e = threadIdx.x; e < E; e += kThreads) cnt[e] = 0;
+    __syncthreads();
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+        const int e = expert_of(ids, entry_index(warp, r, lane), n, base, E);
+        if (e >= 0) atomicAdd(&cnt[e], 1);    // a sum of ones: the same in any order
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kThreads) hist[(int64_t)blockIdx.x * E + e] = cnt[e];
+}
+
+// Places the entries.  Stable counting sort by expert: slot(i) = entries of
+// smaller experts + entries of the same expert in earlier chunks, earlier
+// warps of the chunk and earlier entries of the warp.  With one chunk
+// (hist == nullptr) the counts come from the warps' own.
+__global__ void __launch_bounds__(kThreads)
+route_place(const int32_t *__restrict__ ids, int64_t n, int k, int base, int E,
+            const int32_t *__restrict__ hist, int chunks, int32_t *__restrict__ rowptr,
+            int32_t *__restrict__ source, int32_t *__restrict__ slot) {
+    extern __shared__ int32_t sm[];
+    int32_t *tot = sm;                        // E: entries per expert, then their exclusive scan
+    int32_t *mine = tot + E;                  // E: entries of earlier chunks
+    uint16_t *wh = reinterpret_cast<uint16_t *>(mine + E);   // kWarps x E: the warps' counts
+    __shared__ int32_t wsum[kWarps];
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    for (int i = threadIdx.x; i < kWarps * E; i += kThreads) wh[i] = 0;
+    __syncthreads();
+    // ranks inside the warp, in entry order
+    int ex[kPer], rank[kPer];
+    uint16_t *my = wh + warp * E;
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+        ex[r] = expert_of(ids, entry_index(warp, r, lane), n, base, E);
+        const unsigned same = __match_any_sync(0xffffffffu, ex[r]);
+        const int before = __popc(same & ((1u << lane) - 1u));
+        int have = 0;
+        if (ex[r] >= 0) have = my[ex[r]];
+        __syncwarp();
+        if (ex[r] >= 0 && before == 0) my[ex[r]] = (uint16_t)(have + __popc(same));
+        __syncwarp();
+        rank[r] = have + before;
+    }
+    __syncthreads();
+    // counts over the warps become each warp's offset inside the chunk
+    for (int e = threadIdx.x; e < E; e += kThreads) {
+        int run = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            const int c = wh[w * E + e];
+            wh[w * E + e] = (uint16_t)run;
+            run += c;
+        }
+        int all = run, before = 0;
+        if (hist) {
+            all = 0;
+            for (int c = 0; c < chunks; ++c) {
+                const int h = __ldg(hist + (int64_t)c * E + e);
+                if (c < (int)blockIdx.x) before += h;
+                all += h;
+            }
+        }
+        tot[e] = all;
+        mine[e] = before;
+    }
+    __syncthreads();
+    // exclusive scan of tot over the experts, kThreads at a time
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += kThreads) {
+        const int e = e0 + threadIdx.x;
+        const int v = e < E ? tot[e] : 0;
+        int inc = v;
+#pragma unroll
+        for (int o = 1; o < kWarp; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == kWarp - 1) wsum[warp] = inc;
+        __syncthreads();
+        if (warp == 0) {
+            int s = wsum[lane];
+#pragma unroll
+            for (int o = 1; o < kWarp; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += u;
+            }
+            wsum[lane] = s;
+        }
+        __syncthreads();
+        const int excl = carry + (warp ? wsum[warp - 1] : 0) + inc - v;
+        if (e < E) {
+            tot[e] = excl;
+            if (blockIdx.x == 0) rowptr[e] = excl + base;
+        }
+        carry += wsum[kWarps - 1];
+        __syncthreads();
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) rowptr[E] = carry + base;
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+        const int64_t i = entry_index(warp, r, lane);
+        if (i >= n) continue;
+        const int e = ex[r];
+        if (e >= 0) {
+            const int p = tot[e] + mine[e] + my[e] + rank[r];
+            slot[i] = p + base;
+            source[p] = (int32_t)(i / k) + base;
+        } else {
+            slot[i] = base - 1;
+        }
+        if (i >= carry) source[i] = base - 1;    // slots that no entry took
+    }
+}
+
+// ------------------------------------------------------------ value access
+template <typename T>
+struct Val;
+template <>
+struct Val<float> {
+    static constexpr int kVec = 4;
+    static __device__ __forceinline__ float get(const float *p) { return __ldg(p); }
+    static __device__ __forceinline__ void put(float *p, float v) { *p = v; }
+    static __device__ __forceinline__ void load(const float *p, float *v) {
+        const float4 q = __ldg(reinterpret_cast<const float4 *>(p));
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    }
+    static __device__ __forceinline__ void store(float *p, const float *v) {
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+};
+template <>
+struct Val<__nv_bfloat16> {
+    static constexpr int kVec = 8;
+    static __device__ __forceinline__ float get(const __nv_bfloat16 *p) {
+        return __bfloat162float(*p);
+    }
+    static __device__ __forceinline__ void put(__nv_bfloat16 *p, float v) {
+        *p = __float2bfloat16_rn(v);
+    }
+    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float *v) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float *v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// y[t] = sum_j g[t, j] z[slot[t, j]] in the order of j, fp32 sums rounded
+// once to the value type.  V columns a thread (16 bytes, or one when the
+// layout is not aligned); blockDim = (column threads, tokens).
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+combine_rows(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__restrict__ slot,
+             const float *__restrict__ g, const T *__restrict__ z, int64_t ldz,
+             T *__restrict__ y, int64_t ldy) {
+    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (t >= T_) return;
+    const int32_t *sl = slot + t * k;
+    for (int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V; c < N;
+         c += (int64_t)gridDim.y * blockDim.x * V) {
+        float acc[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+        for (int j = 0; j < k; ++j) {
+            const int64_t p = (int64_t)__ldg(sl + j) - base;
+            if (p < 0) continue;                  // dropped entry
+            if (p >= S) {
+                dev_error(DEV_ERR_BOUNDS);
+                continue;
+            }
+            const float w = g ? __ldg(g + t * k + j) : 1.0f;
+            float v[V];
+            if (V == 1) v[0] = Val<T>::get(z + p * ldz + c);
+            else Val<T>::load(z + p * ldz + c, v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+        }
+        if (V == 1) Val<T>::put(y + t * ldy + c, acc[0]);
+        else Val<T>::store(y + t * ldy + c, acc);
+    }
+}
+
+// dz[slot[t, j]] = g[t, j] dy[t] and dg[t, j] = <dy[t], z[slot[t, j]]>: one
+// CTA a token, dy read once for up to 8 entries.  Rows of dz past the last
+// slot are zeroed.  The dot product's terms are summed per thread, then by a
+// fixed tree over the CTA.
+constexpr int kBwdThreads = 128, kBwdJ = 8;
+template <typename T, int V>
+__global__ void __launch_bounds__(kBwdThreads)
+combine_bwd(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__restrict__ slot,
+            const int32_t *__restrict__ live_end, const float *__restrict__ g,
+            const T *__restrict__ z, int64_t ldz, const T *__restrict__ dy, int64_t lddy,
+            T *__restrict__ dz, int64_t lddz, float *__restrict__ dg) {
+    __shared__ float part[kBwdThreads / kWarp][kBwdJ];
+    const int64_t t = blockIdx.x;
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    if (t >= T_) {                                // the CTAs after the tokens: rows of no slot
+        int64_t end = (int64_t)__ldg(live_end) - base;
+        end = end < 0 ? 0 : end > S ? S : end;
+        for (int64_t p = end + (t - T_); p < S; p += (int64_t)gridDim.x - T_)
+            for (int64_t c = (int64_t)threadIdx.x; c < N; c += kBwdThreads)
+                Val<T>::put(dz + p * lddz + c, 0.0f);
+        return;
+    }
+    for (int j0 = 0; j0 < k; j0 += kBwdJ) {
+        int64_t p[kBwdJ];
+        float w[kBwdJ], dot[kBwdJ];
+#pragma unroll
+        for (int j = 0; j < kBwdJ; ++j) {
+            p[j] = -1;
+            w[j] = dot[j] = 0.0f;
+            if (j0 + j < k) {
+                p[j] = (int64_t)__ldg(slot + t * k + j0 + j) - base;
+                w[j] = g ? __ldg(g + t * k + j0 + j) : 1.0f;
+                if (p[j] >= S) {
+                    dev_error(DEV_ERR_BOUNDS);
+                    p[j] = -1;
+                }
+            }
+        }
+        for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += kBwdThreads * V) {
+            float d[V];
+            if (V == 1) d[0] = Val<T>::get(dy + t * lddy + c);
+            else Val<T>::load(dy + t * lddy + c, d);
+#pragma unroll
+            for (int j = 0; j < kBwdJ; ++j) {
+                if (p[j] < 0) continue;
+                float v[V], o[V];
+                if (V == 1) v[0] = Val<T>::get(z + p[j] * ldz + c);
+                else Val<T>::load(z + p[j] * ldz + c, v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    dot[j] = fmaf(d[i], v[i], dot[j]);
+                    o[i] = w[j] * d[i];
+                }
+                if (V == 1) Val<T>::put(dz + p[j] * lddz + c, o[0]);
+                else Val<T>::store(dz + p[j] * lddz + c, o);
+            }
+        }
+        if (dg) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kBwdJ; ++j) {
+                const float s = warp_sum(dot[j]);
+                if (lane == 0) part[warp][j] = s;
+            }
+            __syncthreads();
+            if (threadIdx.x < kBwdJ && j0 + (int)threadIdx.x < k) {
+                float s = 0.0f;
+                for (int q = 0; q < kBwdThreads / kWarp; ++q) s += part[q][threadIdx.x];
+                dg[t * k + j0 + threadIdx.x] = s;
+            }
+        }
+    }
+}
+
+static size_t place_smem(int64_t E) { return (size_t)E * (8 + 2 * kWarps); }
+
+}  // namespace routing
+}  // namespace jlb
+
+using namespace jlb;
+
+extern "C" JLB_API size_t jlb_route_workspace_size(int64_t T, int64_t k, int64_t E) {
+    if (T <= 0 || k <= 0 || E <= 0) return 0;
+    const int64_t chunks = ceil_div(T * k, routing::kChunk);
+    return chunks > 1 ? (size_t)(chunks * E * 4) : 0;
+}
+
+extern "C" JLB_API int jlb_route(void *stream, int idx_base, int64_t T, int64_t k, int64_t E,
+                                 const int32_t *ids, int32_t *rowptr, int32_t *source,
+                                 int32_t *slot, void *workspace, size_t workspace_bytes) {
+    using namespace routing;
+    if (idx_base != 0 && idx_base != 1) return fail(JLB_ERR_INVALID_ARGUMENT, "idx_base must be 0 or 1");
+    if (T < 0 || k < 0 || E < 0) return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "negative extent");
+    if (E > kMaxE)
+        return fail(JLB_ERR_UNSUPPORTED_FORMAT, "more than %d experts (%lld)", kMaxE, (long long)E);
+    if (k > 0 && T > (int64_t)(INT32_MAX - kChunk) / k)
+        return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "T * k exceeds Int32 positions");
+    const int64_t n = T * k;
+    if (!rowptr || (n > 0 && (!ids || !source || !slot)))
+        return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
+    const int chunks = (int)ceil_div(n > 0 ? n : 1, kChunk);
+    const size_t need = jlb_route_workspace_size(T, k, E);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(JLB_ERR_WORKSPACE, "route needs %zu workspace bytes", need);
+    cudaStream_t st = as_stream(stream);
+    int32_t *hist = chunks > 1 ? (int32_t *)workspace : nullptr;
+    if (hist) {
+        route_count<<<chunks, kThreads, (size_t)E * 4, st>>>(ids, n, idx_base, (int)E, hist);
+        JLB_LAUNCH_CHECK("route_count");
+    }
+    const size_t smem = place_smem(E);
+    if (smem > 48 * 1024)
+        JLB_CUDA(cudaFuncSetAttribute(route_place, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)smem));
+    route_place<<<chunks, kThreads, smem, st>>>(ids, n, (int)(k > 0 ? k : 1), idx_base, (int)E,
+                                                hist, chunks, rowptr, source, slot);
+    JLB_LAUNCH_CHECK("route_place");
+    return ok();
+}
+
+namespace {
+
+int check_combine(int dtype, int idx_base, int64_t T, int64_t k, int64_t S, int64_t N) {
+    if (dtype != JLB_F32 && dtype != JLB_BF16)
+        return fail(JLB_ERR_UNSUPPORTED_VALUE_TYPE, "combine runs on F32 and BF16 values");
+    if (idx_base != 0 && idx_base != 1) return fail(JLB_ERR_INVALID_ARGUMENT, "idx_base must be 0 or 1");
+    if (T < 0 || k < 0 || S < 0 || N < 0) return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "negative extent");
+    if (T > INT32_MAX / 2 || S > INT32_MAX || k > INT32_MAX)
+        return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent exceeds Int32 positions");
+    return JLB_OK;
+}
+
+template <typename T>
+int run_combine(cudaStream_t st, int64_t Tn, int64_t k, int64_t S, int64_t N, int base,
+                const int32_t *slot, const float *g, const T *z, int64_t ldz, T *y, int64_t ldy) {
+    using routing::Val;
+    constexpr int V = Val<T>::kVec;
+    const bool vec = N % V == 0 && ldz % V == 0 && ldy % V == 0 && aligned16(z) && aligned16(y);
+    const int64_t items = vec ? N / V : N;
+    int tx = 32;
+    while (tx < 256 && tx < items) tx *= 2;
+    const int ty = 256 / tx;
+    const dim3 block(tx, ty);
+    const dim3 grid((unsigned)ceil_div(Tn, ty),
+                    (unsigned)(ceil_div(items, tx) < 65535 ? ceil_div(items, tx) : 65535));
+    if (vec)
+        routing::combine_rows<T, V><<<grid, block, 0, st>>>(Tn, (int)k, S, N, base, slot, g, z, ldz, y, ldy);
+    else
+        routing::combine_rows<T, 1><<<grid, block, 0, st>>>(Tn, (int)k, S, N, base, slot, g, z, ldz, y, ldy);
+    JLB_LAUNCH_CHECK("combine_rows");
+    return ok();
+}
+
+template <typename T>
+int run_combine_bwd(cudaStream_t st, int64_t Tn, int64_t k, int64_t S, int64_t N, int base,
+                    const int32_t *slot, const int32_t *live_end, const float *g, const T *z,
+                    int64_t ldz, const T *dy, int64_t lddy, T *dz, int64_t lddz, float *dg) {
+    using routing::Val;
+    constexpr int V = Val<T>::kVec;
+    const bool vec = N % V == 0 && ldz % V == 0 && lddy % V == 0 && lddz % V == 0 &&
+                     aligned16(z) && aligned16(dy) && aligned16(dz);
+    const unsigned grid = (unsigned)(Tn + 148);   // 148 CTAs for the rows of no slot
+    if (vec)
+        routing::combine_bwd<T, V><<<grid, routing::kBwdThreads, 0, st>>>(
+            Tn, (int)k, S, N, base, slot, live_end, g, z, ldz, dy, lddy, dz, lddz, dg);
+    else
+        routing::combine_bwd<T, 1><<<grid, routing::kBwdThreads, 0, st>>>(
+            Tn, (int)k, S, N, base, slot, live_end, g, z, ldz, dy, lddy, dz, lddz, dg);
+    JLB_LAUNCH_CHECK("combine_bwd");
+    return ok();
+}
+
+}  // namespace
+
+extern "C" JLB_API int jlb_combine(void *stream, int dtype, int idx_base, int64_t T, int64_t k,
+                                   int64_t S, int64_t N, const int32_t *slot, const float *g,
+                                   const void *z, int64_t ldz, void *y, int64_t ldy) {
+    const int r = check_combine(dtype, idx_base, T, k, S, N);
+    if (r) return r;
+    if (ldz < N || ldy < N) return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "leading dimension smaller than N");
+    if (T == 0 || N == 0) return ok();
+    if (!y || (k > 0 && !slot) || (k > 0 && S > 0 && !z))
+        return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
+    cudaStream_t st = as_stream(stream);
+    return dtype == JLB_F32 ? run_combine<float>(st, T, k, S, N, idx_base, slot, g, (const float *)z,
+                                                 ldz, (float *)y, ldy)
+                            : run_combine<__nv_bfloat16>(st, T, k, S, N, idx_base, slot, g,
+                                                         (const __nv_bfloat16 *)z, ldz,
+                                                         (__nv_bfloat16 *)y, ldy);
+}
+
+extern "C" JLB_API int jlb_combine_backward(void *stream, int dtype, int idx_base, int64_t T,
+                                            int64_t k, int64_t S, int64_t N, int64_t E,
+                                            const int32_t *rowptr, const int32_t *slot,
+                                            const float *g, const void *z, int64_t ldz,
+                                            const void *dy, int64_t lddy, void *dz, int64_t lddz,
+                                            float *dg) {
+    const int r = check_combine(dtype, idx_base, T, k, S, N);
+    if (r) return r;
+    if (E < 0) return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "negative extent");
+    if (ldz < N || lddy < N || lddz < N)
+        return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "leading dimension smaller than N");
+    if (S == 0 && T * k == 0) return ok();
+    if (!rowptr || (T * k > 0 && (!slot || (N > 0 && !dy) || (S > 0 && N > 0 && !z))) ||
+        (S > 0 && N > 0 && !dz))
+        return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
+    cudaStream_t st = as_stream(stream);
+    return dtype == JLB_F32
+               ? run_combine_bwd<float>(st, T, k, S, N, idx_base, slot, rowptr + E, g,
+                                        (const float *)z, ldz, (const float *)dy, lddy, (float *)dz,
+                                        lddz, dg)
+               : run_combine_bwd<__nv_bfloat16>(st, T, k, S, N, idx_base, slot, rowptr + E, g,
+                                                (const __nv_bfloat16 *)z, ldz,
+                                                (const __nv_bfloat16 *)dy, lddy,
+                                                (__nv_bfloat16 *)dz, lddz, dg);
+}

@@ -45,6 +45,9 @@ DenseToSparseOp = OpType("DenseToSparse", "Dense to sparse.")
 BlockSpMVOp = OpType("BlockSpMV", "Block sparse matrix x vector (src/ops.jl:128-130).")
 BlockSpMMOp = OpType("BlockSpMM", "Block sparse matrix x dense matrix (src/ops.jl:132-134).")
 BBMSpMVOp = OpType("BBMSpMV", "Block-banded matrix x vector.")
+GroupedMMOp = OpType("GroupedMM", "y[p] = act(x[rows[p]] W[e] + b[e]), p in row group e "
+                                  "(no counterpart in the reference).")
+FusedMMOp = OpType("FusedMM", "y = act(x W + b) + r (no counterpart in the reference).")
 
 
 def op_tag(op) -> str:
