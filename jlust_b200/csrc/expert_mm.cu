@@ -312,6 +312,10 @@ static int check_act(int act) {
 }
 
 static int run_product(cudaStream_t st, const Product &P) {
+    if (tc_product_ok(P)) {
+        const int r = tc_product(st, P);
+        if (r >= 0) return r;
+    }
     const int64_t ntiles = ceil_div(P.N, kTile), rtiles = row_tiles_bound(P.E, P.S, P.rowptr, kTile);
     if (rtiles > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "too many rows (%lld)", (long long)P.S);
     const dim3 grid((unsigned)ntiles, (unsigned)rtiles);
@@ -322,6 +326,10 @@ static int run_product(cudaStream_t st, const Product &P) {
 }
 
 static int run_gradient(cudaStream_t st, const Gradient &G) {
+    if (tc_gradient_ok(G)) {
+        const int r = tc_gradient(st, G);
+        if (r >= 0) return r;
+    }
     const bool col = G.w_order == JLB_COL_MAJOR;
     const int64_t mt = ceil_div(col ? G.N : G.K, kTile), nt = ceil_div(col ? G.K : G.N, kTile);
     if (mt > 65535 || G.E > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent too large");

@@ -43,6 +43,13 @@ struct Gradient {
     int64_t lddw, dw_stride;
 };
 
+// The tensor-core kernels (expert_mm_tc.cu): whether a call's operands suit
+// them, and the launch; -1 when the driver refuses a tensor map.
+bool tc_product_ok(const Product &P);
+int tc_product(cudaStream_t st, const Product &P);
+bool tc_gradient_ok(const Gradient &G);
+int tc_gradient(cudaStream_t st, const Gradient &G);
+
 // Rows [lo, hi) of group e, kept inside [0, S] whatever rowptr holds.
 __device__ __forceinline__ void group_rows(const int32_t *__restrict__ rowptr, int base, int64_t S,
                                            int64_t e, int &lo, int &hi) {
