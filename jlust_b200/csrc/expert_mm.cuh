@@ -73,39 +73,58 @@ __device__ __forceinline__ bool group_bad(const int32_t *__restrict__ rowptr, in
 }
 
 // ------------------------------------------------------------ activations
-// relu keeps NaN.  silu = z / (1 + e^-z); gelu = z (1 + erf(z / sqrt 2)) / 2.
-// For BF16 results (T) the exponential and the quotient are the fast ones:
-// their error, a few units of 2^-22, is far below the rounding to 8 bits.
-template <typename T>
-__device__ __forceinline__ float exp_of(float v) {
-    return sizeof(T) == 2 ? __expf(v) : expf(v);
-}
-template <typename T>
-__device__ __forceinline__ float quotient(float a, float b) {
-    return sizeof(T) == 2 ? a * __frcp_rn(b) : a / b;
+// relu keeps NaN.  silu = z / (1 + e^-z); gelu = z Phi(z), Phi(z) = (1 + erf(z /
+// sqrt 2)) / 2.  For F32 results they call expf and erff.  For BF16 results the
+// exponential, the quotient and Phi are cheaper: their errors (a few units of
+// 2^-22; 1e-7 for Phi) are far below the rounding to 8 bits.
+
+// Phi(z), and e = exp(-z^2 / 2) on the way: Abramowitz and Stegun 7.1.26,
+// erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), |error| < 1.5e-7,
+// with x = |z| / sqrt 2; the tail is taken as it is, not as 1 - erf.
+__device__ __forceinline__ float phi_fast(float z, float &e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    e = __expf(-x * x);
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    q = 0.5f * q * t * e;
+    return z < 0.0f ? q : 1.0f - q;
 }
 
 template <typename T>
 __device__ __forceinline__ float act_value(float z, int act) {
+    constexpr bool fast = sizeof(T) == 2;
     switch (act) {
         case JLB_ACT_RELU: return z < 0.0f ? 0.0f : z;
-        case JLB_ACT_SILU: return quotient<T>(z, 1.0f + exp_of<T>(-z));
-        case JLB_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case JLB_ACT_SILU: return fast ? __fdividef(z, 1.0f + __expf(-z)) : z / (1.0f + expf(-z));
+        case JLB_ACT_GELU: {
+            float e;
+            return fast ? z * phi_fast(z, e) : 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        }
         default: return z;
     }
 }
 
 template <typename T>
 __device__ __forceinline__ float act_slope(float z, int act) {
+    constexpr bool fast = sizeof(T) == 2;
     switch (act) {
         case JLB_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case JLB_ACT_SILU: {
-            const float s = quotient<T>(1.0f, 1.0f + exp_of<T>(-z));
+            const float s = fast ? __fdividef(1.0f, 1.0f + __expf(-z)) : 1.0f / (1.0f + expf(-z));
             return s * (1.0f + z * (1.0f - s));
         }
-        case JLB_ACT_GELU:
+        case JLB_ACT_GELU: {
+            if (fast) {
+                float e;
+                const float p = phi_fast(z, e);
+                return fmaf(z * 0.39894228040143268f, e, p);
+            }
             return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-                   z * (0.39894228040143268f * exp_of<T>(-0.5f * z * z));
+                   z * (0.39894228040143268f * expf(-0.5f * z * z));
+        }
         default: return 1.0f;
     }
 }

@@ -16,19 +16,24 @@
 // 32 KB a CTA for 64 of the inner dimension (512 tensor cycles at full rate:
 // 64 B a cycle, what the L2 delivers to an SM; one CTA alone would need 96).
 //
-// Lanes of D are neighbouring i, so the epilogue's plain stores of one column
-// are 64 contiguous bytes a warp whatever the leading dimension's alignment.
+// Epilogue.  A thread holds one lane (one i) of 32 columns: bias, activation
+// and residual work on 32 independent values.  The rounded results turn
+// through shared memory as pairs of columns, so that a thread then holds 8
+// neighbouring i of two rows and stores 16-byte vectors.
 //
-// Ragged sums.  The gradient's last 64-row step of a group must not see the
-// next group's rows (they may hold NaN): its rows are fetched by TMA row
-// gathers (four rows a copy) whose rows past the group lie past the matrix,
-// which TMA fills with zeros.  The same gathers fetch rows through `rows`.
+// Gathered rows and ragged sums.  Rows fetched through `rows`, and the
+// gradient's last 64-row step of a group, which must not see the next group's
+// rows (they may hold NaN), are copied by four loader warps: 16-byte cp.async
+// into the swizzled places a TMA box would fill, absent rows zero-filled.
+// (TMA row gathers, four rows a copy, ran at 88 cycles a copy: 2549 us for the
+// 8192 x 4096 x 16384 product against 1007 us without the gather.)
 //
 // Work split: a persistent grid of CTA pairs; pair c takes tiles c, c + G, ...
 // numbered group by group from rowptr on the device (each warp role walks 32
 // groups at a time), inside a group in column blocks of 8 tiles for L2 reuse.
-// Roles (192 threads): warp 0 copies, warp 1 of the leader issues products,
-// warps 2-5 read TMEM and store; two TMEM accumulators, so a tile's epilogue
+// Roles: warp 0 copies, warp 1 of the leader issues products, warps 2-9 read
+// TMEM and store, warps 10-13 (only in launches that need them) load rows and
+// warp 14 reports their stages to the leader; two TMEM accumulators, so a tile's epilogue
 // overlaps the next tile's products.  Every wait is bounded: on expiry the
 // device error word is raised and all roles leave.
 #include "expert_mm.cuh"
@@ -45,7 +50,13 @@ namespace emm {
 
 using namespace tc;
 
-constexpr int kTcThreads = 192;
+constexpr int kEpiWarps = 8;                            // two for each quarter of TMEM's lanes
+constexpr int kTcThreads = 64 + kEpiWarps * 32;         // without the loaders
+constexpr int kLoadWarp = 2 + kEpiWarps, kLoaders = 128;  // the loader warps
+constexpr int kForward = 32;                            // the warp that reports the loaders' stages
+constexpr int kPitch = 36;                              // words a pair of columns takes in the epilogue's turn
+constexpr int kAhead = 8;                               // gradient: stages of row indices read at a time
+constexpr uint32_t kTurnBytes = kEpiWarps * 16 * kPitch * 4;
 constexpr int kMaxStages = 10;
 constexpr uint32_t kABytes = 128 * 128;                 // 128 lanes x 64 inner, a CTA's half of A
 constexpr uint32_t kBox = 64 * 128;                     // 64 x 64 bf16
@@ -58,19 +69,23 @@ struct TcArgs {
     int64_t glimit;               // rows the gathered matrix has
     const int32_t *rowptr, *rows;
     int gather;                   // product: 1 = B's rows; gradient: 1 = A's, 2 = B's
-    int a_past, b_past;           // gradient: a row index past A's / B's matrix
+    int vec;                      // out, z and res allow 16-byte vectors
+    const __nv_bfloat16 *ga, *gb; // the operands' matrices, for the loader warps
+    int64_t lda, ldb_;
     const __nv_bfloat16 *bias, *res;
     int64_t ldb, ldr;
     __nv_bfloat16 *z, *out;
     int64_t ldz, ldo, out_stride;
     int stages, bn_max;
+    int a_pair, b_pair;           // mA / mB: both 64-wide boxes of an operand in one copy
 };
 
 // A pipeline stage: A's half and, in 32-row boxes, B's.
 __host__ __device__ inline uint32_t stage_size(int bn_max) { return kABytes + (uint32_t)((bn_max / 2 + 31) / 32) * 4096u; }
 
 struct TcCtl {
-    uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2], done;
+    int idx[kLoaders / 32][kAhead * 16];          // a loader warp's rows, -1: none
+    uint64_t full[kMaxStages], empty[kMaxStages], rows[kMaxStages], tfull[2], tempty[2], done;
     uint32_t tmem, fills;
     int abort;
 };
@@ -174,44 +189,104 @@ struct Walk {
     }
 };
 
-// One row index of a gather: its row, or one past the matrix (zeros) when the
-// row is outside it.
-__device__ __forceinline__ int gather_row(const TcArgs &P, int64_t p, int past, bool &bad) {
-    const int64_t r = (int64_t)__ldg(P.rows + p) - P.base;
-    if (r >= 0 && r < P.glimit) return (int)r;
-    bad = true;
-    return past;
+// cp.async of up to 16 bytes; the rest of the 16 is zeroed (bytes == 0: all).
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-template <int ACT>
-__device__ __forceinline__ void store_column(const TcArgs &P, float v, bool has_z, int64_t row, int64_t i, float r) {
-    if (has_z) P.z[row * P.ldz + i] = __float2bfloat16_rn(v);
-    v = act_value<__nv_bfloat16>(v, ACT) + r;
-    P.out[row * P.ldo + i] = __float2bfloat16_rn(v);
+// Bytes of the 16 at element `at` of a row of `cols` elements.
+__device__ __forceinline__ uint32_t bytes_at(int64_t at, int64_t cols) {
+    const int64_t left = cols - at;
+    return left >= 8 ? 16u : left > 0 ? (uint32_t)left * 2u : 0u;
 }
 
-// 32 columns of one lane: r[c] is column c0 + c.
-template <int ACT>
-__device__ __forceinline__ void store_chunk(const TcArgs &P, const uint32_t (&r)[32], float bias, int64_t row0, int n,
-                                            int64_t i) {
-    float add[32];
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Stores 32 columns of the warp's 32 lanes: v[c] = out[row0 + c][ib + lane],
+// columns c < n.
+__device__ __forceinline__ void store32(const float (&v)[32], uint32_t *turn, bool vec, __nv_bfloat16 *out,
+                                        int64_t ld, int64_t row0, int n, int64_t ib, int64_t I) {
+    const int lane = threadIdx.x % kWarp;
+    if (!vec) {                                   // 32 neighbouring values a store, no alignment needed
+        if (ib + lane < I) {
+            __nv_bfloat16 *o = out + row0 * ld + ib + lane;
 #pragma unroll
-    for (int c = 0; c < 32; ++c) add[c] = P.res && c < n ? __bfloat162float(P.res[(row0 + c) * P.ldr + i]) : 0.0f;
+            for (int c = 0; c < 32; ++c)
+                if (c < n) o[c * ld] = __float2bfloat16_rn(v[c]);
+        }
+        return;
+    }
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
-        if (c < n) store_column<ACT>(P, __uint_as_float(r[c]) + bias, P.z != nullptr, row0 + c, i, add[c]);
+    for (int c = 0; c < 16; ++c) turn[c * kPitch + lane] = pack2(v[2 * c], v[2 * c + 1]);
+    __syncwarp();
+    const int pr = lane / 4, oct = (lane % 4) * 8;
+    __nv_bfloat16 *o = out + (row0 + 2 * pr) * ld + ib + oct;
+    const uint32_t *w = turn + pr * kPitch + oct;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t a[8], lo[4], hi[4];
+        *reinterpret_cast<uint4 *>(a) = *reinterpret_cast<const uint4 *>(w + h * 8 * kPitch);
+        *reinterpret_cast<uint4 *>(a + 4) = *reinterpret_cast<const uint4 *>(w + h * 8 * kPitch + 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            lo[c] = __byte_perm(a[2 * c], a[2 * c + 1], 0x5410);
+            hi[c] = __byte_perm(a[2 * c], a[2 * c + 1], 0x7632);
+        }
+        const int c = 16 * h + 2 * pr;
+        if (c < n) *reinterpret_cast<uint4 *>(o + 16 * h * ld) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (c + 1 < n) *reinterpret_cast<uint4 *>(o + (16 * h + 1) * ld) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    }
+    __syncwarp();
+}
+
+// Every second 32-column chunk of the tile's columns [0, nj), from chunk
+// `first` on, of this warp's 32 lanes; column c is output row row0 + c.
+template <int ACT, bool GRAD>
+__device__ __forceinline__ void store_tile(const TcArgs &P, uint32_t taddr, uint32_t *turn, int first, int64_t row0,
+                                           int nj, int64_t ib, float bias, __nv_bfloat16 *out) {
+    const int64_t i = ib + threadIdx.x % kWarp;
+    const bool vec = P.vec && ib + 32 <= P.I;
+#pragma unroll 1
+    for (int c0 = first * 32; c0 < nj; c0 += 64) {
+        const int n = nj - c0;
+        uint32_t r[32];
+        __syncwarp();
+        JLB_TC_LD32(taddr + (uint32_t)c0, r);
+        wait_ld();
+        float v[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(r[c]) + (GRAD ? 0.0f : bias);
+        if (!GRAD) {
+            if (P.z) store32(v, turn, vec, P.z, P.ldz, row0 + c0, n, ib, P.I);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = act_value<__nv_bfloat16>(v[c], ACT);
+            if (P.res && i < P.I) {
+                const __nv_bfloat16 *q = P.res + (row0 + c0) * P.ldr + i;
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    if (c < n) v[c] += __bfloat162float(q[c * P.ldr]);
+            }
+        }
+        store32(v, turn, vec, out, P.ldo, row0 + c0, n, ib, P.I);
+    }
+    __syncwarp();
 }
 
 template <bool A_MN, bool GRAD>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads + kLoaders + kForward, 1)
 product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB,
-           const __grid_constant__ CUtensorMap mAg, const __grid_constant__ CUtensorMap mBg,
-           const __grid_constant__ TcArgs P) {
+           const __grid_constant__ CUtensorMap mBig, const __grid_constant__ TcArgs P) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t tiles_u32 = (raw + 1023u) & ~1023u;
     const uint32_t stage_bytes = stage_size(P.bn_max);
-    TcCtl *ctl = reinterpret_cast<TcCtl *>(smem_raw + (tiles_u32 - raw) + (size_t)P.stages * stage_bytes);
+    uint8_t *after = smem_raw + (tiles_u32 - raw) + (size_t)P.stages * stage_bytes;
+    uint32_t *turns = reinterpret_cast<uint32_t *>(after);
+    TcCtl *ctl = reinterpret_cast<TcCtl *>(after + kTurnBytes);
+    const bool loaders = blockDim.x > kTcThreads;
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     const uint32_t rank = cluster_rank();
     const int64_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
@@ -219,12 +294,13 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < P.stages; ++s) {
-            mbar_init(smem_u32(&ctl->full[s]), 1);
+            mbar_init(smem_u32(&ctl->full[s]), loaders ? 3 : 1);   // the leader's copies; both CTAs' rows
+            mbar_init(smem_u32(&ctl->rows[s]), kLoaders);
             mbar_init(smem_u32(&ctl->empty[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&ctl->tfull[b]), 1);
-            mbar_init(smem_u32(&ctl->tempty[b]), 8);      // four epilogue warps of each CTA
+            mbar_init(smem_u32(&ctl->tempty[b]), 2 * kEpiWarps);
         }
         mbar_init(smem_u32(&ctl->done), 1);
         ctl->abort = 0;
@@ -251,79 +327,58 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Tile T;
         for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
             const int a0 = T.i0 + (int)rank * 128;
-            if (!GRAD) {
-                const int bh = T.bn / 2, nkb = (int)((P.Kc + 63) / 64);
-                const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
-                int gi[4];
-                if (P.gather)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int64_t p = b0 + lane * 4 + q;
-                        gi[q] = lane * 4 + q < bh && p < T.hi ? gather_row(P, p, P.b_past, bad) : P.b_past;
-                    }
-                const int boxes = (bh + 31) / 32;
-                const uint32_t bytes = 2u * (kABytes + (P.gather ? (uint32_t)bh * 128u : (uint32_t)boxes * 4096u));
-                for (int kb = 0; kb < nkb; ++kb) {
-                    if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
+            const int nkb = GRAD ? (T.hi - T.lo + 63) / 64 : (int)((P.Kc + 63) / 64);
+            const int bh = T.bn / 2, boxes = (bh + 31) / 32;           // product: B's rows, in 32-row boxes
+            const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
+            const int nb = T.bn / 128, bj0 = T.j0 + (int)rank * bh;    // gradient: B's 64-column boxes
+            for (int kb = 0; lane == 0 && kb < nkb; ++kb) {
+                if (!tc_wait(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
+                {
                     const uint32_t sA = tiles_u32 + (uint32_t)stage * stage_bytes, sB = sA + kABytes;
                     const uint32_t full = full0 + (uint32_t)stage * 8u;
-                    if (lane == 0) {
-                        if (rank == 0) mbar_expect_tx(smem_u32(&ctl->full[stage]), bytes);
-                        if (A_MN) {
+                    if (!GRAD) {
+                        if (rank == 0)
+                            mbar_expect_tx(smem_u32(&ctl->full[stage]),
+                                           2u * (kABytes + (P.gather ? 0u : (uint32_t)boxes * 4096u)));
+                        if (!A_MN) {
+                            tma_3d(sA, &mA, full, kb * 64, a0, T.e);
+                        } else if (P.a_pair) {
+                            tma_4d(sA, &mA, full, 0, kb * 64, a0 / 64, T.e);
+                        } else {
                             tma_3d(sA, &mA, full, a0, kb * 64, T.e);
                             tma_3d(sA + kBox, &mA, full, a0 + 64, kb * 64, T.e);
-                        } else {
-                            tma_3d(sA, &mA, full, kb * 64, a0, T.e);
                         }
-                        if (!P.gather)
+                        if (boxes == 4 && !P.gather)
+                            tma_2d(sB, &mBig, full, kb * 64, (int)b0);
+                        else if (!P.gather)
                             for (int x = 0; x < boxes; ++x)
                                 tma_2d(sB + (uint32_t)x * 4096u, &mB, full, kb * 64, (int)b0 + 32 * x);
-                    }
-                    __syncwarp();
-                    if (P.gather && lane * 4 < bh) tma_gather4(sB + (uint32_t)lane * 512u, &mBg, full, kb * 64, gi);
-                    ++fills;
-                    if (++stage == P.stages) { stage = 0; pe ^= 1u; }
-                }
-            } else {
-                const int nb = T.bn / 128, rows = T.hi - T.lo, nkb = (rows + 63) / 64;
-                const int bj0 = T.j0 + (int)rank * (T.bn / 2);
-                const uint32_t bytes = 2u * (kABytes + (uint32_t)nb * kBox);
-                // lane l gathers rows 4*(l%16).. of the l/16-th 64-column box
-                const int box = lane / 16, r4 = (lane % 16) * 4;
-                for (int kb = 0; kb < nkb; ++kb) {
-                    const bool tail = rows - kb * 64 < 64;
-                    const bool ga = tail || P.gather == 1, gb = tail || P.gather == 2;
-                    const int64_t p0 = (int64_t)T.lo + kb * 64;
-                    int gia[4], gib[4];
-                    if (ga || gb)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int64_t p = p0 + r4 + q;
-                            const bool in = p < T.hi;
-                            gia[q] = !in ? P.a_past : P.gather == 1 ? gather_row(P, p, P.a_past, bad) : (int)p;
-                            gib[q] = !in ? P.b_past : P.gather == 2 ? gather_row(P, p, P.b_past, bad) : (int)p;
+                    } else {
+                        const bool tail = T.hi - T.lo - kb * 64 < 64;
+                        const bool ta = !tail && P.gather != 1, tb = !tail && P.gather != 2;
+                        const int p0 = T.lo + kb * 64;
+                        if (rank == 0)
+                            mbar_expect_tx(smem_u32(&ctl->full[stage]),
+                                           2u * ((ta ? kABytes : 0u) + (tb ? (uint32_t)nb * kBox : 0u)));
+                        if (rank == 0 && ta && tb)             // no rows to load: their arrivals
+                            mbar_arrive_count(smem_u32(&ctl->full[stage]), 2);
+                        if (ta && P.a_pair) {
+                            tma_3d(sA, &mA, full, 0, p0, a0 / 64);
+                        } else if (ta) {
+                            tma_2d(sA, &mA, full, a0, p0);
+                            tma_2d(sA + kBox, &mA, full, a0 + 64, p0);
                         }
-                    if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
-                    const uint32_t sA = tiles_u32 + (uint32_t)stage * stage_bytes, sB = sA + kABytes;
-                    const uint32_t full = full0 + (uint32_t)stage * 8u;
-                    if (lane == 0) {
-                        if (rank == 0) mbar_expect_tx(smem_u32(&ctl->full[stage]), bytes);
-                        if (!ga) {
-                            tma_2d(sA, &mA, full, a0, (int)p0);
-                            tma_2d(sA + kBox, &mA, full, a0 + 64, (int)p0);
-                        }
-                        if (!gb)
+                        if (tb && nb == 2 && P.b_pair)
+                            tma_3d(sB, &mBig, full, 0, p0, bj0 / 64);
+                        else if (tb)
                             for (int x = 0; x < nb; ++x)
-                                tma_2d(sB + (uint32_t)x * kBox, &mB, full, bj0 + 64 * x, (int)p0);
+                                tma_2d(sB + (uint32_t)x * kBox, &mB, full, bj0 + 64 * x, p0);
                     }
-                    __syncwarp();
-                    const uint32_t at = (uint32_t)box * kBox + (uint32_t)(lane % 16) * 512u;
-                    if (ga) tma_gather4(sA + at, &mAg, full, a0 + 64 * box, gia);
-                    if (gb && box < nb) tma_gather4(sB + at, &mBg, full, bj0 + 64 * box, gib);
-                    ++fills;
-                    if (++stage == P.stages) { stage = 0; pe ^= 1u; }
                 }
+                ++fills;
+                if (++stage == P.stages) { stage = 0; pe ^= 1u; }
             }
+            ok = __all_sync(0xffffffffu, ok);
         }
         if (bad) dev_error(DEV_ERR_BOUNDS);
         if (lane == 0) ctl->fills = fills;
@@ -345,37 +400,38 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 te[buf] ^= 1u;
                 fence_after();
                 const uint32_t idesc = instr_desc(256, (uint32_t)T.bn, A_MN, GRAD);
-                for (int kb = 0; kb < nkb; ++kb) {
-                    if (!tc_wait_warp(smem_u32(&ctl->full[stage]), pf, abort_flag)) { ok = false; break; }
-                    fence_after();
-                    if (lane == 0) {
-                        const uint64_t off = (uint64_t)(((uint32_t)stage * stage_bytes) >> 4);
-                        mma_pair_k64<A_MN ? 128u : 2u, GRAD ? 128u : 2u>(tmem + (uint32_t)buf * 256u, a_desc + off,
-                                                                        b_desc + off, idesc, kb > 0);
+                if (lane == 0)
+                    for (int kb = 0; kb < nkb; ++kb) {
+                        if (!tc_wait(smem_u32(&ctl->full[stage]), pf, abort_flag)) { ok = false; break; }
+                        fence_after();
+                        const uint32_t off = ((uint32_t)stage * stage_bytes) >> 4;
+                        mma_pair_k64<A_MN ? 128 : 2, GRAD ? 128 : 2>(tmem + (uint32_t)buf * 256u, (uint32_t)a_desc + off,
+                                                                     (uint32_t)(a_desc >> 32), (uint32_t)b_desc + off,
+                                                                     (uint32_t)(b_desc >> 32), idesc, (uint32_t)kb);
                         commit_pair(smem_u32(&ctl->empty[stage]));
-                        if (kb == nkb - 1) commit_pair(smem_u32(&ctl->tfull[buf]));
+                        if (++stage == P.stages) { stage = 0; pf ^= 1u; }
                     }
-                    __syncwarp();
-                    if (++stage == P.stages) { stage = 0; pf ^= 1u; }
-                }
+                if (lane == 0 && ok) commit_pair(smem_u32(&ctl->tfull[buf]));
+                ok = __all_sync(0xffffffffu, ok);
                 buf ^= 1;
             }
             if (lane == 0) commit_pair(smem_u32(&ctl->done));
             __syncwarp();
         }
-    } else {
+    } else if (warp < kLoadWarp) {
         // ----------------------------------------------------------- epilogue
         const int qd = warp & 3;
+        const int first = (warp - 2) / 4;                 // the 32-column chunks of this parity
+        uint32_t *turn = turns + (warp - 2) * 16 * kPitch;
         uint32_t tf[2] = {0u, 0u};
         int buf = 0;
-        bool ok = true;
         const uint32_t te0 = map_rank(smem_u32(&ctl->tempty[0]), 0);
         // rows of no group are zero
         if (!GRAD && P.rowptr) {
             int lo, hi;
             group_rows(P.rowptr, P.base, P.S, P.E - 1, lo, hi);
             for (int64_t r = (int64_t)hi + blockIdx.x; r < P.S; r += gridDim.x)
-                for (int64_t c = threadIdx.x - 64; c < P.I; c += 128) {
+                for (int64_t c = threadIdx.x - 64; c < P.I; c += kEpiWarps * 32) {
                     P.out[r * P.ldo + c] = __float2bfloat16_rn(0.0f);
                     if (P.z) P.z[r * P.ldz + c] = __float2bfloat16_rn(0.0f);
                 }
@@ -383,48 +439,193 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Walk<GRAD> walk;
         walk.init(P);
         Tile T;
-        for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
-            const int64_t i = (int64_t)T.i0 + rank * 128 + qd * 32 + lane;
-            const bool in = i < P.I;
+        for (int64_t t = pair; walk.find(P, t, T); t += pairs) {
+            const int64_t ib = (int64_t)T.i0 + rank * 128 + qd * 32;
             // column 0's row of the output, and its columns
             const int64_t row0 = GRAD ? T.j0 : (int64_t)T.lo + T.j0;
             const int nj = GRAD ? (int)min((int64_t)T.bn, P.J - T.j0) : min(T.bn, T.hi - T.lo - T.j0);
+            __nv_bfloat16 *out = P.out + (GRAD ? T.e * P.out_stride : 0);
             if (GRAD && T.hi == T.lo) {
-                if (in)
-                    for (int c = 0; c < nj; ++c)
-                        P.out[T.e * P.out_stride + (row0 + c) * P.ldo + i] = __float2bfloat16_rn(0.0f);
+                if (ib + lane < P.I)
+                    for (int c = first; c < nj; c += 2) out[(row0 + c) * P.ldo + ib + lane] = __float2bfloat16_rn(0.0f);
                 continue;
             }
-            const float bias = !GRAD && P.bias && in ? __bfloat162float(P.bias[T.e * P.ldb + i]) : 0.0f;
-            if (!tc_wait_warp(smem_u32(&ctl->tfull[buf]), tf[buf], abort_flag)) { ok = false; break; }
+            const float bias = !GRAD && P.bias && ib + lane < P.I ? __bfloat162float(P.bias[T.e * P.ldb + ib + lane]) : 0.0f;
+            if (!tc_wait_warp(smem_u32(&ctl->tfull[buf]), tf[buf], abort_flag)) break;
             tf[buf] ^= 1u;
             fence_after();
-#pragma unroll 1
-            for (int c0 = 0; c0 < nj; c0 += 32) {
-                uint32_t r[32];
-                __syncwarp();
-                JLB_TC_LD32(tmem + ((uint32_t)(qd * 32) << 16) + (uint32_t)(buf * 256 + c0), r);
-                wait_ld();
-                if (!in) continue;
-                const int n = nj - c0;
-                if (GRAD) {
-                    __nv_bfloat16 *o = P.out + T.e * P.out_stride + (row0 + c0) * P.ldo + i;
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (c < n) o[c * P.ldo] = __float2bfloat16_rn(__uint_as_float(r[c]));
-                } else {
-                    switch (P.act) {
-                        case JLB_ACT_RELU: store_chunk<JLB_ACT_RELU>(P, r, bias, row0 + c0, n, i); break;
-                        case JLB_ACT_SILU: store_chunk<JLB_ACT_SILU>(P, r, bias, row0 + c0, n, i); break;
-                        case JLB_ACT_GELU: store_chunk<JLB_ACT_GELU>(P, r, bias, row0 + c0, n, i); break;
-                        default: store_chunk<JLB_ACT_NONE>(P, r, bias, row0 + c0, n, i);
-                    }
+            const uint32_t taddr = tmem + ((uint32_t)(qd * 32) << 16) + (uint32_t)(buf * 256);
+            if (ib < P.I) {
+                switch (GRAD ? JLB_ACT_NONE : P.act) {
+                    case JLB_ACT_RELU: store_tile<JLB_ACT_RELU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
+                    case JLB_ACT_SILU: store_tile<JLB_ACT_SILU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
+                    case JLB_ACT_GELU: store_tile<JLB_ACT_GELU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
+                    default: store_tile<JLB_ACT_NONE, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out);
                 }
             }
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(te0 + (uint32_t)buf * 8u);
             buf ^= 1;
+        }
+    } else if (warp < kLoadWarp + kLoaders / 32) {
+        // ------------------------------------------------------ loader warps
+        // Loader warp w of the CTA copies rows w*4 + 16*n + lane/8 of a stage,
+        // 8 lanes a 128-byte piece; each thread's arrival on the CTA's rows
+        // barrier follows its copies' completion by itself, so every stage of
+        // the ring can have copies in flight.
+        const int lw = warp - kLoadWarp, sub = lane / 8, c8 = lane % 8;
+        // rows r = lw*4 + sub + 16*n of a box: r % 8, and so the swizzle, is the same for all n
+        const uint32_t at0 = (uint32_t)(lw * 4 + sub) * 128u + (uint32_t)((c8 ^ ((lw * 4 + sub) & 7)) * 16);
+        int stage = 0;
+        uint32_t pe = 1u;
+        bool ok = true, bad = false;
+        Walk<GRAD> walk;
+        walk.init(P);
+        Tile T;
+        for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
+            const int nkb = GRAD ? (T.hi - T.lo + 63) / 64 : (int)((P.Kc + 63) / 64);
+            const int bh = T.bn / 2, nb = T.bn / 128;
+            if (!GRAD) {
+                // the (at most 8) rows of B this lane copies 16 bytes of
+                const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
+                const __nv_bfloat16 *row[8];
+                uint32_t some = 0;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const int r = lw * 4 + n * 16 + sub;
+                    row[n] = P.gb;
+                    if (r < bh && b0 + r < T.hi) {
+                        const int64_t s = (int64_t)__ldg(P.rows + b0 + r) - P.base;
+                        if (s >= 0 && s < P.glimit) {
+                            row[n] = P.gb + s * P.ldb_ + c8 * 8;
+                            some |= 1u << n;
+                        } else {
+                            bad = true;
+                        }
+                    }
+                }
+                const int rows = (bh - lw * 4 + 15) / 16;       // bh is a multiple of 16: all lanes alike
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
+                    const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + kABytes + at0;
+                    const uint32_t bytes = bytes_at((int64_t)kb * 64 + c8 * 8, P.Kc);
+                    if (rows == 8) {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const uint32_t q = some >> n & 1u ? bytes : 0u;
+                            copy16(dst + (uint32_t)n * 2048u, q ? row[n] + kb * 64 : P.gb, q);
+                        }
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const uint32_t q = some >> n & 1u ? bytes : 0u;
+                            if (n < rows) copy16(dst + (uint32_t)n * 2048u, q ? row[n] + kb * 64 : P.gb, q);
+                        }
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->rows[stage]))
+                                 : "memory");
+                    if (++stage == P.stages) { stage = 0; pe ^= 1u; }
+                }
+                continue;
+            }
+            // gradient: rows lw*4 + sub + 16*n (n < 4) of every step, both operands
+            const int64_t ca = (int64_t)T.i0 + rank * 128 + c8 * 8, cb = (int64_t)T.j0 + rank * bh + c8 * 8;
+            const uint32_t qa[2] = {bytes_at(ca, P.I), bytes_at(ca + 64, P.I)};
+            const uint32_t qb[2] = {bytes_at(cb, P.J), nb == 2 ? bytes_at(cb + 64, P.J) : 0u};
+            int ahead[kAhead * 16 / kWarp];
+            // the warp's row indices of steps k0 .. k0 + kAhead - 1, -1 where none
+            auto fetch = [&](int k0) {
+#pragma unroll
+                for (int n = 0; n < kAhead * 16 / kWarp; ++n) {
+                    const int q = n * kWarp + lane, r = q % 16;
+                    const int64_t p = (int64_t)T.lo + (k0 + q / 16) * 64 + lw * 4 + (r / 4) * 16 + r % 4;
+                    ahead[n] = p < T.hi ? __ldg(P.rows + p) - P.base : -1;
+                    if (p < T.hi && (ahead[n] < 0 || ahead[n] >= P.glimit)) {
+                        bad = true;
+                        ahead[n] = -1;
+                    }
+                }
+            };
+            if (P.gather) fetch(0);
+            for (int kb = 0; kb < nkb; ++kb) {
+                // the indices of kAhead steps are kept in shared memory, the
+                // next ones' loads already on their way: a load in every step
+                // would wait for the step's copies before it
+                const bool tail = T.hi - T.lo - kb * 64 < 64;
+                const bool la = tail || P.gather == 1, lb = tail || P.gather == 2;
+                if (P.gather && kb % kAhead == 0) {
+                    __syncwarp();
+#pragma unroll
+                    for (int n = 0; n < kAhead * 16 / kWarp; ++n) ctl->idx[lw][n * kWarp + lane] = ahead[n];
+                    __syncwarp();
+                    if (kb + kAhead < nkb) fetch(kb + kAhead);
+                }
+                if (!la && !lb) {
+                    if (++stage == P.stages) { stage = 0; pe ^= 1u; }
+                    continue;
+                }
+                int sg[4], sp[4];                         // gathered and plain rows
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const int p = T.lo + kb * 64 + lw * 4 + n * 16 + sub;
+                    sp[n] = p < T.hi ? p : -1;
+                    sg[n] = P.gather ? ctl->idx[lw][(kb % kAhead) * 16 + n * 4 + sub] : sp[n];
+                }
+                if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
+                const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + at0;
+#pragma unroll
+                for (int op = 0; op < 2; ++op) {
+                    if (!(op ? lb : la)) continue;
+                    const __nv_bfloat16 *m = op ? P.gb : P.ga;
+                    const int64_t ld = op ? P.ldb_ : P.lda, col = op ? cb : ca;
+                    const bool g = P.gather == 1 + op;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const int sr = g ? sg[n] : sp[n];
+                        const __nv_bfloat16 *src = m + (int64_t)sr * ld + col;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t q = sr >= 0 ? (op ? qb[x] : qa[x]) : 0u;
+                            if (op == 0 || x < nb)
+                                copy16(dst + (op ? kABytes : 0u) + (uint32_t)x * kBox + (uint32_t)n * 2048u,
+                                       q ? src + 64 * x : m, q);
+                        }
+                    }
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->rows[stage]))
+                             : "memory");
+                if (++stage == P.stages) { stage = 0; pe ^= 1u; }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (bad) dev_error(DEV_ERR_BOUNDS);
+    } else {
+        // ------------------------------------------------- the loaders' report
+        // A stage whose rows have landed: the copies (generic proxy) are made
+        // visible to the tensor cores' reads (async proxy), then the leader's
+        // barrier gets this CTA's arrival.
+        const uint32_t full0 = map_rank(smem_u32(&ctl->full[0]), 0);
+        int stage = 0;
+        uint32_t pr = 0;                          // the phase of each stage's rows barrier, a bit each
+        bool ok = true;
+        Walk<GRAD> walk;
+        walk.init(P);
+        Tile T;
+        for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
+            const int nkb = GRAD ? (T.hi - T.lo + 63) / 64 : (int)((P.Kc + 63) / 64);
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (!GRAD || P.gather || T.hi - T.lo - kb * 64 < 64) {
+                    if (!tc_wait_warp(smem_u32(&ctl->rows[stage]), (pr >> stage) & 1u, abort_flag)) { ok = false; break; }
+                    pr ^= 1u << stage;
+                    if (lane == 0) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        mbar_arrive_cluster(full0 + (uint32_t)stage * 8u);
+                    }
+                    __syncwarp();
+                }
+                if (++stage == P.stages) stage = 0;
+            }
         }
     }
 
@@ -458,18 +659,34 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
+static bool encode(CUtensorMap *m, const void *p, int rank, const cuuint64_t *dims, const cuuint64_t *strides,
+                   const cuuint32_t *box) {
+    auto fn = encode_fn();
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(p), dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // rows x cols (x experts) of bf16 as {cols, rows[, experts]}, box {64, box_rows}.
 static bool make_map(CUtensorMap *m, const void *p, int64_t cols, int64_t rows, int64_t ld, int64_t experts,
                      int64_t stride, int box_rows) {
-    auto fn = encode_fn();
-    if (!fn) return false;
-    const int rank = experts > 0 ? 3 : 2;
-    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)experts};
-    cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)stride * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(p), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)experts};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    return encode(m, p, experts > 0 ? 3 : 2, dims, strides, box);
+}
+
+// The same matrices as {64, rows, cols / 64[, experts]}, so that one copy of
+// box {64, 64, 2} brings two neighbouring 64-column boxes, stacked.  Only for
+// cols a multiple of 64: the last box would otherwise leave its row.
+static bool make_pair_map(CUtensorMap *m, const void *p, int64_t cols, int64_t rows, int64_t ld, int64_t experts,
+                          int64_t stride) {
+    if (cols % 64) return false;
+    const cuuint64_t dims[4] = {64, (cuuint64_t)rows, (cuuint64_t)(cols / 64), (cuuint64_t)experts};
+    const cuuint64_t strides[3] = {(cuuint64_t)ld * 2, 128, (cuuint64_t)stride * 2};
+    const cuuint32_t box[4] = {64, 64, 2, 1};
+    return encode(m, p, experts > 0 ? 4 : 3, dims, strides, box);
 }
 
 static bool tma_matrix(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
@@ -495,17 +712,17 @@ static int device_sms() {
 }
 
 template <bool A_MN, bool GRAD>
-static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &ag,
-                     const CUtensorMap &bg, TcArgs &P, int64_t tiles) {
+static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &big, TcArgs &P, int64_t tiles,
+                     bool loaders) {
     const uint32_t stage = stage_size(P.bn_max);
-    const size_t extra = 1024 + sizeof(TcCtl);
+    const size_t extra = 1024 + kTurnBytes + sizeof(TcCtl);
     P.stages = (int)((227 * 1024 - extra) / stage);
     if (P.stages > kMaxStages) P.stages = kMaxStages;
     const size_t smem = (size_t)P.stages * stage + extra;
     JLB_CUDA(cudaFuncSetAttribute(product_tc<A_MN, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     int64_t pairs = device_sms() / 2;
     if (tiles < pairs) pairs = tiles;
-    product_tc<A_MN, GRAD><<<(unsigned)(2 * pairs), kTcThreads, smem, st>>>(a, b, ag, bg, P);
+    product_tc<A_MN, GRAD><<<(unsigned)(2 * pairs), kTcThreads + (loaders ? kLoaders + kForward : 0), smem, st>>>(a, b, big, P);
     JLB_LAUNCH_CHECK("product_tc");
     return ok();
 }
@@ -513,13 +730,13 @@ static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b
 // Status, or -1 when the driver refuses a tensor map (the caller takes
 // another kernel).
 int tc_product(cudaStream_t st, const Product &p) {
-    CUtensorMap a, b, bg;
+    CUtensorMap a, b, big;
     const bool mn = p.w_order == JLB_ROW_MAJOR;
     const int64_t ws = p.E > 1 ? p.w_stride : (mn ? p.K : p.N) * p.ldw;
-    if (!(mn ? make_map(&a, p.w, p.N, p.K, p.ldw, p.E, ws, 64) : make_map(&a, p.w, p.K, p.N, p.ldw, p.E, ws, 128)) ||
-        !make_map(&b, p.x, p.K, p.T, p.ldx, 0, 0, 32) || (p.rows && !make_map(&bg, p.x, p.K, p.T, p.ldx, 0, 0, 1)))
+    const bool pair = mn && make_pair_map(&a, p.w, p.N, p.K, p.ldw, p.E, ws);
+    if (!pair && !(mn ? make_map(&a, p.w, p.N, p.K, p.ldw, p.E, ws, 64) : make_map(&a, p.w, p.K, p.N, p.ldw, p.E, ws, 128)))
         return -1;
-    if (!p.rows) bg = b;
+    if (!make_map(&b, p.x, p.K, p.T, p.ldx, 0, 0, 32) || !make_map(&big, p.x, p.K, p.T, p.ldx, 0, 0, 128)) return -1;
     TcArgs P{};
     P.base = p.base;
     P.act = p.act;
@@ -531,7 +748,9 @@ int tc_product(cudaStream_t st, const Product &p) {
     P.rowptr = p.rowptr;
     P.rows = p.rows;
     P.gather = p.rows ? 1 : 0;
-    P.b_past = (int)p.T;
+    P.a_pair = pair;
+    P.gb = (const __nv_bfloat16 *)p.x;
+    P.ldb_ = p.ldx;
     P.bias = (const __nv_bfloat16 *)p.bias;
     P.ldb = p.ldb;
     P.res = (const __nv_bfloat16 *)p.res;
@@ -540,37 +759,47 @@ int tc_product(cudaStream_t st, const Product &p) {
     P.ldz = p.ldz;
     P.out = (__nv_bfloat16 *)p.y;
     P.ldo = p.ldy;
+    P.vec = tma_matrix(p.y, p.ldy) && (!p.z || tma_matrix(p.z, p.ldz)) && (!p.res || tma_matrix(p.res, p.ldr));
     P.bn_max = p.S >= 256 ? 256 : (int)((p.S + 31) / 32 * 32);
     const int64_t cols = ceil_div(p.S, P.bn_max) + (p.rowptr ? (p.E < p.S ? p.E : p.S) : 0);
     const int64_t tiles = cols * ceil_div(p.N, 256);
-    return mn ? launch_tc<true, false>(st, a, b, a, bg, P, tiles) : launch_tc<false, false>(st, a, b, a, bg, P, tiles);
+    return mn ? launch_tc<true, false>(st, a, b, big, P, tiles, p.rows)
+              : launch_tc<false, false>(st, a, b, big, P, tiles, p.rows);
 }
 
 int tc_gradient(cudaStream_t st, const Gradient &g) {
     // dw row-major: lanes = columns n (dz), columns = k (x); column-major: exchanged
     const bool row = g.w_order == JLB_ROW_MAJOR;
-    CUtensorMap x, xg, d, dg;
-    if (!make_map(&x, g.x, g.K, g.T, g.ldx, 0, 0, 64) || !make_map(&xg, g.x, g.K, g.T, g.ldx, 0, 0, 1) ||
-        !make_map(&d, g.dz, g.N, g.S, g.lddz, 0, 0, 64) || !make_map(&dg, g.dz, g.N, g.S, g.lddz, 0, 0, 1))
-        return -1;
+    const void *ap = row ? g.dz : g.x, *bp = row ? g.x : g.dz;
+    const int64_t ac = row ? g.N : g.K, ar = row ? g.S : g.T, lda = row ? g.lddz : g.ldx;
+    const int64_t bc = row ? g.K : g.N, br = row ? g.T : g.S, ldb = row ? g.ldx : g.lddz;
+    CUtensorMap a, b, big;
+    const bool a_pair = make_pair_map(&a, ap, ac, ar, lda, 0, 0), b_pair = make_pair_map(&big, bp, bc, br, ldb, 0, 0);
+    if ((!a_pair && !make_map(&a, ap, ac, ar, lda, 0, 0, 64)) || !make_map(&b, bp, bc, br, ldb, 0, 0, 64)) return -1;
+    if (!b_pair) big = b;
     TcArgs P{};
     P.base = g.base;
     P.E = g.E;
     P.S = g.S;
-    P.I = row ? g.N : g.K;
-    P.J = row ? g.K : g.N;
+    P.I = ac;
+    P.J = bc;
+    P.a_pair = a_pair;
+    P.b_pair = b_pair;
     P.glimit = g.T;
     P.rowptr = g.rowptr;
     P.rows = g.rows;
     P.gather = g.rows ? (row ? 2 : 1) : 0;
-    P.a_past = (int)(row ? g.S : g.T);
-    P.b_past = (int)(row ? g.T : g.S);
+    P.ga = (const __nv_bfloat16 *)ap;
+    P.lda = lda;
+    P.gb = (const __nv_bfloat16 *)bp;
+    P.ldb_ = ldb;
+    P.vec = tma_matrix(g.dw, g.lddw) && (g.E == 1 || g.dw_stride % 8 == 0);
     P.out = (__nv_bfloat16 *)g.dw;
     P.ldo = g.lddw;
     P.out_stride = g.dw_stride;
     P.bn_max = P.J > 128 ? 256 : 128;
     const int64_t tiles = g.E * ceil_div(P.I, 256) * ceil_div(P.J, 256);
-    return row ? launch_tc<true, true>(st, d, x, dg, xg, P, tiles) : launch_tc<true, true>(st, x, d, xg, dg, P, tiles);
+    return launch_tc<true, true>(st, a, b, big, P, tiles, true);
 }
 
 }  // namespace emm

@@ -1,5 +1,5 @@
 // tcgen05.cuh -- PTX glue of the paired-CTA tensor-core kernels: mbarriers in
-// a cluster of two, TMA tile and gather copies that signal the leader's
+// a cluster of two, TMA tile copies that signal the leader's
 // barrier, tcgen05 allocation, products and commits with cta_group::2.
 #pragma once
 
@@ -33,15 +33,22 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
 }
+// `count` arrivals on a barrier of this CTA.
+__device__ __forceinline__ void mbar_arrive_count(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
 // Arrives on a barrier of any CTA of the cluster (shared::cluster address).
+// What it reports is done and fenced before (TMEM reads by tcgen05.fence, row
+// copies by a proxy fence), so the default CTA-scope release is enough; a
+// cluster-scope release took about 1 us an arrival here.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
         : "r"(bar), "r"(parity)
@@ -62,13 +69,10 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const void *map, uint32_t b
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
-}
-// Four rows r of a matrix, each the map's one-row box wide, from column x.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const void *map, uint32_t bar, int x, const int (&r)[4]) {
+}__device__ __forceinline__ void tma_4d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z, int w) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4"
-        ".mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 
@@ -104,17 +108,28 @@ __device__ __forceinline__ uint32_t instr_desc(uint32_t m, uint32_t n, bool a_mn
            ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-// Four products of 16 inner elements each; the descriptors' address words
-// advance by a_step and b_step (16-byte units).  first == 0 overwrites D.
-template <uint32_t A_STEP, uint32_t B_STEP>
-__device__ __forceinline__ void mma_pair_k64(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t first) {
-#pragma unroll
-    for (uint32_t s = 0; s < 4; ++s)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a + s * A_STEP), "l"(b + s * B_STEP), "r"(idesc), "r"(s == 0 ? first : 1u)
-            : "memory");
+// Four products of 16 inner elements each, from one asm block: the
+// descriptors' low (address) words advance by a_step and b_step (16-byte
+// units, no carry: addresses stay below 256 KB).  first == 0 overwrites D.
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ void mma_pair_k64(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                             uint32_t idesc, uint32_t first) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t.reg .b32 t, u;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, p;\n\t"
+        "add.u32 t, %1, %7;\n\tadd.u32 u, %3, %8;\n\t"
+        "mov.b64 a, {t, %2};\n\tmov.b64 b, {u, %4};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t"
+        "add.u32 t, t, %7;\n\tadd.u32 u, u, %8;\n\t"
+        "mov.b64 a, {t, %2};\n\tmov.b64 b, {u, %4};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t"
+        "add.u32 t, t, %7;\n\tadd.u32 u, u, %8;\n\t"
+        "mov.b64 a, {t, %2};\n\tmov.b64 b, {u, %4};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(first), "r"(idesc), "n"(A_STEP), "n"(B_STEP)
+        : "memory");
 }
 
 #define JLB_TC_LD32(taddr, r)                                                                \
