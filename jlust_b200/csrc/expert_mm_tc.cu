@@ -85,7 +85,8 @@ __host__ __device__ inline uint32_t stage_size(int bn_max) { return kABytes + (u
 
 struct TcCtl {
     int idx[kLoaders / 32][kAhead * 16];          // a loader warp's rows, -1: none
-    uint64_t full[kMaxStages], empty[kMaxStages], rows[kMaxStages], tfull[2], tempty[2], done;
+    uint64_t full[kMaxStages], empty[kMaxStages], rows[kMaxStages], go[kMaxStages];
+    uint64_t tfull[2], tempty[2], done;
     uint32_t tmem, fills;
     int abort;
 };
@@ -296,6 +297,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         for (int s = 0; s < P.stages; ++s) {
             mbar_init(smem_u32(&ctl->full[s]), loaders ? 3 : 1);   // the leader's copies; both CTAs' rows
             mbar_init(smem_u32(&ctl->rows[s]), kLoaders);
+            mbar_init(smem_u32(&ctl->go[s]), 1);
             mbar_init(smem_u32(&ctl->empty[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -362,6 +364,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                                            2u * ((ta ? kABytes : 0u) + (tb ? (uint32_t)nb * kBox : 0u)));
                         if (rank == 0 && ta && tb)             // no rows to load: their arrivals
                             mbar_arrive_count(smem_u32(&ctl->full[stage]), 2);
+                        if (tail && !P.gather) mbar_arrive_count(smem_u32(&ctl->go[stage]), 1);
                         if (ta && P.a_pair) {
                             tma_3d(sA, &mA, full, 0, p0, a0 / 64);
                         } else if (ta) {
@@ -380,6 +383,17 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             }
             ok = __all_sync(0xffffffffu, ok);
         }
+        // every stage's last release has arrived: none can reach this CTA later
+        if (lane == 0)
+            for (uint32_t n = 0; ok && n < (uint32_t)P.stages && n < fills; ++n) {
+                if (fills < (uint32_t)P.stages) {
+                    ok = tc_wait(smem_u32(&ctl->empty[n]), 0u, abort_flag);
+                } else {
+                    ok = tc_wait(smem_u32(&ctl->empty[stage]), pe, abort_flag);
+                    if (++stage == P.stages) { stage = 0; pe ^= 1u; }
+                }
+            }
+        __syncwarp();
         if (bad) dev_error(DEV_ERR_BOUNDS);
         if (lane == 0) ctl->fills = fills;
     } else if (warp == 1) {
@@ -478,7 +492,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         // rows r = lw*4 + sub + 16*n of a box: r % 8, and so the swizzle, is the same for all n
         const uint32_t at0 = (uint32_t)(lw * 4 + sub) * 128u + (uint32_t)((c8 ^ ((lw * 4 + sub) & 7)) * 16);
         int stage = 0;
-        uint32_t pe = 1u;
+        uint32_t pe = 1u, pgo = 0u;
         bool ok = true, bad = false;
         Walk<GRAD> walk;
         walk.init(P);
@@ -549,6 +563,9 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             };
             if (P.gather) fetch(0);
             for (int kb = 0; kb < nkb; ++kb) {
+                // (without gather only a group's last step is loaded; the copy
+                // thread, which waits for every stage, says when: a wait for
+                // the stage's own barrier could be laps of the ring early)
                 // the indices of kAhead steps are kept in shared memory, the
                 // next ones' loads already on their way: a load in every step
                 // would wait for the step's copies before it
@@ -572,7 +589,12 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                     sp[n] = p < T.hi ? p : -1;
                     sg[n] = P.gather ? ctl->idx[lw][(kb % kAhead) * 16 + n * 4 + sub] : sp[n];
                 }
-                if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
+                if (!(P.gather ? tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)
+                               : tc_wait_warp(smem_u32(&ctl->go[stage]), pgo >> stage & 1u, abort_flag))) {
+                    ok = false;
+                    break;
+                }
+                pgo ^= 1u << stage;               // a bit a stage: its next go comes after its release
                 const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + at0;
 #pragma unroll
                 for (int op = 0; op < 2; ++op) {

@@ -130,7 +130,7 @@ def test_combine_strided_and_in_place_buffers():
 GROUPS = {
     "one_row": [1], "decode": [1, 0, 2, 1, 0, 0, 3, 1], "few": [5, 0, 7, 12, 33, 0],
     "mid": [100, 3, 0, 260, 31, 65], "long": [513, 0, 1, 700], "all_empty": [0, 0, 0],
-    "many_experts": [(i * 7) % 5 for i in range(70)],
+    "many_steps": [1601, 70, 0, 900, 64], "many_experts": [(i * 7) % 5 for i in range(70)],
 }
 
 
@@ -184,6 +184,8 @@ def test_grouped(dtype, order, groups, K, N, name, base, tail, gather):
     ("long", 256, 384, "gelu", 0, 0, False),
     ("all_empty", 32, 48, "relu", 0, 4, False),
     ("many_experts", 64, 72, None, 0, 0, True),
+    ("many_steps", 128, 136, None, 0, 0, False),
+    ("many_steps", 72, 264, "silu", 0, 5, True),
 ])
 def test_grouped_backward(dtype, order, groups, K, N, name, base, tail, gather):
     sizes = GROUPS[groups]
