@@ -65,6 +65,7 @@ int take_dev_error_spgemm();
 int take_dev_error_routing();
 int take_dev_error_emm();
 int take_dev_error_emm_tc();
+int take_dev_error_emm_skinny();
 
 #define JLB_DEFINE_DEV_ERROR(unit)                                           \
     static __device__ int g_dev_error;                                       \

@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kSimtThreads) product_simt(const Product P) {
             if (P.bias) v += to_f32(((const T *)P.bias)[f.e * P.ldb + n]);
             if (P.z) ((T *)P.z)[r * P.ldz + n] = from_f32<T>(v);
             v = act_value<T>(v, P.act);
-            if (P.res) v += to_f32(((const T *)P.res)[r * P.ldr + n]);
+            if (P.res) v = add_rn(v, to_f32(((const T *)P.res)[r * P.ldr + n]));
             ((T *)P.y)[r * P.ldy + n] = from_f32<T>(v);
         }
     }
@@ -311,9 +311,91 @@ static int check_act(int act) {
                : JLB_OK;
 }
 
-static int run_product(cudaStream_t st, const Product &P) {
-    if (tc_product_ok(P)) {
-        const int r = tc_product(st, P);
+// ------------------------------------------------- copies for the tensor path
+// Rows of bf16 whose leading dimension or address TMA cannot take, copied to a
+// leading dimension of a multiple of 8: a warp moves 256 neighbouring elements
+// of a row, 64 bytes a load whatever the alignment.
+__global__ void __launch_bounds__(256)
+align_rows(int64_t experts, int64_t rows, int64_t cols, const uint16_t *__restrict__ src, int64_t ld,
+           int64_t stride, uint16_t *__restrict__ dst, int64_t ldd) {
+    const int64_t pieces = (cols + 255) / 256, all = experts * rows * pieces;
+    const int lane = threadIdx.x % kWarp;
+    for (int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / kWarp; w < all; w += (int64_t)gridDim.x * 8) {
+        const int64_t r = w / pieces, c0 = (w - r * pieces) * 256 + lane;
+        const int64_t e = r / rows;
+        const uint16_t *s = src + e * stride + (r - e * rows) * ld;
+        uint16_t *d = dst + r * ldd;
+        uint16_t v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = c0 + q * 32 < cols ? s[c0 + q * 32] : (uint16_t)0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (c0 + q * 32 < cols) d[c0 + q * 32] = v[q];
+    }
+}
+
+static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+static size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
+static bool tma_rows(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+static int align_copy(cudaStream_t st, int64_t experts, int64_t rows, int64_t cols, const void *src, int64_t ld,
+                      int64_t stride, void *dst) {
+    const int64_t warps = experts * rows * ceil_div(cols, 256), blocks = ceil_div(warps, 8);
+    align_rows<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(
+        experts, rows, cols, (const uint16_t *)src, ld, stride, (uint16_t *)dst, pad8(cols));
+    JLB_LAUNCH_CHECK("align_rows");
+    return JLB_OK;
+}
+
+// The tensor path of a product: which operands need an aligned copy, and
+// where the workspace holds them (parts of split tiles first).
+struct ProductPlan {
+    bool tc, copy_x, copy_w;
+    size_t x_at, w_at, bytes;
+    Product p;              // with the copies' leading dimensions
+};
+static ProductPlan plan_product(const Product &P) {
+    ProductPlan q{};
+    q.p = P;
+    if (P.dtype != JLB_BF16 || P.K == 0 || P.N == 0 || P.S == 0 || P.T == 0 || P.E == 0 || skinny_ok(P)) return q;
+    const int64_t inner = P.w_order == JLB_ROW_MAJOR ? P.N : P.K, outer = P.w_order == JLB_ROW_MAJOR ? P.K : P.N;
+    q.tc = true;
+    q.copy_x = !tma_rows(P.x, P.ldx);
+    q.copy_w = !tma_rows(P.w, P.ldw) || (P.E > 1 && P.w_stride % 8);
+    q.bytes = pad256(tc_product_workspace(P));
+    if (q.copy_x) {
+        q.x_at = q.bytes;
+        q.bytes += pad256((size_t)P.T * pad8(P.K) * 2);
+        q.p.ldx = pad8(P.K);
+    }
+    if (q.copy_w) {
+        q.w_at = q.bytes;
+        q.bytes += pad256((size_t)P.E * outer * pad8(inner) * 2);
+        q.p.ldw = pad8(inner);
+        q.p.w_stride = outer * pad8(inner);
+    }
+    return q;
+}
+
+static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_bytes) {
+    if (skinny_ok(P) && P.T > 0) return skinny_product(st, P);
+    ProductPlan q = plan_product(P);
+    if (q.tc) {
+        if (q.bytes && (!ws || ws_bytes < q.bytes))
+            return fail(JLB_ERR_WORKSPACE, "the product needs %zu workspace bytes", q.bytes);
+        if (q.copy_x) {
+            q.p.x = (char *)ws + q.x_at;
+            const int r = align_copy(st, 1, P.T, P.K, P.x, P.ldx, 0, (char *)ws + q.x_at);
+            if (r) return r;
+        }
+        if (q.copy_w) {
+            const bool row = P.w_order == JLB_ROW_MAJOR;
+            q.p.w = (char *)ws + q.w_at;
+            const int r = align_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride,
+                                     (char *)ws + q.w_at);
+            if (r) return r;
+        }
+        const int r = tc_product(st, q.p, ws);
         if (r >= 0) return r;
     }
     const int64_t ntiles = ceil_div(P.N, kTile), rtiles = row_tiles_bound(P.E, P.S, P.rowptr, kTile);
@@ -325,9 +407,48 @@ static int run_product(cudaStream_t st, const Product &P) {
     return ok();
 }
 
-static int run_gradient(cudaStream_t st, const Gradient &G) {
-    if (tc_gradient_ok(G)) {
-        const int r = tc_gradient(st, G);
+struct GradientPlan {
+    bool tc, copy_x, copy_d;
+    size_t x_at, d_at, bytes;
+    Gradient g;
+};
+static GradientPlan plan_gradient(const Gradient &G) {
+    GradientPlan q{};
+    q.g = G;
+    if (G.dtype != JLB_BF16 || G.S == 0 || G.T == 0 || G.E == 0 || G.K == 0 || G.N == 0) return q;
+    q.tc = true;
+    q.copy_x = !tma_rows(G.x, G.ldx);
+    q.copy_d = !tma_rows(G.dz, G.lddz);
+    q.bytes = pad256(tc_gradient_workspace(G));
+    if (q.copy_x) {
+        q.x_at = q.bytes;
+        q.bytes += pad256((size_t)G.T * pad8(G.K) * 2);
+        q.g.ldx = pad8(G.K);
+    }
+    if (q.copy_d) {
+        q.d_at = q.bytes;
+        q.bytes += pad256((size_t)G.S * pad8(G.N) * 2);
+        q.g.lddz = pad8(G.N);
+    }
+    return q;
+}
+
+static int run_gradient(cudaStream_t st, const Gradient &G, void *ws, size_t ws_bytes) {
+    GradientPlan q = plan_gradient(G);
+    if (q.tc) {
+        if (q.bytes && (!ws || ws_bytes < q.bytes))
+            return fail(JLB_ERR_WORKSPACE, "the gradient needs %zu workspace bytes", q.bytes);
+        if (q.copy_x) {
+            q.g.x = (char *)ws + q.x_at;
+            const int r = align_copy(st, 1, G.T, G.K, G.x, G.ldx, 0, (char *)ws + q.x_at);
+            if (r) return r;
+        }
+        if (q.copy_d) {
+            q.g.dz = (char *)ws + q.d_at;
+            const int r = align_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, (char *)ws + q.d_at);
+            if (r) return r;
+        }
+        const int r = tc_gradient(st, q.g, ws);
         if (r >= 0) return r;
     }
     const bool col = G.w_order == JLB_COL_MAJOR;
@@ -404,8 +525,19 @@ extern "C" JLB_API int jlb_mm_plan_destroy(jlb_mm_plan plan) {
 
 extern "C" JLB_API size_t jlb_mm_plan_workspace_size(jlb_mm_plan plan, int64_t S, int64_t T,
                                                      const void *x, int64_t ldx, int gather) {
-    (void)plan; (void)S; (void)T; (void)x; (void)ldx; (void)gather;
-    return 0;
+    if (!plan) return 0;
+    emm::Product P = plan->p;
+    P.S = S;
+    P.T = T;
+    P.x = x;
+    P.ldx = ldx;
+    (void)gather;
+    // with and without a row pointer, which is not known here: the larger
+    static const int32_t some = 0;
+    const size_t dense = P.E == 1 ? emm::plan_product(P).bytes : 0;
+    P.rowptr = &some;
+    const size_t ragged = emm::plan_product(P).bytes;
+    return dense > ragged ? dense : ragged;
 }
 
 extern "C" JLB_API int jlb_mm_plan_execute(jlb_mm_plan plan, void *stream, int64_t S, int64_t T,
@@ -413,7 +545,6 @@ extern "C" JLB_API int jlb_mm_plan_execute(jlb_mm_plan plan, void *stream, int64
                                            const void *x, int64_t ldx, const void *res,
                                            int64_t ldr, void *z, int64_t ldz, void *y, int64_t ldy,
                                            void *workspace, size_t workspace_bytes) {
-    (void)workspace; (void)workspace_bytes;
     if (!plan) return fail(JLB_ERR_INVALID_ARGUMENT, "null plan");
     emm::Product P = plan->p;
     P.S = S;
@@ -431,7 +562,7 @@ extern "C" JLB_API int jlb_mm_plan_execute(jlb_mm_plan plan, void *stream, int64
     const int r = emm::check_call(P);
     if (r) return r;
     if (S == 0 || P.N == 0) return ok();
-    return emm::run_product(as_stream(stream), P);
+    return emm::run_product(as_stream(stream), P, workspace, workspace_bytes);
 }
 
 extern "C" JLB_API size_t jlb_grouped_mm_workspace_size(int dtype, int64_t E, int64_t S, int64_t T,
@@ -472,9 +603,21 @@ extern "C" JLB_API size_t jlb_grouped_mm_wgrad_workspace_size(int dtype, int64_t
                                                               const void *x, int64_t ldx,
                                                               const void *dz, int64_t lddz,
                                                               int w_order, int gather) {
-    (void)dtype; (void)E; (void)S; (void)T; (void)K; (void)N; (void)x; (void)ldx; (void)dz;
-    (void)lddz; (void)w_order; (void)gather;
-    return 0;
+    (void)gather;
+    if (E < 0 || S < 0 || T < 0 || K < 0 || N < 0) return 0;
+    emm::Gradient G{};
+    G.dtype = dtype;
+    G.E = E;
+    G.S = S;
+    G.T = T;
+    G.K = K;
+    G.N = N;
+    G.x = x;
+    G.ldx = ldx;
+    G.dz = dz;
+    G.lddz = lddz;
+    G.w_order = w_order;
+    return emm::plan_gradient(G).bytes;
 }
 
 extern "C" JLB_API int jlb_grouped_mm_wgrad(void *stream, int dtype, int idx_base, int64_t E,
@@ -484,7 +627,6 @@ extern "C" JLB_API int jlb_grouped_mm_wgrad(void *stream, int dtype, int idx_bas
                                             int64_t lddz, void *dw, int64_t lddw,
                                             int64_t dw_stride, int w_order, void *workspace,
                                             size_t workspace_bytes) {
-    (void)workspace; (void)workspace_bytes;
     int r = emm::check_types(dtype, idx_base);
     if (!r) r = emm::check_extents(E, S, T, K, N, rowptr, rows);
     if (!r) r = emm::check_weight(w_order, E, K, N, lddw, dw_stride);
@@ -495,7 +637,7 @@ extern "C" JLB_API int jlb_grouped_mm_wgrad(void *stream, int dtype, int idx_bas
     if (!dw || (S > 0 && (!dz || (T > 0 && !x)))) return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
     const emm::Gradient G{dtype, idx_base, w_order, E, S, T, K, N, rowptr, rows,
                           x, ldx, dz, lddz, dw, lddw, dw_stride};
-    return emm::run_gradient(as_stream(stream), G);
+    return emm::run_gradient(as_stream(stream), G, workspace, workspace_bytes);
 }
 
 extern "C" JLB_API size_t jlb_act_backward_workspace_size(int64_t E, int64_t S, int64_t N,

@@ -43,12 +43,18 @@ struct Gradient {
     int64_t lddw, dw_stride;
 };
 
-// The tensor-core kernels (expert_mm_tc.cu): whether a call's operands suit
-// them, and the launch; -1 when the driver refuses a tensor map.
-bool tc_product_ok(const Product &P);
-int tc_product(cudaStream_t st, const Product &P);
-bool tc_gradient_ok(const Gradient &G);
-int tc_gradient(cudaStream_t st, const Gradient &G);
+// The tensor-core kernels (expert_mm_tc.cu), bf16 operands of 16-byte aligned
+// rows: the workspace of their split tiles, and the launch; -1 when the driver
+// refuses a tensor map.
+size_t tc_product_workspace(const Product &P);
+int tc_product(cudaStream_t st, const Product &P, void *ws);
+size_t tc_gradient_workspace(const Gradient &G);
+int tc_gradient(cudaStream_t st, const Gradient &G, void *ws);
+
+// A stream over the weights for a few rows a group (expert_mm_skinny.cu), any
+// type, order and alignment.
+bool skinny_ok(const Product &P);
+int skinny_product(cudaStream_t st, const Product &P);
 
 // Rows [lo, hi) of group e, kept inside [0, S] whatever rowptr holds.
 __device__ __forceinline__ void group_rows(const int32_t *__restrict__ rowptr, int base, int64_t S,
@@ -93,6 +99,9 @@ __device__ __forceinline__ float phi_fast(float z, float &e) {
     return z < 0.0f ? q : 1.0f - q;
 }
 
+// act's last product and the residual's sum are rounded separately (mul_rn,
+// add_rn): contracted in one caller and not in another they would give a call
+// with the pre-activation kept other bits than one without.
 template <typename T>
 __device__ __forceinline__ float act_value(float z, int act) {
     constexpr bool fast = sizeof(T) == 2;
@@ -101,7 +110,7 @@ __device__ __forceinline__ float act_value(float z, int act) {
         case JLB_ACT_SILU: return fast ? __fdividef(z, 1.0f + __expf(-z)) : z / (1.0f + expf(-z));
         case JLB_ACT_GELU: {
             float e;
-            return fast ? z * phi_fast(z, e) : 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+            return fast ? mul_rn(z, phi_fast(z, e)) : mul_rn(0.5f * z, 1.0f + erff(z * 0.70710678118654752f));
         }
         default: return z;
     }

@@ -1,0 +1,299 @@
+// expert_mm_skinny.cu -- the grouped and dense products for a few rows a group
+// (decode steps, single tokens): the weights are read once and nothing else
+// costs, so the kernel is a stream over W with the rows' values beside it.
+//
+// A CTA takes one group and one tile of its columns; up to 8 rows at a time
+// sit in shared memory as fp32.  Row-major W: 8 lanes read 128 contiguous
+// bytes of one row of W, 32 rows of W a pass; a thread keeps sums[rows][8]
+// and each weight it loads meets every row.  Column-major W: 8 lanes read 128
+// bytes along K, a thread holds 4 columns.  The inner dimension is split over
+// the CTAs of a cluster when there are few tiles, and the parts are added
+// through distributed shared memory in rank order: one launch, no workspace,
+// the same order on every run.  Unaligned W is read one element a lane.
+//
+// Bound: HBM (L2 for repeated weights).  Sums are fp32 FMAs, one rounding to
+// the value type.
+#include "expert_mm.cuh"
+
+#include <cooperative_groups.h>
+
+namespace jlb {
+
+JLB_DEFINE_DEV_ERROR(emm_skinny)
+
+namespace emm {
+
+namespace cg = cooperative_groups;
+
+constexpr int kSkThreads = 256, kSkWarps = 8;
+constexpr int kSkK = 1024;                 // inner elements of x staged at a time
+constexpr int kSkCols = 4;                 // columns a thread holds for column-major W
+
+// Tile width: VEC values a lane (16 bytes, or one), LX lanes side by side.
+template <typename T, bool COL, int VEC>
+struct SkShape {
+    static constexpr int kLX = VEC > 1 ? 8 : 32;
+    static constexpr int kTile = COL ? kSkCols * (32 / kLX) : kLX * VEC;
+};
+
+// VEC values as they lie in memory, and their fp32 values.
+template <typename T, int VEC>
+struct SkRaw {
+    uint4 q;
+    T one;
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void sk_fetch(SkRaw<T, VEC> &r, const T *p, int n) {
+    if constexpr (VEC == 1) {
+        r.one = n > 0 ? *p : from_f32<T>(0.0f);
+    } else if (n >= VEC) {
+        r.q = __ldg(reinterpret_cast<const uint4 *>(p));
+    } else {                                       // the matrix's edge: the rest is zero
+        T v[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = i < n ? p[i] : from_f32<T>(0.0f);
+        r.q = *reinterpret_cast<const uint4 *>(v);
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void sk_value(const SkRaw<T, VEC> &r, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = to_f32(r.one);
+    } else {
+        const uint32_t w[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            v[i] = sizeof(T) == 4 ? __uint_as_float(w[i % 4])
+                                  : __uint_as_float(i % 2 ? w[i / 2 % 4] & 0xffff0000u : w[i / 2 % 4] << 16);
+    }
+}
+
+// Sums of MR rows over inner elements [k0, k1), this thread's part; the CTA's
+// sums end in red[0 .. MR * tile).
+template <typename T, bool COL, int VEC, int MR>
+__device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0, int row, int nrows, int64_t k0,
+                                        int64_t k1, float *xs, float *red, bool &bad) {
+    using S = SkShape<T, COL, VEC>;
+    constexpr int LX = S::kLX, CT = S::kTile;
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, lx = lane % LX;
+    constexpr int NS = COL ? kSkCols : VEC;        // sums a row and thread
+    float acc[MR][NS];
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int c = 0; c < NS; ++c) acc[m][c] = 0.0f;
+    for (int64_t kc = k0; kc < k1; kc += kSkK) {
+        const int kn = (int)(k1 - kc < kSkK ? k1 - kc : kSkK);
+        __syncthreads();                           // the values of the step before are used
+        for (int q = threadIdx.x; q < MR * kn; q += kSkThreads) {
+            const int m = q / kn, k = q - m * kn;
+            float v = 0.0f;
+            if (m < nrows) {
+                int64_t s = row + m;
+                if (P.rows) s = (int64_t)__ldg(P.rows + s) - P.base;
+                if (s < 0 || s >= P.T) bad = true;
+                else v = to_f32(((const T *)P.x)[s * P.ldx + kc + k]);
+            }
+            xs[COL ? m * (kSkK + 8) + k : k * MR + m] = v;
+        }
+        // a column-major step may read up to 16 bytes past kn: zeros there
+        if (COL && threadIdx.x < MR * VEC) xs[(threadIdx.x / VEC) * (kSkK + 8) + kn + threadIdx.x % VEC] = 0.0f;
+        __syncthreads();
+        // U loads are on their way before the first is used
+        if (!COL) {
+            constexpr int KY = kSkThreads / LX;    // rows of W a pass
+            constexpr int U = MR <= 2 ? 8 : 4;
+            const int ky = threadIdx.x / LX, n = (int)min((int64_t)VEC, P.N - (n0 + lx * VEC));
+            const T *p = w + kc * P.ldw + n0 + lx * VEC;
+            for (int kb = ky; kb < kn && n > 0; kb += U * KY) {
+                SkRaw<T, VEC> raw[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = kb + u * KY;
+                    sk_fetch<T, VEC>(raw[u], p + (int64_t)k * P.ldw, k < kn ? n : 0);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = kb + u * KY;
+                    float v[VEC];
+                    sk_value<T, VEC>(raw[u], v);
+#pragma unroll
+                    for (int m = 0; m < MR; ++m) {
+                        const float xv = k < kn ? xs[k * MR + m] : 0.0f;
+#pragma unroll
+                        for (int c = 0; c < VEC; ++c) acc[m][c] = fmaf(xv, v[c], acc[m][c]);
+                    }
+                }
+            }
+        } else {
+            constexpr int KP = LX * VEC;           // inner elements a warp's pass
+            constexpr int U = MR <= 2 ? 2 : 1;
+            const T *p[kSkCols];
+#pragma unroll
+            for (int c = 0; c < kSkCols; ++c) {
+                const int64_t n = n0 + (lane / LX) + c * (32 / LX);
+                p[c] = w + (n < P.N ? n : n0) * P.ldw + kc;
+            }
+            for (int kb = warp * KP + lx * VEC; kb < kn; kb += U * kSkWarps * KP) {
+                SkRaw<T, VEC> raw[U][kSkCols];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int c = 0; c < kSkCols; ++c) {
+                        const int k = kb + u * kSkWarps * KP;
+                        sk_fetch<T, VEC>(raw[u][c], p[c] + k, kn - k);
+                    }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = kb + u * kSkWarps * KP;
+                    if (k >= kn) break;
+                    float v[kSkCols][VEC];
+#pragma unroll
+                    for (int c = 0; c < kSkCols; ++c) sk_value<T, VEC>(raw[u][c], v[c]);
+#pragma unroll
+                    for (int m = 0; m < MR; ++m) {
+                        float xv[VEC];
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) xv[i] = xs[m * (kSkK + 8) + k + i];
+#pragma unroll
+                        for (int c = 0; c < kSkCols; ++c)
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) acc[m][c] = fmaf(xv[i], v[c][i], acc[m][c]);
+                    }
+                }
+            }
+        }
+    }
+    // the warp's sums, then the warps' in order
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int c = 0; c < NS; ++c) {
+            float s = acc[m][c];
+            if (COL) {
+#pragma unroll
+                for (int o = 1; o < LX; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (lx == 0) red[(warp * MR + m) * CT + lane / LX + c * (32 / LX)] = s;
+            } else {
+#pragma unroll
+                for (int o = LX; o < kWarp; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (lane < LX) red[(warp * MR + m) * CT + lx * VEC + c] = s;
+            }
+        }
+    __syncthreads();
+    for (int o = threadIdx.x; o < MR * CT; o += kSkThreads) {
+        float s = red[o];
+#pragma unroll
+        for (int q = 1; q < kSkWarps; ++q) s += red[q * MR * CT + o];
+        red[o] = s;
+    }
+}
+
+// MAXR: rows taken at a time.
+template <typename T, bool COL, int VEC, int MAXR>
+__global__ void __launch_bounds__(kSkThreads, MAXR <= 2 ? 4 : 2)
+product_skinny(const __grid_constant__ Product P, int splits) {
+    using S = SkShape<T, COL, VEC>;
+    constexpr int CT = S::kTile;
+    extern __shared__ __align__(16) float sk_smem[];
+    float *xs = sk_smem;                              // MAXR x (kSkK + 8)
+    float *red = sk_smem + MAXR * (kSkK + 8);         // kSkWarps x MAXR x CT
+    const int64_t e = blockIdx.y, n0 = (int64_t)blockIdx.x * CT;
+    int lo, hi;
+    group_rows(P.rowptr, P.base, P.S, e, lo, hi);
+    bool bad = P.rowptr && group_bad(P.rowptr, P.base, P.S, e);
+    if (P.rowptr && blockIdx.z == 0) {                // rows of no group are zero
+        int a, end;
+        group_rows(P.rowptr, P.base, P.S, P.E - 1, a, end);
+        for (int64_t r = (int64_t)end + e; r < P.S; r += P.E)
+            for (int c = threadIdx.x; c < CT && n0 + c < P.N; c += kSkThreads) {
+                ((T *)P.y)[r * P.ldy + n0 + c] = from_f32<T>(0.0f);
+                if (P.z) ((T *)P.z)[r * P.ldz + n0 + c] = from_f32<T>(0.0f);
+            }
+    }
+    // this CTA's part of the inner dimension, in whole 16-byte groups
+    const int64_t share = (ceil_div(P.K, splits) + 63) / 64 * 64;
+    const int64_t k0 = min(P.K, share * blockIdx.z), k1 = min(P.K, k0 + share);
+    const T *w = (const T *)P.w + e * P.w_stride;
+    cg::cluster_group cluster = cg::this_cluster();
+    for (int row = lo; row < hi; row += MAXR) {
+        const int nr = min(MAXR, hi - row);
+        if (nr == 1) sk_rows<T, COL, VEC, 1>(P, w, n0, row, nr, k0, k1, xs, red, bad);
+        else if (MAXR == 2 || nr == 2) sk_rows<T, COL, VEC, 2>(P, w, n0, row, nr, k0, k1, xs, red, bad);
+        else if (nr <= 4) sk_rows<T, COL, VEC, MAXR < 4 ? MAXR : 4>(P, w, n0, row, nr, k0, k1, xs, red, bad);
+        else sk_rows<T, COL, VEC, MAXR>(P, w, n0, row, nr, k0, k1, xs, red, bad);
+        if (splits > 1) cluster.sync();
+        else __syncthreads();
+        if (blockIdx.z == 0)
+            for (int o = threadIdx.x; o < nr * CT; o += kSkThreads) {
+                const int64_t r = row + o / CT, n = n0 + o % CT;
+                if (n >= P.N) continue;
+                float v = red[o];
+                for (int q = 1; q < splits; ++q) v += *cluster.map_shared_rank(red + o, q);
+                if (P.bias) v += to_f32(((const T *)P.bias)[e * P.ldb + n]);
+                if (P.z) ((T *)P.z)[r * P.ldz + n] = from_f32<T>(v);
+                v = act_value<T>(v, P.act);
+                if (P.res) v = add_rn(v, to_f32(((const T *)P.res)[r * P.ldr + n]));
+                ((T *)P.y)[r * P.ldy + n] = from_f32<T>(v);
+            }
+        if (splits > 1) cluster.sync();               // the parts are read before they are overwritten
+    }
+    if (bad) dev_error(DEV_ERR_BOUNDS);
+}
+
+// Few rows: one or two in bf16, where the tensor path is as fast from there
+// on; F32 up to 16 rows, or two a group.
+bool skinny_ok(const Product &P) {
+    if (P.E > 65535 || P.K == 0) return false;
+    if (P.dtype == JLB_BF16) return P.S <= 2;
+    return P.S <= (P.rowptr ? 2 * P.E : 16) && P.S <= 4096;
+}
+
+template <typename T, bool COL, int VEC, int MAXR>
+static int launch_skinny(cudaStream_t st, const Product &P) {
+    using S = SkShape<T, COL, VEC>;
+    const int64_t tiles = ceil_div(P.N, S::kTile);
+    // about three CTAs an SM, at least 128 inner elements each
+    const int64_t live = tiles * (P.rowptr ? (P.E < P.S ? P.E : P.S) : 1);
+    int64_t splits = 444 / (live > 0 ? live : 1);
+    if (splits > P.K / 128) splits = P.K / 128;
+    splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
+    const size_t smem = (size_t)(MAXR * (kSkK + 8) + kSkWarps * MAXR * S::kTile) * 4;
+    JLB_CUDA(cudaFuncSetAttribute(product_skinny<T, COL, VEC, MAXR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = (unsigned)splits;
+    cfg.gridDim = dim3((unsigned)tiles, (unsigned)P.E, (unsigned)splits);
+    cfg.blockDim = dim3(kSkThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    JLB_CUDA(cudaLaunchKernelEx(&cfg, product_skinny<T, COL, VEC, MAXR>, P, (int)splits));
+    return ok();
+}
+
+template <typename T, bool COL, int VEC>
+static int skinny_rows(cudaStream_t st, const Product &P) {
+    return P.S <= 2 ? launch_skinny<T, COL, VEC, 2>(st, P) : launch_skinny<T, COL, VEC, 8>(st, P);
+}
+
+template <typename T>
+static int skinny_of(cudaStream_t st, const Product &P) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool vec = aligned16(P.w) && P.ldw % V == 0 && (P.E == 1 || P.w_stride % V == 0);
+    if (P.w_order == JLB_ROW_MAJOR)
+        return vec ? skinny_rows<T, false, V>(st, P) : skinny_rows<T, false, 1>(st, P);
+    return vec ? skinny_rows<T, true, V>(st, P) : skinny_rows<T, true, 1>(st, P);
+}
+
+int skinny_product(cudaStream_t st, const Product &P) {
+    return P.dtype == JLB_F32 ? skinny_of<float>(st, P) : skinny_of<__nv_bfloat16>(st, P);
+}
+
+}  // namespace emm
+}  // namespace jlb

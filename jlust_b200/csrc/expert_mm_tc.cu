@@ -31,6 +31,10 @@
 // Work split: a persistent grid of CTA pairs; pair c takes tiles c, c + G, ...
 // numbered group by group from rowptr on the device (each warp role walks 32
 // groups at a time), inside a group in column blocks of 8 tiles for L2 reuse.
+// The tiles that do not fill a last round of the G pairs (all of them, when
+// there are few) are split along the inner dimension among the pairs; their
+// fp32 parts go to the workspace and finish_tc adds them in order and applies
+// the epilogue.
 // Roles: warp 0 copies, warp 1 of the leader issues products, warps 2-9 read
 // TMEM and store, warps 10-13 (only in launches that need them) load rows and
 // warp 14 reports their stages to the leader; two TMEM accumulators, so a tile's epilogue
@@ -77,7 +81,10 @@ struct TcArgs {
     __nv_bfloat16 *z, *out;
     int64_t ldz, ldo, out_stride;
     int stages, bn_max;
-    int a_pair, b_pair;           // mA / mB: both 64-wide boxes of an operand in one copy
+    int a_pair, b_pair;           // mA / mBig: both 64-wide boxes of an operand in one copy
+    int pairs, max_splits;        // CTA pairs launched; parts a tile may be split into (> 1: rowptr decides)
+    int full, splits;             // tiles not split and the parts of the others, when the host knows
+    float *part;                  // one 256 x bn_max fp32 tile for each part
 };
 
 // A pipeline stage: A's half and, in 32-row boxes, B's.
@@ -121,71 +128,128 @@ __device__ __forceinline__ void tc_drain(uint32_t bar, uint32_t parity) {
 struct Tile {
     int e, lo, hi;      // group and its rows
     int i0, j0, bn;     // first lane, first column (product: relative to lo), columns of the instruction
+    int kb0, kb1;       // 64-wide steps of the inner dimension
+    int part;           // where a split tile's sums go, or -1
 };
 
+// width of a group's column tiles: equal shares rounded up to 32
+__host__ __device__ __forceinline__ int col_width(int r, int bn_max) {
+    const unsigned nt = (unsigned)(r + bn_max - 1) / (unsigned)bn_max;
+    return (int)((((unsigned)r + nt - 1u) / nt + 31u) & ~31u);
+}
+__host__ __device__ __forceinline__ int col_tiles(int r, int bn_max) {
+    if (r <= bn_max) return r > 0;
+    const int w = col_width(r, bn_max);
+    return (int)((unsigned)(r + w - 1) / (unsigned)w);
+}
+
+// Tiles of the full rounds, and into how many parts each of the rest is split.
+__host__ __device__ inline void split_schedule(int all, int pairs, int max_splits, int &full, int &splits) {
+    full = (int)((unsigned)all / (unsigned)pairs) * pairs;
+    const int rest = all - full;
+    splits = rest && max_splits > 1 ? (int)((unsigned)pairs / (unsigned)rest) : 1;
+    if (splits > max_splits) splits = max_splits;
+    if (splits <= 1) {
+        splits = 1;
+        full = all;
+    }
+}
+
 // Walks the tiles in order, 32 groups at a time; every lane of the warp calls.
+// 32-bit arithmetic and one copy of the code for all roles: a launch of few
+// tiles is as long as its first instruction misses (with 64-bit divisions
+// inlined in each role, 10,000 cycles went by before the first copy).
 template <bool GRAD>
 struct Walk {
-    int64_t e0, before;
-    int total, lo, hi, first, tiles, lane, it;
-    __device__ void load(const TcArgs &P) {
+    int e0, before, total, lo, hi, first, tiles, it, jt;
+    int full, splits;                 // tiles not split; parts of each other one
+
+    __device__ __forceinline__ int count(const TcArgs &P, int e, int &a, int &b) const {
+        group_rows(P.rowptr, P.base, P.S, e, a, b);
+        return GRAD ? it * jt : it * col_tiles(b - a, P.bn_max);
+    }
+    __device__ __forceinline__ void load(const TcArgs &P) {
+        const int lane = threadIdx.x % kWarp;
         lo = hi = tiles = 0;
-        if (e0 + lane < P.E) {
-            group_rows(P.rowptr, P.base, P.S, e0 + lane, lo, hi);
-            tiles = GRAD ? it * (int)((P.J + 255) / 256) : it * col_tiles(hi - lo, P.bn_max);
-        }
+        if (e0 + lane < (int)P.E) tiles = count(P, e0 + lane, lo, hi);
         int inc = tiles;
+        if (P.E > 1)
 #pragma unroll
-        for (int o = 1; o < kWarp; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
-        }
+            for (int o = 1; o < kWarp; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += u;
+            }
         first = inc - tiles;
-        total = __shfl_sync(0xffffffffu, inc, 31);
+        total = __shfl_sync(0xffffffffu, inc, P.E > 1 ? 31 : 0);
     }
-    // width of a group's column tiles: equal shares rounded up to 32
-    static __device__ __forceinline__ int col_width(int r, int bn_max) {
-        const int nt = (r + bn_max - 1) / bn_max;
-        return ((r + nt - 1) / nt + 31) & ~31;
-    }
-    static __device__ __forceinline__ int col_tiles(int r, int bn_max) {
-        if (r <= 0) return 0;
-        const int w = col_width(r, bn_max);
-        return (r + w - 1) / w;
-    }
-    __device__ void init(const TcArgs &P) {
-        lane = threadIdx.x % kWarp;
-        it = (int)((P.I + 255) / 256);
+    __device__ __noinline__ void init(const TcArgs &P) {
+        it = (int)((P.I + 255) >> 8);
+        jt = (int)((P.J + 255) >> 8);
+        full = P.full;
+        splits = P.splits;
+        if (P.max_splits > 1) {       // a product whose tiles only rowptr tells
+            const int lane = threadIdx.x % kWarp;
+            int all = 0;
+            for (int e = lane; e < (int)P.E; e += kWarp) {
+                int a, b;
+                all += count(P, e, a, b);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            split_schedule(all, P.pairs, P.max_splits, full, splits);
+        }
         e0 = 0;
         before = 0;
         load(P);
     }
-    __device__ bool find(const TcArgs &P, int64_t t, Tile &T) {
+    __device__ __forceinline__ int steps(const TcArgs &P, const Tile &T) const {
+        return GRAD ? (T.hi - T.lo + 63) >> 6 : (int)((P.Kc + 63) >> 6);
+    }
+    // Work item u of a pair: a whole tile, or a part of one of the rest.
+    __device__ __noinline__ bool find(const TcArgs &P, int u, Tile &T) {
+        if (u < full || splits == 1) {
+            if (!tile(P, u, T)) return false;
+            T.kb0 = 0;
+            T.kb1 = steps(P, T);
+            T.part = -1;
+            return true;
+        }
+        const unsigned q = (unsigned)(u - full), t = q / (unsigned)splits, sp = q - t * splits;
+        if (!tile(P, full + (int)t, T)) return false;
+        const unsigned nkb = (unsigned)steps(P, T);    // < 2^25 steps, < 2^7 parts
+        T.kb0 = (int)(nkb * sp / splits);
+        T.kb1 = (int)(nkb * (sp + 1) / splits);
+        T.part = (int)q;
+        return true;
+    }
+    __device__ __forceinline__ bool tile(const TcArgs &P, int t, Tile &T) {
         while (t >= before + total) {
             before += total;
             e0 += kWarp;
-            if (e0 >= P.E) return false;
+            if (e0 >= (int)P.E) return false;
             load(P);
         }
-        const int want = (int)(t - before);
-        const int src = __ffs(__ballot_sync(0xffffffffu, want >= first && want < first + tiles)) - 1;
-        T.e = (int)e0 + src;
+        const int want = t - before;
+        int src = 0;
+        if (P.E > 1) src = __ffs(__ballot_sync(0xffffffffu, want >= first && want < first + tiles)) - 1;
+        T.e = e0 + src;
         T.lo = __shfl_sync(0xffffffffu, lo, src);
         T.hi = __shfl_sync(0xffffffffu, hi, src);
         const int l = want - __shfl_sync(0xffffffffu, first, src);
-        const int n = __shfl_sync(0xffffffffu, tiles, src) / it;      // column tiles
-        const int jb = l / (kJBlock * it), rem = l - jb * kJBlock * it;
-        const int w = min(kJBlock, n - kJBlock * jb);
-        const int i = rem / w, j = kJBlock * jb + rem - i * w;
-        T.i0 = i * 256;
-        if (GRAD) {
-            T.j0 = j * 256;
-            T.bn = P.J - T.j0 > 128 ? 256 : 128;
-        } else {
-            const int cw = col_width(T.hi - T.lo, P.bn_max);
-            T.j0 = j * cw;
-            T.bn = min(cw, (T.hi - T.lo - T.j0 + 31) & ~31);
+        // column tiles j, in blocks of kJBlock, lane tiles i inside a block
+        const int cw = GRAD ? 256 : col_width(T.hi - T.lo, P.bn_max);
+        const int n = GRAD ? jt : (int)((unsigned)(T.hi - T.lo + cw - 1) / (unsigned)cw);
+        int i = l, j = 0;
+        if (n > 1) {
+            const int jb = n <= kJBlock ? 0 : (int)((unsigned)l / (unsigned)(kJBlock * it));
+            const int rem = l - jb * kJBlock * it, w = min(kJBlock, n - kJBlock * jb);
+            i = (int)((unsigned)rem / (unsigned)w);
+            j = kJBlock * jb + rem - i * w;
         }
+        T.i0 = i * 256;
+        T.j0 = j * cw;
+        if (GRAD) T.bn = P.J - T.j0 > 128 ? 256 : 128;
+        else T.bn = min(cw, (T.hi - T.lo - T.j0 + 31) & ~31);
         return true;
     }
 };
@@ -268,7 +332,7 @@ __device__ __forceinline__ void store_tile(const TcArgs &P, uint32_t taddr, uint
                 const __nv_bfloat16 *q = P.res + (row0 + c0) * P.ldr + i;
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
-                    if (c < n) v[c] += __bfloat162float(q[c * P.ldr]);
+                    if (c < n) v[c] = add_rn(v[c], __bfloat162float(q[c * P.ldr]));
             }
         }
         store32(v, turn, vec, out, P.ldo, row0 + c0, n, ib, P.I);
@@ -290,7 +354,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
     const bool loaders = blockDim.x > kTcThreads;
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     const uint32_t rank = cluster_rank();
-    const int64_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
     volatile int *abort_flag = &ctl->abort;
 
     if (threadIdx.x == 0) {
@@ -315,6 +379,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
     cluster_sync();
     fence_after();
     const uint32_t tmem = ctl->tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == 0) {
         // ------------------------------------------------------------ copies
@@ -327,13 +392,12 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Walk<GRAD> walk;
         walk.init(P);
         Tile T;
-        for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
+        for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
             const int a0 = T.i0 + (int)rank * 128;
-            const int nkb = GRAD ? (T.hi - T.lo + 63) / 64 : (int)((P.Kc + 63) / 64);
             const int bh = T.bn / 2, boxes = (bh + 31) / 32;           // product: B's rows, in 32-row boxes
             const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
             const int nb = T.bn / 128, bj0 = T.j0 + (int)rank * bh;    // gradient: B's 64-column boxes
-            for (int kb = 0; lane == 0 && kb < nkb; ++kb) {
+            for (int kb = T.kb0; lane == 0 && kb < T.kb1; ++kb) {
                 if (!tc_wait(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
                 {
                     const uint32_t sA = tiles_u32 + (uint32_t)stage * stage_bytes, sB = sA + kABytes;
@@ -407,21 +471,20 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             Walk<GRAD> walk;
             walk.init(P);
             Tile T;
-            for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
-                const int nkb = GRAD ? (T.hi - T.lo + 63) / 64 : (int)((P.Kc + 63) / 64);
-                if (nkb == 0) continue;                       // the epilogue writes zeros
+            for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
+                if (T.kb0 == T.kb1) continue;                 // the epilogue writes zeros
                 if (!tc_wait_warp(smem_u32(&ctl->tempty[buf]), te[buf], abort_flag)) break;
                 te[buf] ^= 1u;
                 fence_after();
                 const uint32_t idesc = instr_desc(256, (uint32_t)T.bn, A_MN, GRAD);
                 if (lane == 0)
-                    for (int kb = 0; kb < nkb; ++kb) {
+                    for (int kb = T.kb0; kb < T.kb1; ++kb) {
                         if (!tc_wait(smem_u32(&ctl->full[stage]), pf, abort_flag)) { ok = false; break; }
                         fence_after();
                         const uint32_t off = ((uint32_t)stage * stage_bytes) >> 4;
                         mma_pair_k64<A_MN ? 128 : 2, GRAD ? 128 : 2>(tmem + (uint32_t)buf * 256u, (uint32_t)a_desc + off,
                                                                      (uint32_t)(a_desc >> 32), (uint32_t)b_desc + off,
-                                                                     (uint32_t)(b_desc >> 32), idesc, (uint32_t)kb);
+                                                                     (uint32_t)(b_desc >> 32), idesc, (uint32_t)(kb - T.kb0));
                         commit_pair(smem_u32(&ctl->empty[stage]));
                         if (++stage == P.stages) { stage = 0; pf ^= 1u; }
                     }
@@ -453,15 +516,18 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Walk<GRAD> walk;
         walk.init(P);
         Tile T;
-        for (int64_t t = pair; walk.find(P, t, T); t += pairs) {
+        for (int t = pair; walk.find(P, t, T); t += pairs) {
             const int64_t ib = (int64_t)T.i0 + rank * 128 + qd * 32;
             // column 0's row of the output, and its columns
             const int64_t row0 = GRAD ? T.j0 : (int64_t)T.lo + T.j0;
             const int nj = GRAD ? (int)min((int64_t)T.bn, P.J - T.j0) : min(T.bn, T.hi - T.lo - T.j0);
             __nv_bfloat16 *out = P.out + (GRAD ? T.e * P.out_stride : 0);
-            if (GRAD && T.hi == T.lo) {
-                if (ib + lane < P.I)
-                    for (int c = first; c < nj; c += 2) out[(row0 + c) * P.ldo + ib + lane] = __float2bfloat16_rn(0.0f);
+            float *part = T.part >= 0 ? P.part + (int64_t)T.part * 256 * P.bn_max + (ib - T.i0) + lane : nullptr;
+            if (T.kb0 == T.kb1) {
+                for (int c = first; c < nj; c += 2) {
+                    if (part) part[c * 256] = 0.0f;
+                    else if (ib + lane < P.I) out[(row0 + c) * P.ldo + ib + lane] = __float2bfloat16_rn(0.0f);
+                }
                 continue;
             }
             const float bias = !GRAD && P.bias && ib + lane < P.I ? __bfloat162float(P.bias[T.e * P.ldb + ib + lane]) : 0.0f;
@@ -469,7 +535,16 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             tf[buf] ^= 1u;
             fence_after();
             const uint32_t taddr = tmem + ((uint32_t)(qd * 32) << 16) + (uint32_t)(buf * 256);
-            if (ib < P.I) {
+            if (part) {
+                for (int c0 = first * 32; c0 < nj; c0 += 64) {
+                    uint32_t r[32];
+                    __syncwarp();
+                    JLB_TC_LD32(taddr + (uint32_t)c0, r);
+                    wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) part[(c0 + c) * 256] = __uint_as_float(r[c]);
+                }
+            } else if (ib < P.I) {
                 switch (GRAD ? JLB_ACT_NONE : P.act) {
                     case JLB_ACT_RELU: store_tile<JLB_ACT_RELU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
                     case JLB_ACT_SILU: store_tile<JLB_ACT_SILU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
@@ -497,8 +572,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Walk<GRAD> walk;
         walk.init(P);
         Tile T;
-        for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
-            const int nkb = GRAD ? (T.hi - T.lo + 63) / 64 : (int)((P.Kc + 63) / 64);
+        for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
             const int bh = T.bn / 2, nb = T.bn / 128;
             if (!GRAD) {
                 // the (at most 8) rows of B this lane copies 16 bytes of
@@ -520,7 +594,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                     }
                 }
                 const int rows = (bh - lw * 4 + 15) / 16;       // bh is a multiple of 16: all lanes alike
-                for (int kb = 0; kb < nkb; ++kb) {
+                for (int kb = T.kb0; kb < T.kb1; ++kb) {
                     if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
                     const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + kABytes + at0;
                     const uint32_t bytes = bytes_at((int64_t)kb * 64 + c8 * 8, P.Kc);
@@ -561,8 +635,8 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                     }
                 }
             };
-            if (P.gather) fetch(0);
-            for (int kb = 0; kb < nkb; ++kb) {
+            if (P.gather) fetch(T.kb0);
+            for (int kb = T.kb0; kb < T.kb1; ++kb) {
                 // (without gather only a group's last step is loaded; the copy
                 // thread, which waits for every stage, says when: a wait for
                 // the stage's own barrier could be laps of the ring early)
@@ -571,12 +645,13 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 // would wait for the step's copies before it
                 const bool tail = T.hi - T.lo - kb * 64 < 64;
                 const bool la = tail || P.gather == 1, lb = tail || P.gather == 2;
-                if (P.gather && kb % kAhead == 0) {
+                const int ka = (kb - T.kb0) % kAhead;
+                if (P.gather && ka == 0) {
                     __syncwarp();
 #pragma unroll
                     for (int n = 0; n < kAhead * 16 / kWarp; ++n) ctl->idx[lw][n * kWarp + lane] = ahead[n];
                     __syncwarp();
-                    if (kb + kAhead < nkb) fetch(kb + kAhead);
+                    if (kb + kAhead < T.kb1) fetch(kb + kAhead);
                 }
                 if (!la && !lb) {
                     if (++stage == P.stages) { stage = 0; pe ^= 1u; }
@@ -587,7 +662,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 for (int n = 0; n < 4; ++n) {
                     const int p = T.lo + kb * 64 + lw * 4 + n * 16 + sub;
                     sp[n] = p < T.hi ? p : -1;
-                    sg[n] = P.gather ? ctl->idx[lw][(kb % kAhead) * 16 + n * 4 + sub] : sp[n];
+                    sg[n] = P.gather ? ctl->idx[lw][ka * 16 + n * 4 + sub] : sp[n];
                 }
                 if (!(P.gather ? tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)
                                : tc_wait_warp(smem_u32(&ctl->go[stage]), pgo >> stage & 1u, abort_flag))) {
@@ -634,9 +709,8 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Walk<GRAD> walk;
         walk.init(P);
         Tile T;
-        for (int64_t t = pair; ok && walk.find(P, t, T); t += pairs) {
-            const int nkb = GRAD ? (T.hi - T.lo + 63) / 64 : (int)((P.Kc + 63) / 64);
-            for (int kb = 0; kb < nkb; ++kb) {
+        for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
+            for (int kb = T.kb0; kb < T.kb1; ++kb) {
                 if (!GRAD || P.gather || T.hi - T.lo - kb * 64 < 64) {
                     if (!tc_wait_warp(smem_u32(&ctl->rows[stage]), (pr >> stage) & 1u, abort_flag)) { ok = false; break; }
                     pr ^= 1u << stage;
@@ -665,6 +739,66 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
     if (warp == 1) {
         fence_after();
         dealloc_pair(tmem, 512);
+    }
+}
+
+// The split tiles: adds their parts in order and applies the epilogue.  CTA
+// (x, y): kFinish columns of the y-th split tile, one lane a thread; four
+// parts of them are loaded before any is added.  Launched
+// while product_tc runs; the wait ends when that grid is complete.
+constexpr int kFinish = 4;
+template <bool GRAD>
+__global__ void __launch_bounds__(256) finish_tc(const __grid_constant__ TcArgs P) {
+    __shared__ Tile ts;
+    __shared__ int ns;
+    if (threadIdx.x < kWarp) {
+        Walk<GRAD> walk;
+        walk.init(P);
+        Tile T;
+        const bool have = walk.splits > 1 && walk.find(P, walk.full + blockIdx.y * walk.splits, T);
+        if (threadIdx.x == 0) {
+            ns = have ? walk.splits : 0;
+            if (have) ts = T;
+        }
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (ns == 0) return;
+    const Tile T = ts;
+    const int nj = GRAD ? (int)min((int64_t)T.bn, P.J - T.j0) : min(T.bn, T.hi - T.lo - T.j0);
+    const int c0 = blockIdx.x * kFinish;
+    const int64_t i = (int64_t)T.i0 + threadIdx.x, item = (int64_t)256 * P.bn_max;
+    if (i >= P.I || c0 >= nj) return;
+    const float *part = P.part + (int64_t)blockIdx.y * ns * item + threadIdx.x;
+    const float bias = !GRAD && P.bias ? __bfloat162float(P.bias[T.e * P.ldb + i]) : 0.0f;
+    __nv_bfloat16 *out = P.out + (GRAD ? T.e * P.out_stride : 0) + i;
+    const int64_t row0 = GRAD ? T.j0 : (int64_t)T.lo + T.j0;
+    float sum[kFinish] = {};
+    for (int s0 = 0; s0 < ns; s0 += 4) {
+        float v[4][kFinish];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int c = 0; c < kFinish; ++c)
+                v[q][c] = s0 + q < ns && c0 + c < nj ? part[(s0 + q) * item + (int64_t)(c0 + c) * 256] : 0.0f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int c = 0; c < kFinish; ++c) sum[c] += v[q][c];
+    }
+#pragma unroll
+    for (int x = 0; x < kFinish; ++x) {
+        const int c = c0 + x;
+        if (c >= nj) break;
+        float v = sum[x];
+        const int64_t r = row0 + c;
+        if (!GRAD) {
+            v += bias;
+            if (P.z) P.z[r * P.ldz + i] = __float2bfloat16_rn(v);
+            v = act_value<__nv_bfloat16>(v, P.act);
+            if (P.res) v = add_rn(v, __bfloat162float(P.res[r * P.ldr + i]));
+        }
+        out[r * P.ldo] = __float2bfloat16_rn(v);
     }
 }
 
@@ -713,15 +847,6 @@ static bool make_pair_map(CUtensorMap *m, const void *p, int64_t cols, int64_t r
 
 static bool tma_matrix(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 
-bool tc_product_ok(const Product &P) {
-    return P.dtype == JLB_BF16 && P.K > 0 && P.T > 0 && P.E > 0 && tma_matrix(P.x, P.ldx) && tma_matrix(P.w, P.ldw) &&
-           (P.E == 1 || P.w_stride % 8 == 0);
-}
-
-bool tc_gradient_ok(const Gradient &G) {
-    return G.dtype == JLB_BF16 && G.S > 0 && G.T > 0 && tma_matrix(G.x, G.ldx) && tma_matrix(G.dz, G.lddz);
-}
-
 static int device_sms() {
     static int sms = [] {
         int dev = 0, n = 0;
@@ -733,30 +858,88 @@ static int device_sms() {
     return sms;
 }
 
+// Columns of the instruction a call needs at most, and how its tiles are
+// split: tiles is their number (product: an upper bound when rowptr decides).
+struct TcPlan {
+    int bn_max, pairs, max_splits, full, splits;
+    bool finish;
+    size_t part_bytes;
+};
+static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, int64_t steps) {
+    TcPlan p{bn_max, device_sms() / 2, 1, INT32_MAX, 1, false, 0};
+    if (tiles > INT32_MAX / 2) return p;           // the launch refuses
+    // at least four steps a part; and finish_tc's launch is worth it only when
+    // a partly filled last round can be a sixth of the work
+    int64_t most = steps / 4 < 64 ? steps / 4 : 64;
+    if (tiles >= 6 * (int64_t)p.pairs) most = 1;
+    if (exact) {
+        split_schedule((int)tiles, p.pairs, (int)most, p.full, p.splits);
+        p.finish = p.splits > 1;
+    } else if (most > 1) {
+        p.max_splits = (int)most;
+        p.finish = true;
+    }
+    if (p.finish) p.part_bytes = (size_t)p.pairs * 256 * bn_max * 4;
+    else if (tiles < p.pairs) p.pairs = (int)tiles;
+    return p;
+}
+
 template <bool A_MN, bool GRAD>
-static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &big, TcArgs &P, int64_t tiles,
-                     bool loaders) {
-    const uint32_t stage = stage_size(P.bn_max);
+static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &big, TcArgs &P,
+                     const TcPlan &plan, void *ws, bool loaders) {
     const size_t extra = 1024 + kTurnBytes + sizeof(TcCtl);
+    const uint32_t stage = stage_size(plan.bn_max);
+    P.bn_max = plan.bn_max;
+    P.pairs = plan.pairs;
+    P.max_splits = plan.max_splits;
+    P.full = plan.full;
+    P.splits = plan.splits;
+    P.part = (float *)ws;
     P.stages = (int)((227 * 1024 - extra) / stage);
     if (P.stages > kMaxStages) P.stages = kMaxStages;
     const size_t smem = (size_t)P.stages * stage + extra;
     JLB_CUDA(cudaFuncSetAttribute(product_tc<A_MN, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    int64_t pairs = device_sms() / 2;
-    if (tiles < pairs) pairs = tiles;
-    product_tc<A_MN, GRAD><<<(unsigned)(2 * pairs), kTcThreads + (loaders ? kLoaders + kForward : 0), smem, st>>>(a, b, big, P);
+    product_tc<A_MN, GRAD><<<(unsigned)(2 * P.pairs), kTcThreads + (loaders ? kLoaders + kForward : 0), smem, st>>>(a, b, big, P);
     JLB_LAUNCH_CHECK("product_tc");
+    if (plan.finish) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3((unsigned)ceil_div(P.bn_max, kFinish), (unsigned)(P.pairs / 2));   // a split tile has two parts at least
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        JLB_CUDA(cudaLaunchKernelEx(&cfg, finish_tc<GRAD>, P));
+    }
     return ok();
 }
 
+static TcPlan plan_product(const Product &p) {
+    const int bn = p.S >= 256 ? 256 : (int)((p.S + 31) / 32 * 32);
+    if (!p.rowptr)
+        return tc_plan(bn, col_tiles((int)p.S, bn) * ceil_div(p.N, 256), true, ceil_div(p.K, 64));
+    const int64_t cols = ceil_div(p.S, bn) + (p.E < p.S ? p.E : p.S);
+    return tc_plan(bn, cols * ceil_div(p.N, 256), false, ceil_div(p.K, 64));
+}
+
+static TcPlan plan_gradient(const Gradient &g) {
+    const int64_t J = g.w_order == JLB_ROW_MAJOR ? g.K : g.N, I = g.w_order == JLB_ROW_MAJOR ? g.N : g.K;
+    return tc_plan(J > 128 ? 256 : 128, g.E * ceil_div(I, 256) * ceil_div(J, 256), true, ceil_div(g.S / g.E, 64));
+}
+
+size_t tc_product_workspace(const Product &P) { return plan_product(P).part_bytes; }
+size_t tc_gradient_workspace(const Gradient &G) { return plan_gradient(G).part_bytes; }
+
 // Status, or -1 when the driver refuses a tensor map (the caller takes
 // another kernel).
-int tc_product(cudaStream_t st, const Product &p) {
+int tc_product(cudaStream_t st, const Product &p, void *ws) {
     CUtensorMap a, b, big;
     const bool mn = p.w_order == JLB_ROW_MAJOR;
-    const int64_t ws = p.E > 1 ? p.w_stride : (mn ? p.K : p.N) * p.ldw;
-    const bool pair = mn && make_pair_map(&a, p.w, p.N, p.K, p.ldw, p.E, ws);
-    if (!pair && !(mn ? make_map(&a, p.w, p.N, p.K, p.ldw, p.E, ws, 64) : make_map(&a, p.w, p.K, p.N, p.ldw, p.E, ws, 128)))
+    const int64_t w_stride = p.E > 1 ? p.w_stride : (mn ? p.K : p.N) * p.ldw;
+    const bool pair = mn && make_pair_map(&a, p.w, p.N, p.K, p.ldw, p.E, w_stride);
+    if (!pair && !(mn ? make_map(&a, p.w, p.N, p.K, p.ldw, p.E, w_stride, 64) : make_map(&a, p.w, p.K, p.N, p.ldw, p.E, w_stride, 128)))
         return -1;
     if (!make_map(&b, p.x, p.K, p.T, p.ldx, 0, 0, 32) || !make_map(&big, p.x, p.K, p.T, p.ldx, 0, 0, 128)) return -1;
     TcArgs P{};
@@ -782,14 +965,13 @@ int tc_product(cudaStream_t st, const Product &p) {
     P.out = (__nv_bfloat16 *)p.y;
     P.ldo = p.ldy;
     P.vec = tma_matrix(p.y, p.ldy) && (!p.z || tma_matrix(p.z, p.ldz)) && (!p.res || tma_matrix(p.res, p.ldr));
-    P.bn_max = p.S >= 256 ? 256 : (int)((p.S + 31) / 32 * 32);
-    const int64_t cols = ceil_div(p.S, P.bn_max) + (p.rowptr ? (p.E < p.S ? p.E : p.S) : 0);
-    const int64_t tiles = cols * ceil_div(p.N, 256);
-    return mn ? launch_tc<true, false>(st, a, b, big, P, tiles, p.rows)
-              : launch_tc<false, false>(st, a, b, big, P, tiles, p.rows);
+    const TcPlan plan = plan_product(p);
+    if (plan.pairs < 1 || (p.rowptr ? p.E : 1) * ceil_div(p.N, 256) * ceil_div(p.S, 32) > INT32_MAX / 2) return -1;
+    return mn ? launch_tc<true, false>(st, a, b, big, P, plan, ws, p.rows)
+              : launch_tc<false, false>(st, a, b, big, P, plan, ws, p.rows);
 }
 
-int tc_gradient(cudaStream_t st, const Gradient &g) {
+int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     // dw row-major: lanes = columns n (dz), columns = k (x); column-major: exchanged
     const bool row = g.w_order == JLB_ROW_MAJOR;
     const void *ap = row ? g.dz : g.x, *bp = row ? g.x : g.dz;
@@ -819,9 +1001,8 @@ int tc_gradient(cudaStream_t st, const Gradient &g) {
     P.out = (__nv_bfloat16 *)g.dw;
     P.ldo = g.lddw;
     P.out_stride = g.dw_stride;
-    P.bn_max = P.J > 128 ? 256 : 128;
-    const int64_t tiles = g.E * ceil_div(P.I, 256) * ceil_div(P.J, 256);
-    return launch_tc<true, true>(st, a, b, big, P, tiles, true);
+    if (P.E * ceil_div(P.I, 256) * ceil_div(P.J, 256) > INT32_MAX / 2) return -1;
+    return launch_tc<true, true>(st, a, b, big, P, plan_gradient(g), ws, true);
 }
 
 }  // namespace emm

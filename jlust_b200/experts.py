@@ -18,7 +18,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .backend import AbstractKernelHandle, _ptr, _same_device, _stream
+from .backend import AbstractKernelHandle
 from .errors import (DeviceMismatch, IncompatibleExtents, InvalidArgument,
                      UnsupportedIndexType, UnsupportedValueType)
 from .tensor import _origin
@@ -28,8 +28,28 @@ _ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU,
          "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
 
 
+# The calls below are short on the GPU, so their host side is kept lean:
+# addresses go to ctypes as integers and each operand is looked at once.
+
 def _base(origin) -> int:
     return _origin(origin).offset
+
+
+def _on(t: torch.Tensor) -> torch.device:
+    """The CUDA device of a call's first operand."""
+    d = t.device
+    if d.type != "cuda":
+        raise DeviceMismatch(f"B200Backend runs on CUDA devices only (operands on {d}); "
+                             "there is no CPU fallback")
+    return d
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _act(act) -> int:
@@ -48,7 +68,7 @@ def _type(t: torch.Tensor, what: str) -> int:
 
 def _rows(t: torch.Tensor, rows, cols, what: str, like: torch.Tensor):
     """Leading dimension of a row-major rows x cols matrix of like's type."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.dim() != 2 or t.shape != (rows, cols):
         raise IncompatibleExtents(f"{what} is {tuple(t.shape)}, expected ({rows}, {cols})")
     if t.dtype != like.dtype:
         raise UnsupportedValueType(f"{what}: operands must share one value type "
@@ -142,7 +162,7 @@ def route(ids: torch.Tensor, n_experts: int, origin=0) -> Routing:
     if ids.dim() != 2:
         raise IncompatibleExtents(f"ids must be tokens x k (got {tuple(ids.shape)})")
     _index(ids, ids.numel(), "ids", ids)
-    dev = _same_device(ids)
+    dev = _on(ids)
     T, k = ids.shape
     E, base = int(n_experts), _base(origin)
     L = _lib.load()
@@ -180,7 +200,9 @@ def combine(z: torch.Tensor, routing: Routing, weights=None, out=None) -> torch.
     S, N = routing.n_slots, z.shape[-1]
     ldz = _rows(z, S, N, "z", z)
     g = _combine_weights(weights, routing, z)
-    dev = _same_device(z, routing.slot)
+    dev = _on(z)
+    if routing.slot.device != dev:
+        raise _elsewhere(routing.slot, z, "routing")
     if out is None:
         out = torch.empty((T, N), dtype=z.dtype, device=dev)
     ldy = _rows(out, T, N, "out", z)
@@ -199,7 +221,9 @@ def combine_backward(dy: torch.Tensor, z: torch.Tensor, routing: Routing, weight
     ldz = _rows(z, S, N, "z", z)
     lddy = _rows(dy, T, N, "dy", z)
     g = _combine_weights(weights, routing, z)
-    dev = _same_device(z, dy, routing.slot, routing.rowptr)
+    dev = _on(z)
+    if routing.slot.device != dev:
+        raise _elsewhere(routing.slot, z, "routing")
     dz = torch.empty((S, N), dtype=z.dtype, device=dev)
     dg = torch.empty((T, k), dtype=torch.float32, device=dev)
     _lib.call("jlb_combine_backward", _stream(dev), dt, routing.origin.offset, T, k, S, N, E,
@@ -216,7 +240,9 @@ def _product(x, w3, rowptr, rows, bias, act, residual, keep_preact, out, base):
     if w3.dtype != x.dtype:
         raise UnsupportedValueType(f"product: x and w must share one value type ({x.dtype}, "
                                    f"{w3.dtype})")
-    dev = _same_device(x, w3)
+    dev = _on(x)
+    if w3.device != dev:
+        raise _elsewhere(w3, x, "w")
     if x.dim() != 2:
         raise IncompatibleExtents(f"x must be a matrix (got {tuple(x.shape)})")
     T = x.shape[0]
@@ -271,7 +297,9 @@ def _backward(dy, x, w3, rowptr, rows, z, act, need_bias, base):
     if w3.dtype != x.dtype:
         raise UnsupportedValueType(f"product gradient: x and w must share one value type "
                                    f"({x.dtype}, {w3.dtype})")
-    dev = _same_device(x, w3, dy)
+    dev = _on(x)
+    if w3.device != dev:
+        raise _elsewhere(w3, x, "w")
     T = x.shape[0]
     ldx = _rows(x, T, K, "x", x)
     S = T
@@ -289,7 +317,8 @@ def _backward(dy, x, w3, rowptr, rows, z, act, need_bias, base):
     if code != _lib.ACT_NONE:
         # dz in the value type: it is an operand of both products, and its
         # rounding enters them like that of any BF16 operand
-        dz, lddz = torch.empty((S, N), dtype=x.dtype, device=dev), max(N, 1)
+        lddz = max(8, -(-N // 8) * 8)      # rows that TMA can take as they are
+        dz = torch.empty((S, lddz), dtype=x.dtype, device=dev)
     if need_bias:
         db = torch.empty((E, N), dtype=x.dtype, device=dev)
     if need_bias or dz is not dy:
@@ -356,7 +385,7 @@ class B200ProductHandle(AbstractKernelHandle):
         w3 = w if grouped else w.unsqueeze(0)
         self.dtype = _type(w3, "product")
         self.E, self.K, self.N, ldw, sw, order = _weight(w3)
-        self.device = _same_device(w3)
+        self.device = _on(w3)
         self.grouped = grouped
         ldb = _bias(bias, self.E, self.N, w3)
         self.w, self.bias = w3, bias            # keep the buffers alive
@@ -390,15 +419,11 @@ class B200ProductHandle(AbstractKernelHandle):
         ldr = _rows(residual, S, N, "residual", w) if residual is not None else 0
         z = torch.empty((S, N), dtype=x.dtype, device=self.device) if keep_preact else None
         L = _lib.load()
-        xp = x.data_ptr()
-        wsb = L.jlb_mm_plan_workspace_size(self._plan, S, T, xp, ldx, 0 if rows is None else 1)
+        wsb = L.jlb_mm_plan_workspace_size(self._plan, S, T, _ptr(x), ldx, 0 if rows is None else 1)
         ws = _workspace(wsb, self.device)
-        st = L.jlb_mm_plan_execute(
-            self._plan, torch.cuda.current_stream(self.device).cuda_stream, S, T,
-            None if rowptr is None else rowptr.data_ptr(), None if rows is None else rows.data_ptr(),
-            xp, ldx, None if residual is None else residual.data_ptr(), ldr,
-            None if z is None else z.data_ptr(), N if N > 1 else 1, out.data_ptr(), ldy,
-            None if ws is None else ws.data_ptr(), wsb)
+        st = L.jlb_mm_plan_execute(self._plan, _stream(self.device), S, T, _ptr(rowptr), _ptr(rows),
+                                   _ptr(x), ldx, _ptr(residual), ldr, _ptr(z), max(N, 1), _ptr(out),
+                                   ldy, _ptr(ws), wsb)
         if st:
             _lib.check(st, "jlb_mm_plan_execute")
         return (out, z) if keep_preact else out
