@@ -156,9 +156,9 @@ __host__ __device__ inline void split_schedule(int all, int pairs, int max_split
 }
 
 // Walks the tiles in order, 32 groups at a time; every lane of the warp calls.
-// 32-bit arithmetic and one copy of the code for all roles: a launch of few
-// tiles is as long as its first instruction misses (with 64-bit divisions
-// inlined in each role, 10,000 cycles went by before the first copy).
+// 32-bit arithmetic throughout: a launch of few tiles pays for its first
+// instructions (with 64-bit divisions 10,000 cycles went by before the first
+// copy, now 4,000; as calls of one function 8,000).
 template <bool GRAD>
 struct Walk {
     int e0, before, total, lo, hi, first, tiles, it, jt;
@@ -182,7 +182,7 @@ struct Walk {
         first = inc - tiles;
         total = __shfl_sync(0xffffffffu, inc, P.E > 1 ? 31 : 0);
     }
-    __device__ __noinline__ void init(const TcArgs &P) {
+    __device__ __forceinline__ void init(const TcArgs &P) {
         it = (int)((P.I + 255) >> 8);
         jt = (int)((P.J + 255) >> 8);
         full = P.full;
@@ -206,7 +206,7 @@ struct Walk {
         return GRAD ? (T.hi - T.lo + 63) >> 6 : (int)((P.Kc + 63) >> 6);
     }
     // Work item u of a pair: a whole tile, or a part of one of the rest.
-    __device__ __noinline__ bool find(const TcArgs &P, int u, Tile &T) {
+    __device__ __forceinline__ bool find(const TcArgs &P, int u, Tile &T) {
         if (u < full || splits == 1) {
             if (!tile(P, u, T)) return false;
             T.kb0 = 0;
@@ -376,7 +376,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
     if (warp == 1) alloc_pair(smem_u32(&ctl->tmem), 512);
     fence_before();
     __syncthreads();
-    cluster_sync();
+    cluster_sync_relaxed();               // the barriers' set-up is fenced above
     fence_after();
     const uint32_t tmem = ctl->tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -735,7 +735,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 tc_drain(smem_u32(&ctl->full[s]), ((ctl->fills - 1 - s) / (uint32_t)P.stages) & 1u);
     }
     __syncthreads();
-    cluster_sync();
+    cluster_sync_relaxed();               // neither CTA's shared memory goes before the other is done
     if (warp == 1) {
         fence_after();
         dealloc_pair(tmem, 512);
