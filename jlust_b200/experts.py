@@ -32,7 +32,7 @@ _ACTS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "relu": _lib.ACT_RELU,
 # addresses go to ctypes as integers and each operand is looked at once.
 
 def _base(origin) -> int:
-    return _origin(origin).offset
+    return 0 if origin == 0 else _origin(origin).offset
 
 
 def _on(t: torch.Tensor) -> torch.device:
@@ -44,12 +44,19 @@ def _on(t: torch.Tensor) -> torch.device:
     return d
 
 
+# The current stream's handle without building a Stream object (2 us a call)
+# where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
 def _act(act) -> int:
@@ -94,29 +101,57 @@ def _index(t: torch.Tensor, n, what: str, like: torch.Tensor):
         raise _elsewhere(t, like, what)
 
 
-def _weight(w: torch.Tensor, what="w"):
-    """(E, K, N, leading dimension, expert stride, order) of E x K x N weights
-    whose matrices are row- or column-major."""
-    if w.dim() != 3:
-        raise IncompatibleExtents(f"{what} must be experts x K x N (got {tuple(w.shape)})")
-    E, K, N = w.shape
-    se, s0, s1 = w.stride()
+def _matrix(K, N, s0, s1, strides):
+    """(leading dimension, order) of a K x N matrix of strides s0, s1."""
     if (s1 == 1 or N <= 1) and (s0 >= N or K <= 1):
-        order, ld = _lib.ROW_MAJOR, (s0 if K > 1 else max(N, 1))
-    elif (s0 == 1 or K <= 1) and (s1 >= K or N <= 1):
-        order, ld = _lib.COL_MAJOR, (s1 if N > 1 else max(K, 1))
+        return (s0 if K > 1 else max(N, 1)), _lib.ROW_MAJOR
+    if (s0 == 1 or K <= 1) and (s1 >= K or N <= 1):
+        return (s1 if N > 1 else max(K, 1)), _lib.COL_MAJOR
+    raise IncompatibleExtents(f"w's matrices must be row- or column-major (strides {strides})")
+
+
+def _weight(w: torch.Tensor):
+    """(E, K, N, leading dimension, expert stride, order) of E x K x N weights,
+    or of one K x N matrix, row- or column-major."""
+    strides = w.stride()
+    if w.dim() == 3:
+        E, K, N = w.shape
+        ld, order = _matrix(K, N, strides[1], strides[2], strides)
+        if E > 1:
+            return E, K, N, ld, strides[0], order
+    elif w.dim() == 2:
+        E, (K, N) = 1, w.shape
+        ld, order = _matrix(K, N, strides[0], strides[1], strides)
     else:
-        raise IncompatibleExtents(f"{what}'s matrices must be row- or column-major "
-                                  f"(strides {w.stride()})")
-    return E, K, N, ld, (se if E > 1 else ld * (K if order == _lib.ROW_MAJOR else N)), order
+        raise IncompatibleExtents(f"w must be experts x K x N or K x N (got {tuple(w.shape)})")
+    return E, K, N, ld, ld * (K if order == _lib.ROW_MAJOR else N), order
+
+
+def _experts(w):
+    if w.dim() != 3:
+        raise IncompatibleExtents(f"w must be experts x K x N (got {tuple(w.shape)})")
+    return w
+
+
+def _dense(w):
+    if w.dim() != 2:
+        raise IncompatibleExtents(f"w must be K x N (got {tuple(w.shape)})")
+    return w
 
 
 def _bias(bias, E, N, w):
     if bias is None:
         return 0
-    if bias.dim() == 1:
-        bias = bias.unsqueeze(0)
-    return _rows(bias, E, N, "bias", w)
+    if bias.dim() == 2:
+        return _rows(bias, E, N, "bias", w)
+    if E != 1 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1):
+        raise IncompatibleExtents(f"bias is {tuple(bias.shape)}, expected {E} x {N} contiguous rows")
+    if bias.dtype != w.dtype:
+        raise UnsupportedValueType(f"bias: operands must share one value type ({bias.dtype}, "
+                                   f"{w.dtype})")
+    if bias.device != w.device:
+        raise _elsewhere(bias, w, "bias")
+    return max(N, 1)
 
 
 def _workspace(nbytes, device):
@@ -170,7 +205,7 @@ def route(ids: torch.Tensor, n_experts: int, origin=0) -> Routing:
     ws = _workspace(wsb, dev)
     n = T * k
     # one allocation for the three index buffers
-    buf = torch.empty(2 * n + max(E, 0) + 1, dtype=torch.int32, device=dev)
+    buf = ids.new_empty(2 * n + max(E, 0) + 1)
     slot, source, rowptr = buf[:n].view(T, k), buf[n:2 * n], buf[2 * n:]
     _lib.call("jlb_route", _stream(dev), base, T, k, E, _ptr(ids), _ptr(rowptr), _ptr(source),
               _ptr(slot), _ptr(ws), wsb)
@@ -204,7 +239,7 @@ def combine(z: torch.Tensor, routing: Routing, weights=None, out=None) -> torch.
     if routing.slot.device != dev:
         raise _elsewhere(routing.slot, z, "routing")
     if out is None:
-        out = torch.empty((T, N), dtype=z.dtype, device=dev)
+        out = z.new_empty((T, N))
     ldy = _rows(out, T, N, "out", z)
     _lib.call("jlb_combine", _stream(dev), dt, routing.origin.offset, T, k, S, N,
               _ptr(routing.slot), _ptr(g), _ptr(z), ldz, _ptr(out), ldy)
@@ -224,7 +259,7 @@ def combine_backward(dy: torch.Tensor, z: torch.Tensor, routing: Routing, weight
     dev = _on(z)
     if routing.slot.device != dev:
         raise _elsewhere(routing.slot, z, "routing")
-    dz = torch.empty((S, N), dtype=z.dtype, device=dev)
+    dz = z.new_empty((S, N))
     dg = torch.empty((T, k), dtype=torch.float32, device=dev)
     _lib.call("jlb_combine_backward", _stream(dev), dt, routing.origin.offset, T, k, S, N, E,
               _ptr(routing.rowptr), _ptr(routing.slot), _ptr(g), _ptr(z), ldz, _ptr(dy), lddy,
@@ -255,10 +290,10 @@ def _product(x, w3, rowptr, rows, bias, act, residual, keep_preact, out, base):
         _index(rows, S, "rows", x)
     ldb = _bias(bias, E, N, x)
     if out is None:
-        out = torch.empty((S, N), dtype=x.dtype, device=dev)
+        out = x.new_empty((S, N))
     ldy = _rows(out, S, N, "out", x)
     ldr = _rows(residual, S, N, "residual", x) if residual is not None else 0
-    z = torch.empty((S, N), dtype=x.dtype, device=dev) if keep_preact else None
+    z = x.new_empty((S, N)) if keep_preact else None
     gather = 0 if rows is None else 1
     wsb = _lib.load().jlb_grouped_mm_workspace_size(dt, E, S, T, K, N, _ptr(x), ldx, _ptr(w3), ldw,
                                                     sw, order, gather)
@@ -278,16 +313,14 @@ def grouped_matmul(x, w, rowptr, *, rows=None, bias=None, act=None, keep_preact=
     with the product before act, which the gradient needs."""
     if rowptr is None:
         raise InvalidArgument("grouped_matmul: rowptr is required")
-    return _product(x, w, rowptr, rows, bias, act, None, keep_preact, out, _base(origin))
+    return _product(x, _experts(w), rowptr, rows, bias, act, None, keep_preact, out, _base(origin))
 
 
 def fused_matmul(x, w, *, bias=None, act=None, residual=None, keep_preact=False, out=None):
     """y = act(x @ w + bias) + residual: x (M x K), w (K x N, row- or
     column-major), bias (N), residual (M x N).  keep_preact returns (y, z) with
     the product before act, which the gradient needs.  out may be residual."""
-    if w.dim() != 2:
-        raise IncompatibleExtents(f"w must be K x N (got {tuple(w.shape)})")
-    return _product(x, w.unsqueeze(0), None, None, bias, act, residual, keep_preact, out, 0)
+    return _product(x, _dense(w), None, None, bias, act, residual, keep_preact, out, 0)
 
 
 def _backward(dy, x, w3, rowptr, rows, z, act, need_bias, base):
@@ -337,10 +370,9 @@ def _backward(dy, x, w3, rowptr, rows, z, act, need_bias, base):
               _ptr(ws), wsb)
     # dw in w's own order
     if order == _lib.ROW_MAJOR:
-        dw = torch.empty((E, K, N), dtype=x.dtype, device=dev)
-        lddw = max(N, 1)
+        dw, lddw = x.new_empty(w3.shape), max(N, 1)
     else:
-        dw = torch.empty((E, N, K), dtype=x.dtype, device=dev).transpose(1, 2)
+        dw = x.new_empty((E, N, K) if w3.dim() == 3 else (N, K)).transpose(-2, -1)
         lddw = max(K, 1)
     gather = 0 if rows is None else 1
     wsb = L.jlb_grouped_mm_wgrad_workspace_size(dt, E, S, T, K, N, _ptr(x), ldx, _ptr(dz), lddz,
@@ -360,15 +392,13 @@ def grouped_matmul_backward(dy, x, w, rowptr, *, rows=None, z=None, act=None, bi
     dz[p] (None unless bias)."""
     if rowptr is None:
         raise InvalidArgument("grouped_matmul_backward: rowptr is required")
-    return _backward(dy, x, w, rowptr, rows, z, act, bias, _base(origin))
+    return _backward(dy, x, _experts(w), rowptr, rows, z, act, bias, _base(origin))
 
 
 def fused_matmul_backward(dy, x, w, *, z=None, act=None, bias=False):
     """Gradients of fused_matmul: (dx, dw, db); the residual's is dy itself."""
-    if w.dim() != 2:
-        raise IncompatibleExtents(f"w must be K x N (got {tuple(w.shape)})")
-    dx, dw, db = _backward(dy, x, w.unsqueeze(0), None, None, z, act, bias, 0)
-    return dx, dw[0], None if db is None else db[0]
+    dx, dw, db = _backward(dy, x, _dense(w), None, None, z, act, bias, 0)
+    return dx, dw, None if db is None else db[0]
 
 
 # ----------------------------------------------------------------- handles
@@ -380,9 +410,7 @@ class B200ProductHandle(AbstractKernelHandle):
     bias=, act=) with w K x N."""
 
     def __init__(self, w, *, grouped, bias=None, act=None, origin=0):
-        if not grouped and w.dim() != 2:
-            raise IncompatibleExtents(f"w must be K x N (got {tuple(w.shape)})")
-        w3 = w if grouped else w.unsqueeze(0)
+        w3 = _experts(w) if grouped else _dense(w)
         self.dtype = _type(w3, "product")
         self.E, self.K, self.N, ldw, sw, order = _weight(w3)
         self.device = _on(w3)
@@ -412,12 +440,12 @@ class B200ProductHandle(AbstractKernelHandle):
         elif rowptr is not None or rows is not None:
             raise InvalidArgument("a dense product takes no rowptr or rows")
         if out is None:
-            out = torch.empty((S, N), dtype=x.dtype, device=self.device)
+            out = x.new_empty((S, N))
             ldy = max(N, 1)
         else:
             ldy = _rows(out, S, N, "out", w)
         ldr = _rows(residual, S, N, "residual", w) if residual is not None else 0
-        z = torch.empty((S, N), dtype=x.dtype, device=self.device) if keep_preact else None
+        z = x.new_empty((S, N)) if keep_preact else None
         L = _lib.load()
         wsb = L.jlb_mm_plan_workspace_size(self._plan, S, T, _ptr(x), ldx, 0 if rows is None else 1)
         ws = _workspace(wsb, self.device)
