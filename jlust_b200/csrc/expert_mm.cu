@@ -2,8 +2,9 @@
 // bias, activation and residual in the epilogue, and their gradients.  The
 // dense product is the same call with one group.
 //
-// This file holds the entry points and the kernels without tensor cores:
-// single precision, and shapes the tensor path does not take.
+// This file holds the entry points, the copies that make operands fit the
+// tensor path (aligned rows of bf16, planes of F32) and the kernels without
+// tensor cores, for shapes the tensor path does not take.
 #include "expert_mm.cuh"
 
 #include <new>
@@ -334,6 +335,69 @@ align_rows(int64_t experts, int64_t rows, int64_t cols, const uint16_t *__restri
     }
 }
 
+// F32 rows as three bf16 planes, h + m + l = the value: h holds its upper 8
+// bits, m the next 8 and l the last 8.  Truncated, not rounded, so that h
+// cannot overflow and the three have one sign (an overflow stays an infinity).
+// Rows come through `rows` when given (an index outside the matrix: zeros).
+// An infinity or NaN goes to l, whose only partner is the other operand's h
+// (never 0 for a value of 2^-133 or more, +-1 for an infinity), with h = +-1
+// for an infinity there; in h it would meet zero m and l planes.
+__global__ void __launch_bounds__(256)
+split_rows(int64_t experts, int64_t rows, int64_t cols, const float *__restrict__ src, int64_t ld, int64_t stride,
+           const int32_t *__restrict__ idx, int base, int64_t limit, const int32_t *__restrict__ live_end,
+           __nv_bfloat16 *__restrict__ dst, int64_t ldd) {
+    const int64_t pieces = (cols + 127) / 128, all = experts * rows * pieces, plane = experts * rows * ldd;
+    const int lane = threadIdx.x % kWarp;
+    const int64_t end = live_end ? (int64_t)__ldg(live_end) - base : rows;
+    bool outside = false;
+    for (int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / kWarp; w < all; w += (int64_t)gridDim.x * 8) {
+        const int64_t r = w / pieces, c0 = (w - r * pieces) * 128 + 2 * lane;
+        const int64_t e = r / rows;
+        int64_t sr = r - e * rows;
+        const bool live = sr < end;               // rows of no group hold anything
+        if (idx && live) {
+            sr = (int64_t)__ldg(idx + sr) - base;
+            if (sr < 0 || sr >= limit) {
+                sr = -1;
+                outside = true;
+            }
+        }
+        const float *s = live && sr >= 0 ? src + e * stride + sr * ld : nullptr;
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t c = c0 + (q / 2) * 64 + q % 2;
+            v[q] = s && c < cols ? s[c] : 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+            const int64_t c = c0 + (q / 2) * 64;
+            if (c >= cols) continue;
+            __nv_bfloat162 o[3];
+            float h[2], m[2], l[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t u = __float_as_uint(v[q + x]);
+                h[x] = __uint_as_float(u & 0xffff0000u);
+                const float rest = v[q + x] - h[x];
+                m[x] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+                l[x] = rest - m[x];
+                if ((u & 0x7f800000u) == 0x7f800000u) {
+                    h[x] = copysignf(1.0f, v[q + x]);
+                    m[x] = 0.0f;
+                    l[x] = v[q + x];
+                }
+            }
+            o[0] = __floats2bfloat162_rn(h[0], h[1]);
+            o[1] = __floats2bfloat162_rn(m[0], m[1]);
+            o[2] = __floats2bfloat162_rn(l[0], l[1]);
+#pragma unroll
+            for (int x = 0; x < 3; ++x) *reinterpret_cast<__nv_bfloat162 *>(dst + x * plane + r * ldd + c) = o[x];
+        }
+    }
+    if (outside) dev_error(DEV_ERR_BOUNDS);
+}
+
 static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 static size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 static bool tma_rows(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
@@ -347,30 +411,45 @@ static int align_copy(cudaStream_t st, int64_t experts, int64_t rows, int64_t co
     return JLB_OK;
 }
 
-// The tensor path of a product: which operands need an aligned copy, and
-// where the workspace holds them (parts of split tiles first).
+static int split_copy(cudaStream_t st, int64_t experts, int64_t rows, int64_t cols, const void *src, int64_t ld,
+                      int64_t stride, const int32_t *idx, int base, int64_t limit, const int32_t *live_end,
+                      void *dst) {
+    const int64_t warps = experts * rows * ceil_div(cols, 128), blocks = ceil_div(warps, 8);
+    split_rows<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(
+        experts, rows, cols, (const float *)src, ld, stride, idx, base, limit, live_end, (__nv_bfloat16 *)dst,
+        pad8(cols));
+    JLB_LAUNCH_CHECK("split_rows");
+    return JLB_OK;
+}
+
+// The tensor path of a product: which operands need an aligned copy (BF16) or
+// are split into planes (F32), and where the workspace holds them (after the
+// parts of split tiles).
 struct ProductPlan {
-    bool tc, copy_x, copy_w;
+    bool tc, split, copy_x, copy_w;
     size_t x_at, w_at, bytes;
     Product p;              // with the copies' leading dimensions
 };
 static ProductPlan plan_product(const Product &P) {
     ProductPlan q{};
     q.p = P;
-    if (P.dtype != JLB_BF16 || P.K == 0 || P.N == 0 || P.S == 0 || P.T == 0 || P.E == 0 || skinny_ok(P)) return q;
+    if (P.K == 0 || P.N == 0 || P.S == 0 || P.T == 0 || P.E == 0 || skinny_ok(P)) return q;
     const int64_t inner = P.w_order == JLB_ROW_MAJOR ? P.N : P.K, outer = P.w_order == JLB_ROW_MAJOR ? P.K : P.N;
+    q.split = P.dtype == JLB_F32;
+    const int64_t planes = q.split ? 3 : 1, xrows = q.split ? P.S : P.T;   // planes of gathered rows
+    if (planes * xrows > INT32_MAX / 2 || planes * P.E > INT32_MAX / 2) return q;
     q.tc = true;
-    q.copy_x = !tma_rows(P.x, P.ldx);
-    q.copy_w = !tma_rows(P.w, P.ldw) || (P.E > 1 && P.w_stride % 8);
+    q.copy_x = q.split || !tma_rows(P.x, P.ldx);
+    q.copy_w = q.split || !tma_rows(P.w, P.ldw) || (P.E > 1 && P.w_stride % 8);
     q.bytes = pad256(tc_product_workspace(P));
     if (q.copy_x) {
         q.x_at = q.bytes;
-        q.bytes += pad256((size_t)P.T * pad8(P.K) * 2);
+        q.bytes += pad256((size_t)(planes * xrows * pad8(P.K)) * 2);
         q.p.ldx = pad8(P.K);
     }
     if (q.copy_w) {
         q.w_at = q.bytes;
-        q.bytes += pad256((size_t)P.E * outer * pad8(inner) * 2);
+        q.bytes += pad256((size_t)(planes * P.E * outer * pad8(inner)) * 2);
         q.p.ldw = pad8(inner);
         q.p.w_stride = outer * pad8(inner);
     }
@@ -383,19 +462,26 @@ static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_by
     if (q.tc) {
         if (q.bytes && (!ws || ws_bytes < q.bytes))
             return fail(JLB_ERR_WORKSPACE, "the product needs %zu workspace bytes", q.bytes);
-        if (q.copy_x) {
-            q.p.x = (char *)ws + q.x_at;
-            const int r = align_copy(st, 1, P.T, P.K, P.x, P.ldx, 0, (char *)ws + q.x_at);
-            if (r) return r;
+        const bool row = P.w_order == JLB_ROW_MAJOR;
+        char *base = (char *)ws;
+        int r = JLB_OK;
+        if (q.split) {
+            r = split_copy(st, 1, P.S, P.K, P.x, P.ldx, 0, P.rows, P.base, P.T, P.rowptr ? P.rowptr + P.E : nullptr,
+                           base + q.x_at);
+            if (!r)
+                r = split_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride, nullptr, 0, 0, nullptr,
+                               base + q.w_at);
+            q.p.rows = nullptr;
+            q.p.T = P.S;
+        } else {
+            if (q.copy_x) r = align_copy(st, 1, P.T, P.K, P.x, P.ldx, 0, base + q.x_at);
+            if (!r && q.copy_w)
+                r = align_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride, base + q.w_at);
         }
-        if (q.copy_w) {
-            const bool row = P.w_order == JLB_ROW_MAJOR;
-            q.p.w = (char *)ws + q.w_at;
-            const int r = align_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride,
-                                     (char *)ws + q.w_at);
-            if (r) return r;
-        }
-        const int r = tc_product(st, q.p, ws);
+        if (r) return r;
+        if (q.copy_x) q.p.x = base + q.x_at;
+        if (q.copy_w) q.p.w = base + q.w_at;
+        r = tc_product(st, q.p, base);
         if (r >= 0) return r;
     }
     const int64_t ntiles = ceil_div(P.N, kTile), rtiles = row_tiles_bound(P.E, P.S, P.rowptr, kTile);
@@ -408,26 +494,29 @@ static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_by
 }
 
 struct GradientPlan {
-    bool tc, copy_x, copy_d;
+    bool tc, split, copy_x, copy_d;
     size_t x_at, d_at, bytes;
     Gradient g;
 };
 static GradientPlan plan_gradient(const Gradient &G) {
     GradientPlan q{};
     q.g = G;
-    if (G.dtype != JLB_BF16 || G.S == 0 || G.T == 0 || G.E == 0 || G.K == 0 || G.N == 0) return q;
+    if (G.S == 0 || G.T == 0 || G.E == 0 || G.K == 0 || G.N == 0) return q;
+    q.split = G.dtype == JLB_F32;
+    const int64_t planes = q.split ? 3 : 1, xrows = q.split ? G.S : G.T;
+    if (planes * xrows > INT32_MAX / 2 || planes * G.S > INT32_MAX / 2) return q;
     q.tc = true;
-    q.copy_x = !tma_rows(G.x, G.ldx);
-    q.copy_d = !tma_rows(G.dz, G.lddz);
+    q.copy_x = q.split || !tma_rows(G.x, G.ldx);
+    q.copy_d = q.split || !tma_rows(G.dz, G.lddz);
     q.bytes = pad256(tc_gradient_workspace(G));
     if (q.copy_x) {
         q.x_at = q.bytes;
-        q.bytes += pad256((size_t)G.T * pad8(G.K) * 2);
+        q.bytes += pad256((size_t)(planes * xrows * pad8(G.K)) * 2);
         q.g.ldx = pad8(G.K);
     }
     if (q.copy_d) {
         q.d_at = q.bytes;
-        q.bytes += pad256((size_t)G.S * pad8(G.N) * 2);
+        q.bytes += pad256((size_t)(planes * G.S * pad8(G.N)) * 2);
         q.g.lddz = pad8(G.N);
     }
     return q;
@@ -438,17 +527,22 @@ static int run_gradient(cudaStream_t st, const Gradient &G, void *ws, size_t ws_
     if (q.tc) {
         if (q.bytes && (!ws || ws_bytes < q.bytes))
             return fail(JLB_ERR_WORKSPACE, "the gradient needs %zu workspace bytes", q.bytes);
-        if (q.copy_x) {
-            q.g.x = (char *)ws + q.x_at;
-            const int r = align_copy(st, 1, G.T, G.K, G.x, G.ldx, 0, (char *)ws + q.x_at);
-            if (r) return r;
+        char *base = (char *)ws;
+        int r = JLB_OK;
+        if (q.split) {
+            const int32_t *end = G.rowptr ? G.rowptr + G.E : nullptr;
+            r = split_copy(st, 1, G.S, G.K, G.x, G.ldx, 0, G.rows, G.base, G.T, end, base + q.x_at);
+            if (!r) r = split_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, nullptr, G.base, 0, end, base + q.d_at);
+            q.g.rows = nullptr;
+            q.g.T = G.S;
+        } else {
+            if (q.copy_x) r = align_copy(st, 1, G.T, G.K, G.x, G.ldx, 0, base + q.x_at);
+            if (!r && q.copy_d) r = align_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, base + q.d_at);
         }
-        if (q.copy_d) {
-            q.g.dz = (char *)ws + q.d_at;
-            const int r = align_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, (char *)ws + q.d_at);
-            if (r) return r;
-        }
-        const int r = tc_gradient(st, q.g, ws);
+        if (r) return r;
+        if (q.copy_x) q.g.x = base + q.x_at;
+        if (q.copy_d) q.g.dz = base + q.d_at;
+        r = tc_gradient(st, q.g, base);
         if (r >= 0) return r;
     }
     const bool col = G.w_order == JLB_COL_MAJOR;

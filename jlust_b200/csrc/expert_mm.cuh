@@ -44,8 +44,8 @@ struct Gradient {
 };
 
 // The tensor-core kernels (expert_mm_tc.cu), bf16 operands of 16-byte aligned
-// rows: the workspace of their split tiles, and the launch; -1 when the driver
-// refuses a tensor map.
+// rows, or F32 ones as three planes of bf16: the workspace of their split
+// tiles, and the launch; -1 when the driver refuses a tensor map.
 size_t tc_product_workspace(const Product &P);
 int tc_product(cudaStream_t st, const Product &P, void *ws);
 size_t tc_gradient_workspace(const Gradient &G);

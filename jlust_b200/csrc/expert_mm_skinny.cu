@@ -102,7 +102,7 @@ __device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0
         // U loads are on their way before the first is used
         if (!COL) {
             constexpr int KY = kSkThreads / LX;    // rows of W a pass
-            constexpr int U = MR <= 2 ? 8 : 4;
+            constexpr int U = 8;
             const int ky = threadIdx.x / LX, n = (int)min((int64_t)VEC, P.N - (n0 + lx * VEC));
             const T *p = w + kc * P.ldw + n0 + lx * VEC;
             for (int kb = ky; kb < kn && n > 0; kb += U * KY) {
@@ -243,11 +243,12 @@ product_skinny(const __grid_constant__ Product P, int splits) {
 }
 
 // Few rows: one or two in bf16, where the tensor path is as fast from there
-// on; F32 up to 16 rows, or two a group.
+// on; F32 up to 8 rows, or two a group, where
+// splitting W into planes for the tensor path costs more than its products.
 bool skinny_ok(const Product &P) {
     if (P.E > 65535 || P.K == 0) return false;
     if (P.dtype == JLB_BF16) return P.S <= 2;
-    return P.S <= (P.rowptr ? 2 * P.E : 16) && P.S <= 4096;
+    return P.S <= (P.rowptr ? 2 * P.E : 8) && P.S <= 4096;
 }
 
 template <typename T, bool COL, int VEC, int MAXR>

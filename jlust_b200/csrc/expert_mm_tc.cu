@@ -1,6 +1,15 @@
 // expert_mm_tc.cu -- the grouped products on sm_100a tensor cores (bf16
 // operands, fp32 sums): tcgen05 products of CTA pairs, operands staged by TMA.
 //
+// F32 operands come as three bf16 planes, x = h + m + l exactly (8 bits each),
+// and six of the nine products of planes are summed: l h, h l, m m, m h, h m,
+// h h; what is left out is below 2^-24 of a term.  The tensor cores' fp32 sums
+// truncate (measured here: a relative bias of 3.7e-6 after 4096 terms, where
+// fp32 FMAs have an error of 2e-7), so a chain of them is kept to 64 inner
+// elements, small products first: each 64-wide step's sums are read from TMEM
+// and added in registers, rounded to nearest.  An infinity or NaN sits in the
+// l plane (with h = +-1), which meets the other operand's h plane alone.
+//
 // Orientation.  An output matrix out[j][i] (i contiguous in memory) is
 // computed as D (256 lanes i) x (up to 256 columns j): the instruction's M is
 // fixed at 256 and its N is a run-time field in steps of 32, so the ragged
@@ -75,10 +84,11 @@ struct TcArgs {
     int gather;                   // product: 1 = B's rows; gradient: 1 = A's, 2 = B's
     int vec;                      // out, z and res allow 16-byte vectors
     const __nv_bfloat16 *ga, *gb; // the operands' matrices, for the loader warps
+    int pa, pb;                   // F32: coordinate from an operand's plane to the next (A of a product: experts)
     int64_t lda, ldb_;
-    const __nv_bfloat16 *bias, *res;
+    const void *bias, *res;       // of the value type
     int64_t ldb, ldr;
-    __nv_bfloat16 *z, *out;
+    void *z, *out;
     int64_t ldz, ldo, out_stride;
     int stages, bn_max;
     int a_pair, b_pair;           // mA / mBig: both 64-wide boxes of an operand in one copy
@@ -184,7 +194,7 @@ struct Walk {
     }
     __device__ __forceinline__ void init(const TcArgs &P) {
         it = (int)((P.I + 255) >> 8);
-        jt = (int)((P.J + 255) >> 8);
+        jt = GRAD ? (int)((unsigned)(P.J + P.bn_max - 1) / (unsigned)P.bn_max) : 1;
         full = P.full;
         splits = P.splits;
         if (P.max_splits > 1) {       // a product whose tiles only rowptr tells
@@ -237,7 +247,7 @@ struct Walk {
         T.hi = __shfl_sync(0xffffffffu, hi, src);
         const int l = want - __shfl_sync(0xffffffffu, first, src);
         // column tiles j, in blocks of kJBlock, lane tiles i inside a block
-        const int cw = GRAD ? 256 : col_width(T.hi - T.lo, P.bn_max);
+        const int cw = GRAD ? P.bn_max : col_width(T.hi - T.lo, P.bn_max);
         const int n = GRAD ? jt : (int)((unsigned)(T.hi - T.lo + cw - 1) / (unsigned)cw);
         int i = l, j = 0;
         if (n > 1) {
@@ -248,7 +258,7 @@ struct Walk {
         }
         T.i0 = i * 256;
         T.j0 = j * cw;
-        if (GRAD) T.bn = P.J - T.j0 > 128 ? 256 : 128;
+        if (GRAD) T.bn = P.bn_max > 128 && P.J - T.j0 > 128 ? 256 : 128;
         else T.bn = min(cw, (T.hi - T.lo - T.j0 + 31) & ~31);
         return true;
     }
@@ -307,6 +317,37 @@ __device__ __forceinline__ void store32(const float (&v)[32], uint32_t *turn, bo
     __syncwarp();
 }
 
+// The 32 columns of F32 results, v[c] = out[row0 + c][i] of every lane: 128
+// contiguous bytes a store.
+__device__ __forceinline__ void store32_f32(const float (&v)[32], float *out, int64_t ld, int64_t row0, int n,
+                                            int64_t i, int64_t I) {
+    if (i >= I) return;
+    float *o = out + row0 * ld + i;
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+        if (c < n) o[c * ld] = v[c];
+}
+
+// The epilogue of 32 columns of F32 sums.
+template <bool GRAD>
+__device__ __forceinline__ void finish32_f32(const TcArgs &P, float (&v)[32], int64_t row0, int n, int64_t i,
+                                             float bias, float *out) {
+    if (!GRAD) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] += bias;
+        if (P.z) store32_f32(v, (float *)P.z, P.ldz, row0, n, i, P.I);
+#pragma unroll 4
+        for (int c = 0; c < 32; ++c) v[c] = act_value<float>(v[c], P.act);
+        if (P.res && i < P.I) {
+            const float *q = (const float *)P.res + row0 * P.ldr + i;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                if (c < n) v[c] = add_rn(v[c], q[c * P.ldr]);
+        }
+    }
+    store32_f32(v, out, P.ldo, row0, n, i, P.I);
+}
+
 // Every second 32-column chunk of the tile's columns [0, nj), from chunk
 // `first` on, of this warp's 32 lanes; column c is output row row0 + c.
 template <int ACT, bool GRAD>
@@ -325,11 +366,11 @@ __device__ __forceinline__ void store_tile(const TcArgs &P, uint32_t taddr, uint
 #pragma unroll
         for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(r[c]) + (GRAD ? 0.0f : bias);
         if (!GRAD) {
-            if (P.z) store32(v, turn, vec, P.z, P.ldz, row0 + c0, n, ib, P.I);
+            if (P.z) store32(v, turn, vec, (__nv_bfloat16 *)P.z, P.ldz, row0 + c0, n, ib, P.I);
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] = act_value<__nv_bfloat16>(v[c], ACT);
             if (P.res && i < P.I) {
-                const __nv_bfloat16 *q = P.res + (row0 + c0) * P.ldr + i;
+                const __nv_bfloat16 *q = (const __nv_bfloat16 *)P.res + (row0 + c0) * P.ldr + i;
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
                     if (c < n) v[c] = add_rn(v[c], __bfloat162float(q[c * P.ldr]));
@@ -340,10 +381,12 @@ __device__ __forceinline__ void store_tile(const TcArgs &P, uint32_t taddr, uint
     __syncwarp();
 }
 
-template <bool A_MN, bool GRAD>
+template <bool A_MN, bool GRAD, typename T_>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads + kLoaders + kForward, 1)
 product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB,
            const __grid_constant__ CUtensorMap mBig, const __grid_constant__ TcArgs P) {
+    constexpr bool F32 = sizeof(T_) == 4;
+    constexpr int kPlanes = F32 ? 3 : 1;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t tiles_u32 = (raw + 1023u) & ~1023u;
@@ -397,32 +440,34 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             const int bh = T.bn / 2, boxes = (bh + 31) / 32;           // product: B's rows, in 32-row boxes
             const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
             const int nb = T.bn / 128, bj0 = T.j0 + (int)rank * bh;    // gradient: B's 64-column boxes
-            for (int kb = T.kb0; lane == 0 && kb < T.kb1; ++kb) {
+            for (int k = T.kb0 * kPlanes; lane == 0 && k < T.kb1 * kPlanes; ++k) {
+                const int kb = k / kPlanes, plane = k - kb * kPlanes;
                 if (!tc_wait(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
                 {
                     const uint32_t sA = tiles_u32 + (uint32_t)stage * stage_bytes, sB = sA + kABytes;
                     const uint32_t full = full0 + (uint32_t)stage * 8u;
                     if (!GRAD) {
+                        const int e = T.e + plane * P.pa, r0 = (int)b0 + plane * P.pb;
                         if (rank == 0)
                             mbar_expect_tx(smem_u32(&ctl->full[stage]),
                                            2u * (kABytes + (P.gather ? 0u : (uint32_t)boxes * 4096u)));
                         if (!A_MN) {
-                            tma_3d(sA, &mA, full, kb * 64, a0, T.e);
+                            tma_3d(sA, &mA, full, kb * 64, a0, e);
                         } else if (P.a_pair) {
-                            tma_4d(sA, &mA, full, 0, kb * 64, a0 / 64, T.e);
+                            tma_4d(sA, &mA, full, 0, kb * 64, a0 / 64, e);
                         } else {
-                            tma_3d(sA, &mA, full, a0, kb * 64, T.e);
-                            tma_3d(sA + kBox, &mA, full, a0 + 64, kb * 64, T.e);
+                            tma_3d(sA, &mA, full, a0, kb * 64, e);
+                            tma_3d(sA + kBox, &mA, full, a0 + 64, kb * 64, e);
                         }
                         if (boxes == 4 && !P.gather)
-                            tma_2d(sB, &mBig, full, kb * 64, (int)b0);
+                            tma_2d(sB, &mBig, full, kb * 64, r0);
                         else if (!P.gather)
                             for (int x = 0; x < boxes; ++x)
-                                tma_2d(sB + (uint32_t)x * 4096u, &mB, full, kb * 64, (int)b0 + 32 * x);
+                                tma_2d(sB + (uint32_t)x * 4096u, &mB, full, kb * 64, r0 + 32 * x);
                     } else {
                         const bool tail = T.hi - T.lo - kb * 64 < 64;
                         const bool ta = !tail && P.gather != 1, tb = !tail && P.gather != 2;
-                        const int p0 = T.lo + kb * 64;
+                        const int pa = T.lo + kb * 64 + plane * P.pa, pb = T.lo + kb * 64 + plane * P.pb;
                         if (rank == 0)
                             mbar_expect_tx(smem_u32(&ctl->full[stage]),
                                            2u * ((ta ? kABytes : 0u) + (tb ? (uint32_t)nb * kBox : 0u)));
@@ -430,16 +475,16 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                             mbar_arrive_count(smem_u32(&ctl->full[stage]), 2);
                         if (tail && !P.gather) mbar_arrive_count(smem_u32(&ctl->go[stage]), 1);
                         if (ta && P.a_pair) {
-                            tma_3d(sA, &mA, full, 0, p0, a0 / 64);
+                            tma_3d(sA, &mA, full, 0, pa, a0 / 64);
                         } else if (ta) {
-                            tma_2d(sA, &mA, full, a0, p0);
-                            tma_2d(sA + kBox, &mA, full, a0 + 64, p0);
+                            tma_2d(sA, &mA, full, a0, pa);
+                            tma_2d(sA + kBox, &mA, full, a0 + 64, pa);
                         }
                         if (tb && nb == 2 && P.b_pair)
-                            tma_3d(sB, &mBig, full, 0, p0, bj0 / 64);
+                            tma_3d(sB, &mBig, full, 0, pb, bj0 / 64);
                         else if (tb)
                             for (int x = 0; x < nb; ++x)
-                                tma_2d(sB + (uint32_t)x * kBox, &mB, full, bj0 + 64 * x, p0);
+                                tma_2d(sB + (uint32_t)x * kBox, &mB, full, bj0 + 64 * x, pb);
                     }
                 }
                 ++fills;
@@ -473,24 +518,55 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             Tile T;
             for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
                 if (T.kb0 == T.kb1) continue;                 // the epilogue writes zeros
-                if (!tc_wait_warp(smem_u32(&ctl->tempty[buf]), te[buf], abort_flag)) break;
-                te[buf] ^= 1u;
-                fence_after();
                 const uint32_t idesc = instr_desc(256, (uint32_t)T.bn, A_MN, GRAD);
-                if (lane == 0)
-                    for (int kb = T.kb0; kb < T.kb1; ++kb) {
-                        if (!tc_wait(smem_u32(&ctl->full[stage]), pf, abort_flag)) { ok = false; break; }
+                auto mma = [&](uint32_t a_off, uint32_t b_off, uint32_t first) {
+                    mma_pair_k64<A_MN ? 128 : 2, GRAD ? 128 : 2>(tmem + (uint32_t)buf * 256u, (uint32_t)a_desc + a_off,
+                                                                 (uint32_t)(a_desc >> 32), (uint32_t)b_desc + b_off,
+                                                                 (uint32_t)(b_desc >> 32), idesc, first);
+                };
+                if (!F32) {
+                    if (!tc_wait_warp(smem_u32(&ctl->tempty[buf]), te[buf], abort_flag)) break;
+                    te[buf] ^= 1u;
+                    fence_after();
+                    if (lane == 0)
+                        for (int kb = T.kb0; kb < T.kb1; ++kb) {
+                            if (!tc_wait(smem_u32(&ctl->full[stage]), pf, abort_flag)) { ok = false; break; }
+                            fence_after();
+                            const uint32_t off = ((uint32_t)stage * stage_bytes) >> 4;
+                            mma(off, off, (uint32_t)(kb - T.kb0));
+                            commit_pair(smem_u32(&ctl->empty[stage]));
+                            if (++stage == P.stages) { stage = 0; pf ^= 1u; }
+                        }
+                    if (lane == 0 && ok) commit_pair(smem_u32(&ctl->tfull[buf]));
+                    buf ^= 1;
+                } else if (lane == 0) {
+                    // a 64-wide step: its three planes' stages, then six products into a fresh accumulator
+                    for (int kb = T.kb0; ok && kb < T.kb1; ++kb) {
+                        ok = tc_wait(smem_u32(&ctl->tempty[buf]), te[buf], abort_flag);
+                        te[buf] ^= 1u;
+                        uint32_t off[3], bar[3];
+#pragma unroll
+                        for (int q = 0; q < 3; ++q) {
+                            ok = ok && tc_wait(smem_u32(&ctl->full[stage]), pf, abort_flag);
+                            off[q] = ((uint32_t)stage * stage_bytes) >> 4;
+                            bar[q] = smem_u32(&ctl->empty[stage]);
+                            if (++stage == P.stages) { stage = 0; pf ^= 1u; }
+                        }
+                        if (!ok) break;
                         fence_after();
-                        const uint32_t off = ((uint32_t)stage * stage_bytes) >> 4;
-                        mma_pair_k64<A_MN ? 128 : 2, GRAD ? 128 : 2>(tmem + (uint32_t)buf * 256u, (uint32_t)a_desc + off,
-                                                                     (uint32_t)(a_desc >> 32), (uint32_t)b_desc + off,
-                                                                     (uint32_t)(b_desc >> 32), idesc, (uint32_t)(kb - T.kb0));
-                        commit_pair(smem_u32(&ctl->empty[stage]));
-                        if (++stage == P.stages) { stage = 0; pf ^= 1u; }
+                        mma(off[2], off[0], 0u);
+                        mma(off[0], off[2], 1u);
+                        mma(off[1], off[1], 1u);
+                        mma(off[1], off[0], 1u);
+                        mma(off[0], off[1], 1u);
+                        mma(off[0], off[0], 1u);
+#pragma unroll
+                        for (int q = 0; q < 3; ++q) commit_pair(bar[q]);
+                        commit_pair(smem_u32(&ctl->tfull[buf]));
+                        buf ^= 1;
                     }
-                if (lane == 0 && ok) commit_pair(smem_u32(&ctl->tfull[buf]));
+                }
                 ok = __all_sync(0xffffffffu, ok);
-                buf ^= 1;
             }
             if (lane == 0) commit_pair(smem_u32(&ctl->done));
             __syncwarp();
@@ -509,8 +585,8 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             group_rows(P.rowptr, P.base, P.S, P.E - 1, lo, hi);
             for (int64_t r = (int64_t)hi + blockIdx.x; r < P.S; r += gridDim.x)
                 for (int64_t c = threadIdx.x - 64; c < P.I; c += kEpiWarps * 32) {
-                    P.out[r * P.ldo + c] = __float2bfloat16_rn(0.0f);
-                    if (P.z) P.z[r * P.ldz + c] = __float2bfloat16_rn(0.0f);
+                    ((T_ *)P.out)[r * P.ldo + c] = from_f32<T_>(0.0f);
+                    if (P.z) ((T_ *)P.z)[r * P.ldz + c] = from_f32<T_>(0.0f);
                 }
         }
         Walk<GRAD> walk;
@@ -521,16 +597,59 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             // column 0's row of the output, and its columns
             const int64_t row0 = GRAD ? T.j0 : (int64_t)T.lo + T.j0;
             const int nj = GRAD ? (int)min((int64_t)T.bn, P.J - T.j0) : min(T.bn, T.hi - T.lo - T.j0);
-            __nv_bfloat16 *out = P.out + (GRAD ? T.e * P.out_stride : 0);
+            T_ *out = (T_ *)P.out + (GRAD ? T.e * P.out_stride : 0);
             float *part = T.part >= 0 ? P.part + (int64_t)T.part * 256 * P.bn_max + (ib - T.i0) + lane : nullptr;
             if (T.kb0 == T.kb1) {
                 for (int c = first; c < nj; c += 2) {
                     if (part) part[c * 256] = 0.0f;
-                    else if (ib + lane < P.I) out[(row0 + c) * P.ldo + ib + lane] = __float2bfloat16_rn(0.0f);
+                    else if (ib + lane < P.I) out[(row0 + c) * P.ldo + ib + lane] = from_f32<T_>(0.0f);
                 }
                 continue;
             }
-            const float bias = !GRAD && P.bias && ib + lane < P.I ? __bfloat162float(P.bias[T.e * P.ldb + ib + lane]) : 0.0f;
+            const float bias = !GRAD && P.bias && ib + lane < P.I ? to_f32(((const T_ *)P.bias)[T.e * P.ldb + ib + lane]) : 0.0f;
+            if constexpr (F32) {
+                // this warp's columns 32 first .. and 64 + 32 first .., step after step
+                float acc[2][32];
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) acc[q][c] = 0.0f;
+                bool ok = true;
+                for (int kb = T.kb0; kb < T.kb1; ++kb) {
+                    ok = tc_wait_warp(smem_u32(&ctl->tfull[buf]), tf[buf], abort_flag);
+                    if (!ok) break;
+                    tf[buf] ^= 1u;
+                    fence_after();
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int c0 = first * 32 + q * 64;
+                        if (c0 >= nj) continue;
+                        uint32_t r[32];
+                        __syncwarp();
+                        JLB_TC_LD32(tmem + ((uint32_t)(qd * 32) << 16) + (uint32_t)(buf * 256 + c0), r);
+                        wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) acc[q][c] += __uint_as_float(r[c]);
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(te0 + (uint32_t)buf * 8u);
+                    buf ^= 1;
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int c0 = first * 32 + q * 64;
+                    if (c0 >= nj) continue;
+                    if (part) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) part[(c0 + c) * 256] = acc[q][c];
+                    } else {
+                        finish32_f32<GRAD>(P, acc[q], row0 + c0, nj - c0, ib + lane, bias, (float *)out);
+                    }
+                }
+                continue;
+            }
             if (!tc_wait_warp(smem_u32(&ctl->tfull[buf]), tf[buf], abort_flag)) break;
             tf[buf] ^= 1u;
             fence_after();
@@ -546,10 +665,10 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 }
             } else if (ib < P.I) {
                 switch (GRAD ? JLB_ACT_NONE : P.act) {
-                    case JLB_ACT_RELU: store_tile<JLB_ACT_RELU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
-                    case JLB_ACT_SILU: store_tile<JLB_ACT_SILU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
-                    case JLB_ACT_GELU: store_tile<JLB_ACT_GELU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out); break;
-                    default: store_tile<JLB_ACT_NONE, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, out);
+                    case JLB_ACT_RELU: store_tile<JLB_ACT_RELU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, (__nv_bfloat16 *)out); break;
+                    case JLB_ACT_SILU: store_tile<JLB_ACT_SILU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, (__nv_bfloat16 *)out); break;
+                    case JLB_ACT_GELU: store_tile<JLB_ACT_GELU, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, (__nv_bfloat16 *)out); break;
+                    default: store_tile<JLB_ACT_NONE, GRAD>(P, taddr, turn, first, row0, nj, ib, bias, (__nv_bfloat16 *)out);
                 }
             }
             fence_before();
@@ -574,7 +693,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Tile T;
         for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
             const int bh = T.bn / 2, nb = T.bn / 128;
-            if (!GRAD) {
+            if (!GRAD && !F32) {
                 // the (at most 8) rows of B this lane copies 16 bytes of
                 const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
                 const __nv_bfloat16 *row[8];
@@ -636,7 +755,8 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 }
             };
             if (P.gather) fetch(T.kb0);
-            for (int kb = T.kb0; kb < T.kb1; ++kb) {
+            for (int k = T.kb0 * kPlanes; k < T.kb1 * kPlanes; ++k) {
+                const int kb = k / kPlanes, plane = k - kb * kPlanes;
                 // (without gather only a group's last step is loaded; the copy
                 // thread, which waits for every stage, says when: a wait for
                 // the stage's own barrier could be laps of the ring early)
@@ -674,8 +794,8 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
 #pragma unroll
                 for (int op = 0; op < 2; ++op) {
                     if (!(op ? lb : la)) continue;
-                    const __nv_bfloat16 *m = op ? P.gb : P.ga;
                     const int64_t ld = op ? P.ldb_ : P.lda, col = op ? cb : ca;
+                    const __nv_bfloat16 *m = (op ? P.gb : P.ga) + (int64_t)plane * (op ? P.pb : P.pa) * ld;
                     const bool g = P.gather == 1 + op;
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
@@ -710,8 +830,8 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         walk.init(P);
         Tile T;
         for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
-            for (int kb = T.kb0; kb < T.kb1; ++kb) {
-                if (!GRAD || P.gather || T.hi - T.lo - kb * 64 < 64) {
+            for (int k = T.kb0 * kPlanes; k < T.kb1 * kPlanes; ++k) {
+                if (!GRAD || P.gather || T.hi - T.lo - k / kPlanes * 64 < 64) {
                     if (!tc_wait_warp(smem_u32(&ctl->rows[stage]), (pr >> stage) & 1u, abort_flag)) { ok = false; break; }
                     pr ^= 1u << stage;
                     if (lane == 0) {
@@ -747,7 +867,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
 // parts of them are loaded before any is added.  Launched
 // while product_tc runs; the wait ends when that grid is complete.
 constexpr int kFinish = 4;
-template <bool GRAD>
+template <bool GRAD, typename T_>
 __global__ void __launch_bounds__(256) finish_tc(const __grid_constant__ TcArgs P) {
     __shared__ Tile ts;
     __shared__ int ns;
@@ -770,8 +890,8 @@ __global__ void __launch_bounds__(256) finish_tc(const __grid_constant__ TcArgs 
     const int64_t i = (int64_t)T.i0 + threadIdx.x, item = (int64_t)256 * P.bn_max;
     if (i >= P.I || c0 >= nj) return;
     const float *part = P.part + (int64_t)blockIdx.y * ns * item + threadIdx.x;
-    const float bias = !GRAD && P.bias ? __bfloat162float(P.bias[T.e * P.ldb + i]) : 0.0f;
-    __nv_bfloat16 *out = P.out + (GRAD ? T.e * P.out_stride : 0) + i;
+    const float bias = !GRAD && P.bias ? to_f32(((const T_ *)P.bias)[T.e * P.ldb + i]) : 0.0f;
+    T_ *out = (T_ *)P.out + (GRAD ? T.e * P.out_stride : 0) + i;
     const int64_t row0 = GRAD ? T.j0 : (int64_t)T.lo + T.j0;
     float sum[kFinish] = {};
     for (int s0 = 0; s0 < ns; s0 += 4) {
@@ -794,11 +914,11 @@ __global__ void __launch_bounds__(256) finish_tc(const __grid_constant__ TcArgs 
         const int64_t r = row0 + c;
         if (!GRAD) {
             v += bias;
-            if (P.z) P.z[r * P.ldz + i] = __float2bfloat16_rn(v);
-            v = act_value<__nv_bfloat16>(v, P.act);
-            if (P.res) v = add_rn(v, __bfloat162float(P.res[r * P.ldr + i]));
+            if (P.z) ((T_ *)P.z)[r * P.ldz + i] = from_f32<T_>(v);
+            v = act_value<T_>(v, P.act);
+            if (P.res) v = add_rn(v, to_f32(((const T_ *)P.res)[r * P.ldr + i]));
         }
-        out[r * P.ldo] = __float2bfloat16_rn(v);
+        out[r * P.ldo] = from_f32<T_>(v);
     }
 }
 
@@ -884,7 +1004,7 @@ static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, int64_t steps) {
     return p;
 }
 
-template <bool A_MN, bool GRAD>
+template <bool A_MN, bool GRAD, typename T_>
 static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &big, TcArgs &P,
                      const TcPlan &plan, void *ws, bool loaders) {
     const size_t extra = 1024 + kTurnBytes + sizeof(TcCtl);
@@ -898,8 +1018,8 @@ static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b
     P.stages = (int)((227 * 1024 - extra) / stage);
     if (P.stages > kMaxStages) P.stages = kMaxStages;
     const size_t smem = (size_t)P.stages * stage + extra;
-    JLB_CUDA(cudaFuncSetAttribute(product_tc<A_MN, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    product_tc<A_MN, GRAD><<<(unsigned)(2 * P.pairs), kTcThreads + (loaders ? kLoaders + kForward : 0), smem, st>>>(a, b, big, P);
+    JLB_CUDA(cudaFuncSetAttribute(product_tc<A_MN, GRAD, T_>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    product_tc<A_MN, GRAD, T_><<<(unsigned)(2 * P.pairs), kTcThreads + (loaders ? kLoaders + kForward : 0), smem, st>>>(a, b, big, P);
     JLB_LAUNCH_CHECK("product_tc");
     if (plan.finish) {
         cudaLaunchConfig_t cfg{};
@@ -911,13 +1031,15 @@ static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b
         cfg.stream = st;
         cfg.attrs = at;
         cfg.numAttrs = 1;
-        JLB_CUDA(cudaLaunchKernelEx(&cfg, finish_tc<GRAD>, P));
+        JLB_CUDA(cudaLaunchKernelEx(&cfg, finish_tc<GRAD, T_>, P));
     }
     return ok();
 }
 
+static int widest(int dtype) { return dtype == JLB_F32 ? 128 : 256; }   // F32: sums in registers
+
 static TcPlan plan_product(const Product &p) {
-    const int bn = p.S >= 256 ? 256 : (int)((p.S + 31) / 32 * 32);
+    const int wide = widest(p.dtype), bn = p.S >= wide ? wide : (int)((p.S + 31) / 32 * 32);
     if (!p.rowptr)
         return tc_plan(bn, col_tiles((int)p.S, bn) * ceil_div(p.N, 256), true, ceil_div(p.K, 64));
     const int64_t cols = ceil_div(p.S, bn) + (p.E < p.S ? p.E : p.S);
@@ -926,22 +1048,28 @@ static TcPlan plan_product(const Product &p) {
 
 static TcPlan plan_gradient(const Gradient &g) {
     const int64_t J = g.w_order == JLB_ROW_MAJOR ? g.K : g.N, I = g.w_order == JLB_ROW_MAJOR ? g.N : g.K;
-    return tc_plan(J > 128 ? 256 : 128, g.E * ceil_div(I, 256) * ceil_div(J, 256), true, ceil_div(g.S / g.E, 64));
+    const int bn = J > 128 ? widest(g.dtype) : 128;
+    return tc_plan(bn, g.E * ceil_div(I, 256) * ceil_div(J, bn), true, ceil_div(g.S / g.E, 64));
 }
 
 size_t tc_product_workspace(const Product &P) { return plan_product(P).part_bytes; }
 size_t tc_gradient_workspace(const Gradient &G) { return plan_gradient(G).part_bytes; }
 
 // Status, or -1 when the driver refuses a tensor map (the caller takes
-// another kernel).
+// another kernel).  F32: p.x and p.w are three bf16 planes each, [3][T][ldx]
+// and [3][E] matrices, bias, res, z and y are F32.
 int tc_product(cudaStream_t st, const Product &p, void *ws) {
+    const int planes = p.dtype == JLB_F32 ? 3 : 1;
     CUtensorMap a, b, big;
     const bool mn = p.w_order == JLB_ROW_MAJOR;
-    const int64_t w_stride = p.E > 1 ? p.w_stride : (mn ? p.K : p.N) * p.ldw;
-    const bool pair = mn && make_pair_map(&a, p.w, p.N, p.K, p.ldw, p.E, w_stride);
-    if (!pair && !(mn ? make_map(&a, p.w, p.N, p.K, p.ldw, p.E, w_stride, 64) : make_map(&a, p.w, p.K, p.N, p.ldw, p.E, w_stride, 128)))
+    const int64_t experts = p.E * planes, w_stride = experts > 1 ? p.w_stride : (mn ? p.K : p.N) * p.ldw;
+    const bool pair = mn && make_pair_map(&a, p.w, p.N, p.K, p.ldw, experts, w_stride);
+    if (!pair && !(mn ? make_map(&a, p.w, p.N, p.K, p.ldw, experts, w_stride, 64)
+                      : make_map(&a, p.w, p.K, p.N, p.ldw, experts, w_stride, 128)))
         return -1;
-    if (!make_map(&b, p.x, p.K, p.T, p.ldx, 0, 0, 32) || !make_map(&big, p.x, p.K, p.T, p.ldx, 0, 0, 128)) return -1;
+    if (!make_map(&b, p.x, p.K, p.T * planes, p.ldx, 0, 0, 32) ||
+        !make_map(&big, p.x, p.K, p.T * planes, p.ldx, 0, 0, 128))
+        return -1;
     TcArgs P{};
     P.base = p.base;
     P.act = p.act;
@@ -954,32 +1082,40 @@ int tc_product(cudaStream_t st, const Product &p, void *ws) {
     P.rows = p.rows;
     P.gather = p.rows ? 1 : 0;
     P.a_pair = pair;
+    P.pa = (int)p.E;
+    P.pb = (int)p.T;
     P.gb = (const __nv_bfloat16 *)p.x;
     P.ldb_ = p.ldx;
-    P.bias = (const __nv_bfloat16 *)p.bias;
+    P.bias = p.bias;
     P.ldb = p.ldb;
-    P.res = (const __nv_bfloat16 *)p.res;
+    P.res = p.res;
     P.ldr = p.ldr;
-    P.z = (__nv_bfloat16 *)p.z;
+    P.z = p.z;
     P.ldz = p.ldz;
-    P.out = (__nv_bfloat16 *)p.y;
+    P.out = p.y;
     P.ldo = p.ldy;
-    P.vec = tma_matrix(p.y, p.ldy) && (!p.z || tma_matrix(p.z, p.ldz)) && (!p.res || tma_matrix(p.res, p.ldr));
+    P.vec = tma_matrix(p.y, p.ldy) && (!p.z || tma_matrix(p.z, p.ldz));
     const TcPlan plan = plan_product(p);
     if (plan.pairs < 1 || (p.rowptr ? p.E : 1) * ceil_div(p.N, 256) * ceil_div(p.S, 32) > INT32_MAX / 2) return -1;
-    return mn ? launch_tc<true, false>(st, a, b, big, P, plan, ws, p.rows)
-              : launch_tc<false, false>(st, a, b, big, P, plan, ws, p.rows);
+    if (p.dtype == JLB_F32)
+        return mn ? launch_tc<true, false, float>(st, a, b, big, P, plan, ws, false)
+                  : launch_tc<false, false, float>(st, a, b, big, P, plan, ws, false);
+    return mn ? launch_tc<true, false, __nv_bfloat16>(st, a, b, big, P, plan, ws, p.rows)
+              : launch_tc<false, false, __nv_bfloat16>(st, a, b, big, P, plan, ws, p.rows);
 }
 
 int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     // dw row-major: lanes = columns n (dz), columns = k (x); column-major: exchanged
+    const int planes = g.dtype == JLB_F32 ? 3 : 1;
     const bool row = g.w_order == JLB_ROW_MAJOR;
     const void *ap = row ? g.dz : g.x, *bp = row ? g.x : g.dz;
     const int64_t ac = row ? g.N : g.K, ar = row ? g.S : g.T, lda = row ? g.lddz : g.ldx;
     const int64_t bc = row ? g.K : g.N, br = row ? g.T : g.S, ldb = row ? g.ldx : g.lddz;
     CUtensorMap a, b, big;
-    const bool a_pair = make_pair_map(&a, ap, ac, ar, lda, 0, 0), b_pair = make_pair_map(&big, bp, bc, br, ldb, 0, 0);
-    if ((!a_pair && !make_map(&a, ap, ac, ar, lda, 0, 0, 64)) || !make_map(&b, bp, bc, br, ldb, 0, 0, 64)) return -1;
+    const bool a_pair = make_pair_map(&a, ap, ac, ar * planes, lda, 0, 0),
+               b_pair = make_pair_map(&big, bp, bc, br * planes, ldb, 0, 0);
+    if ((!a_pair && !make_map(&a, ap, ac, ar * planes, lda, 0, 0, 64)) || !make_map(&b, bp, bc, br * planes, ldb, 0, 0, 64))
+        return -1;
     if (!b_pair) big = b;
     TcArgs P{};
     P.base = g.base;
@@ -989,6 +1125,8 @@ int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     P.J = bc;
     P.a_pair = a_pair;
     P.b_pair = b_pair;
+    P.pa = (int)ar;
+    P.pb = (int)br;
     P.glimit = g.T;
     P.rowptr = g.rowptr;
     P.rows = g.rows;
@@ -998,11 +1136,12 @@ int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     P.gb = (const __nv_bfloat16 *)bp;
     P.ldb_ = ldb;
     P.vec = tma_matrix(g.dw, g.lddw) && (g.E == 1 || g.dw_stride % 8 == 0);
-    P.out = (__nv_bfloat16 *)g.dw;
+    P.out = g.dw;
     P.ldo = g.lddw;
     P.out_stride = g.dw_stride;
-    if (P.E * ceil_div(P.I, 256) * ceil_div(P.J, 256) > INT32_MAX / 2) return -1;
-    return launch_tc<true, true>(st, a, b, big, P, plan_gradient(g), ws, true);
+    if (P.E * ceil_div(P.I, 256) * ceil_div(P.J, 128) > INT32_MAX / 2) return -1;
+    return g.dtype == JLB_F32 ? launch_tc<true, true, float>(st, a, b, big, P, plan_gradient(g), ws, true)
+                              : launch_tc<true, true, __nv_bfloat16>(st, a, b, big, P, plan_gradient(g), ws, true);
 }
 
 }  // namespace emm
