@@ -208,34 +208,106 @@ __global__ void __launch_bounds__(kSimtThreads) gradient_simt(const Gradient G) 
 
 // ------------------------------------------------- activation's gradient
 // dz = dy * act'(z), and the column sums of each group's dz (the bias's
-// gradient) over kSumRows rows a CTA: 64 columns x 4 row lanes.  Sums of
-// unrounded products in fp32; a second kernel adds a group's parts in order.
-constexpr int kSumRows = 128, kSumCols = 64;
-template <typename T>
-__global__ void __launch_bounds__(256)
+// gradient) over kSumRows rows a CTA: 32 threads of V columns (16 bytes, or
+// one where the layout is not aligned) x 8 row lanes, four rows' loads on
+// their way at a time.  Sums of unrounded products in fp32: a lane's rows,
+// then the 8 lanes in order; sum_parts adds a group's CTAs in order.  Bound by
+// HBM.
+constexpr int kSumRows = 128;
+template <typename T, int V>
+struct Values {                    // as they lie in memory, until they are used
+    uint4 q;
+    T one;
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (V == 1) one = *p;
+        else q = *reinterpret_cast<const uint4 *>(p);
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (V == 1) return to_f32(one);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        return sizeof(T) == 4 ? __uint_as_float(w[i % 4])
+                              : __uint_as_float(i % 2 ? w[i / 2 % 4] & 0xffff0000u : w[i / 2 % 4] << 16);
+    }
+};
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T *p, const float (&v)[V]) {
+    if constexpr (V == 1) {
+        *p = from_f32<T>(v[0]);
+    } else {
+        __align__(16) T o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = from_f32<T>(v[i]);
+        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(o);
+    }
+}
+
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void act_rows(int lo, int hi, int64_t c, const T *__restrict__ dy, int64_t lddy,
+                                         const T *__restrict__ z, int64_t ldz, T *__restrict__ dz, int64_t lddz,
+                                         float (&sum)[V]) {
+    constexpr int U = 4;
+    for (int r0 = lo + threadIdx.x / 32; r0 < hi; r0 += 8 * U) {
+        Values<T, V> d[U], q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = r0 + 8 * u;
+            if (r < hi) {
+                d[u].load(dy + r * lddy + c);
+                if (ACT != JLB_ACT_NONE) q[u].load(z + r * ldz + c);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = r0 + 8 * u;
+            if (r >= hi) break;
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[i] = d[u].get(i);
+                if (ACT != JLB_ACT_NONE) v[i] *= act_slope<T>(q[u].get(i), ACT);
+                sum[i] += v[i];
+            }
+            if (dz) store_v<T, V>(dz + r * lddz + c, v);
+        }
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256, 4)
 act_backward(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__ rowptr, int act,
              const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z, int64_t ldz,
              T *__restrict__ dz, int64_t lddz, float *__restrict__ part) {
     __shared__ Found f;
-    __shared__ float red[4][kSumCols];
+    __shared__ float red[8][32 * V];
     find_row_tile(rowptr, base, S, E, kSumRows, blockIdx.y, &f);
     __syncthreads();
     if (f.e < 0) return;
-    const int cx = threadIdx.x % kSumCols, ry = threadIdx.x / kSumCols;
-    const int64_t c = (int64_t)blockIdx.x * kSumCols + cx;
-    float sum = 0.0f;
-    if (c < N)
-        for (int r = f.row0 + ry; r < f.hi && r < f.row0 + kSumRows; r += 4) {
-            float d = to_f32(dy[(int64_t)r * lddy + c]);
-            if (z) d *= act_slope<T>(to_f32(z[(int64_t)r * ldz + c]), act);
-            if (dz) dz[(int64_t)r * lddz + c] = from_f32<T>(d);
-            sum += d;
+    const int cx = threadIdx.x % 32;
+    const int64_t c = ((int64_t)blockIdx.x * 32 + cx) * V;
+    const int hi = min(f.hi, f.row0 + kSumRows);
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+    if (c < N) {
+        switch (act) {
+            case JLB_ACT_RELU: act_rows<T, V, JLB_ACT_RELU>(f.row0, hi, c, dy, lddy, z, ldz, dz, lddz, sum); break;
+            case JLB_ACT_SILU: act_rows<T, V, JLB_ACT_SILU>(f.row0, hi, c, dy, lddy, z, ldz, dz, lddz, sum); break;
+            case JLB_ACT_GELU: act_rows<T, V, JLB_ACT_GELU>(f.row0, hi, c, dy, lddy, z, ldz, dz, lddz, sum); break;
+            default: act_rows<T, V, JLB_ACT_NONE>(f.row0, hi, c, dy, lddy, z, ldz, dz, lddz, sum);
         }
+    }
     if (!part) return;
-    red[ry][cx] = sum;
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[threadIdx.x / 32][cx * V + i] = sum[i];
     __syncthreads();
-    if (ry == 0 && c < N)
-        part[(int64_t)blockIdx.y * N + c] = (red[0][cx] + red[1][cx]) + (red[2][cx] + red[3][cx]);
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+        const int64_t col = (int64_t)blockIdx.x * 32 * V + i;
+        if (col >= N) continue;
+        float s = red[0][i];
+#pragma unroll
+        for (int q = 1; q < 8; ++q) s += red[q][i];
+        part[(int64_t)blockIdx.y * N + col] = s;
+    }
 }
 
 template <typename T>
@@ -265,8 +337,27 @@ sum_parts(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= N) return;
     float s = 0.0f;
+#pragma unroll 8
     for (int i = 0; i < count_s; ++i) s += part[(first_s + i) * N + c];
     db[e * lddb + c] = from_f32<T>(s);
+}
+
+template <typename T>
+static int launch_act(cudaStream_t st, int64_t tiles, int64_t E, int64_t S, int64_t N, int base, const int32_t *rowptr,
+                      int act, const void *dy, int64_t lddy, const void *z, int64_t ldz, void *dz, int64_t lddz,
+                      float *part) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool vec = N % V == 0 && lddy % V == 0 && aligned16(dy) && (!z || (ldz % V == 0 && aligned16(z))) &&
+                     (!dz || (lddz % V == 0 && aligned16(dz)));
+    const dim3 grid((unsigned)ceil_div(N, vec ? 32 * V : 32), (unsigned)tiles);
+    if (vec)
+        act_backward<T, V><<<grid, 256, 0, st>>>(E, S, N, base, rowptr, act, (const T *)dy, lddy, (const T *)z, ldz,
+                                                 (T *)dz, lddz, part);
+    else
+        act_backward<T, 1><<<grid, 256, 0, st>>>(E, S, N, base, rowptr, act, (const T *)dy, lddy, (const T *)z, ldz,
+                                                 (T *)dz, lddz, part);
+    JLB_LAUNCH_CHECK("act_backward");
+    return JLB_OK;
 }
 
 static int64_t row_tiles_bound(int64_t E, int64_t S, bool ragged, int size) {
@@ -313,26 +404,48 @@ static int check_act(int act) {
 }
 
 // ------------------------------------------------- copies for the tensor path
-// Rows of bf16 whose leading dimension or address TMA cannot take, copied to a
-// leading dimension of a multiple of 8: a warp moves 256 neighbouring elements
-// of a row, 64 bytes a load whatever the alignment.
+// Rows of bf16 copied to a leading dimension of a multiple of 8: those whose
+// leading dimension or address TMA cannot take, and the gradient's gathered
+// rows (idx; an index outside the matrix: a row of zeros; rows from *live_end
+// on are of no group and left out).  A warp moves 256 neighbouring elements of
+// a row: 16 bytes a lane where the source is aligned, else 64 bytes a load.
 __global__ void __launch_bounds__(256)
 align_rows(int64_t experts, int64_t rows, int64_t cols, const uint16_t *__restrict__ src, int64_t ld,
-           int64_t stride, uint16_t *__restrict__ dst, int64_t ldd) {
+           int64_t stride, const int32_t *__restrict__ idx, int base, int64_t limit,
+           const int32_t *__restrict__ live_end, int vec, uint16_t *__restrict__ dst, int64_t ldd) {
     const int64_t pieces = (cols + 255) / 256, all = experts * rows * pieces;
     const int lane = threadIdx.x % kWarp;
+    const int64_t end = live_end ? (int64_t)__ldg(live_end) - base : rows;
+    bool outside = false;
     for (int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / kWarp; w < all; w += (int64_t)gridDim.x * 8) {
-        const int64_t r = w / pieces, c0 = (w - r * pieces) * 256 + lane;
+        const int64_t r = w / pieces, p0 = (w - r * pieces) * 256;
         const int64_t e = r / rows;
-        const uint16_t *s = src + e * stride + (r - e * rows) * ld;
+        int64_t sr = r - e * rows;
+        if (sr >= end) continue;
+        if (idx) {
+            sr = (int64_t)__ldg(idx + sr) - base;
+            if (sr < 0 || sr >= limit) {
+                sr = -1;
+                outside = true;
+            }
+        }
+        const uint16_t *s = src + e * stride + (sr < 0 ? 0 : sr) * ld;
         uint16_t *d = dst + r * ldd;
+        if (vec && p0 + 256 <= cols) {
+            const uint4 z = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(d + p0 + 8 * lane) =
+                sr < 0 ? z : __ldg(reinterpret_cast<const uint4 *>(s + p0 + 8 * lane));
+            continue;
+        }
+        const int64_t c0 = p0 + lane;
         uint16_t v[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = c0 + q * 32 < cols ? s[c0 + q * 32] : (uint16_t)0;
+        for (int q = 0; q < 8; ++q) v[q] = sr >= 0 && c0 + q * 32 < cols ? s[c0 + q * 32] : (uint16_t)0;
 #pragma unroll
         for (int q = 0; q < 8; ++q)
             if (c0 + q * 32 < cols) d[c0 + q * 32] = v[q];
     }
+    if (outside) dev_error(DEV_ERR_BOUNDS);
 }
 
 // F32 rows as three bf16 planes, h + m + l = the value: h holds its upper 8
@@ -403,10 +516,13 @@ static size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 static bool tma_rows(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 
 static int align_copy(cudaStream_t st, int64_t experts, int64_t rows, int64_t cols, const void *src, int64_t ld,
-                      int64_t stride, void *dst) {
+                      int64_t stride, const int32_t *idx, int base, int64_t limit, const int32_t *live_end,
+                      void *dst) {
     const int64_t warps = experts * rows * ceil_div(cols, 256), blocks = ceil_div(warps, 8);
+    const int vec = tma_rows(src, ld) && (experts == 1 || stride % 8 == 0);
     align_rows<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(
-        experts, rows, cols, (const uint16_t *)src, ld, stride, (uint16_t *)dst, pad8(cols));
+        experts, rows, cols, (const uint16_t *)src, ld, stride, idx, base, limit, live_end, vec, (uint16_t *)dst,
+        pad8(cols));
     JLB_LAUNCH_CHECK("align_rows");
     return JLB_OK;
 }
@@ -474,9 +590,10 @@ static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_by
             q.p.rows = nullptr;
             q.p.T = P.S;
         } else {
-            if (q.copy_x) r = align_copy(st, 1, P.T, P.K, P.x, P.ldx, 0, base + q.x_at);
+            if (q.copy_x) r = align_copy(st, 1, P.T, P.K, P.x, P.ldx, 0, nullptr, 0, 0, nullptr, base + q.x_at);
             if (!r && q.copy_w)
-                r = align_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride, base + q.w_at);
+                r = align_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride, nullptr, 0, 0, nullptr,
+                               base + q.w_at);
         }
         if (r) return r;
         if (q.copy_x) q.p.x = base + q.x_at;
@@ -503,10 +620,12 @@ static GradientPlan plan_gradient(const Gradient &G) {
     q.g = G;
     if (G.S == 0 || G.T == 0 || G.E == 0 || G.K == 0 || G.N == 0) return q;
     q.split = G.dtype == JLB_F32;
-    const int64_t planes = q.split ? 3 : 1, xrows = q.split ? G.S : G.T;
-    if (planes * xrows > INT32_MAX / 2 || planes * G.S > INT32_MAX / 2) return q;
+    const int64_t planes = q.split ? 3 : 1, xrows = G.S;
+    if (planes * G.S > INT32_MAX / 2) return q;
     q.tc = true;
-    q.copy_x = q.split || !tma_rows(G.x, G.ldx);
+    // gathered rows are copied too: every tile of the group reads them, by TMA
+    // from the copy at 1.3 PFLOP/s, by row loads at 0.85 (8192 x 4096 x 4096)
+    q.copy_x = q.split || G.rows || !tma_rows(G.x, G.ldx);
     q.copy_d = q.split || !tma_rows(G.dz, G.lddz);
     q.bytes = pad256(tc_gradient_workspace(G));
     if (q.copy_x) {
@@ -528,16 +647,18 @@ static int run_gradient(cudaStream_t st, const Gradient &G, void *ws, size_t ws_
         if (q.bytes && (!ws || ws_bytes < q.bytes))
             return fail(JLB_ERR_WORKSPACE, "the gradient needs %zu workspace bytes", q.bytes);
         char *base = (char *)ws;
+        const int32_t *end = G.rowptr ? G.rowptr + G.E : nullptr;
         int r = JLB_OK;
         if (q.split) {
-            const int32_t *end = G.rowptr ? G.rowptr + G.E : nullptr;
             r = split_copy(st, 1, G.S, G.K, G.x, G.ldx, 0, G.rows, G.base, G.T, end, base + q.x_at);
             if (!r) r = split_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, nullptr, G.base, 0, end, base + q.d_at);
+        } else {
+            if (q.copy_x) r = align_copy(st, 1, G.S, G.K, G.x, G.ldx, 0, G.rows, G.base, G.T, end, base + q.x_at);
+            if (!r && q.copy_d) r = align_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, nullptr, 0, 0, nullptr, base + q.d_at);
+        }
+        if (q.copy_x) {
             q.g.rows = nullptr;
             q.g.T = G.S;
-        } else {
-            if (q.copy_x) r = align_copy(st, 1, G.T, G.K, G.x, G.ldx, 0, base + q.x_at);
-            if (!r && q.copy_d) r = align_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, base + q.d_at);
         }
         if (r) return r;
         if (q.copy_x) q.g.x = base + q.x_at;
@@ -697,7 +818,7 @@ extern "C" JLB_API size_t jlb_grouped_mm_wgrad_workspace_size(int dtype, int64_t
                                                               const void *x, int64_t ldx,
                                                               const void *dz, int64_t lddz,
                                                               int w_order, int gather) {
-    (void)gather;
+    static const int32_t some = 0;
     if (E < 0 || S < 0 || T < 0 || K < 0 || N < 0) return 0;
     emm::Gradient G{};
     G.dtype = dtype;
@@ -711,6 +832,7 @@ extern "C" JLB_API size_t jlb_grouped_mm_wgrad_workspace_size(int dtype, int64_t
     G.dz = dz;
     G.lddz = lddz;
     G.w_order = w_order;
+    G.rows = gather ? &some : nullptr;
     return emm::plan_gradient(G).bytes;
 }
 
@@ -764,16 +886,10 @@ extern "C" JLB_API int jlb_act_backward(void *stream, int dtype, int idx_base, i
     if (tiles > 65535 || E > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent too large");
     float *part = db ? (float *)workspace : nullptr;
     if (tiles > 0) {
-        const dim3 grid((unsigned)ceil_div(N, emm::kSumCols), (unsigned)tiles);
-        if (dtype == JLB_F32)
-            emm::act_backward<float><<<grid, 256, 0, st>>>(
-                E, S, N, idx_base, rowptr, act, (const float *)dy, lddy, (const float *)z, ldz,
-                (float *)dz, lddz, part);
-        else
-            emm::act_backward<__nv_bfloat16><<<grid, 256, 0, st>>>(
-                E, S, N, idx_base, rowptr, act, (const __nv_bfloat16 *)dy, lddy,
-                (const __nv_bfloat16 *)z, ldz, (__nv_bfloat16 *)dz, lddz, part);
-        JLB_LAUNCH_CHECK("act_backward");
+        r = dtype == JLB_F32 ? emm::launch_act<float>(st, tiles, E, S, N, idx_base, rowptr, act, dy, lddy, z, ldz, dz, lddz, part)
+                             : emm::launch_act<__nv_bfloat16>(st, tiles, E, S, N, idx_base, rowptr, act, dy, lddy, z, ldz,
+                                                              dz, lddz, part);
+        if (r) return r;
     }
     if (db) {
         const dim3 grid((unsigned)ceil_div(N, 256), (unsigned)E);

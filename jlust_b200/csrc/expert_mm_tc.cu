@@ -30,10 +30,11 @@
 // through shared memory as pairs of columns, so that a thread then holds 8
 // neighbouring i of two rows and stores 16-byte vectors.
 //
-// Gathered rows and ragged sums.  Rows fetched through `rows`, and the
-// gradient's last 64-row step of a group, which must not see the next group's
-// rows (they may hold NaN), are copied by four loader warps: 16-byte cp.async
-// into the swizzled places a TMA box would fill, absent rows zero-filled.
+// Gathered rows and ragged sums.  A product's rows fetched through `rows`, and
+// the gradient's last 64-row step of a group, which must not see the next
+// group's rows (they may hold NaN), are copied by four loader warps: 16-byte
+// cp.async into the swizzled places a TMA box would fill, absent rows
+// zero-filled.
 // (TMA row gathers, four rows a copy, ran at 88 cycles a copy: 2549 us for the
 // 8192 x 4096 x 16384 product against 1007 us without the gather.)
 //
@@ -68,7 +69,6 @@ constexpr int kTcThreads = 64 + kEpiWarps * 32;         // without the loaders
 constexpr int kLoadWarp = 2 + kEpiWarps, kLoaders = 128;  // the loader warps
 constexpr int kForward = 32;                            // the warp that reports the loaders' stages
 constexpr int kPitch = 36;                              // words a pair of columns takes in the epilogue's turn
-constexpr int kAhead = 8;                               // gradient: stages of row indices read at a time
 constexpr uint32_t kTurnBytes = kEpiWarps * 16 * kPitch * 4;
 constexpr int kMaxStages = 10;
 constexpr uint32_t kABytes = 128 * 128;                 // 128 lanes x 64 inner, a CTA's half of A
@@ -81,7 +81,7 @@ struct TcArgs {
     int64_t E, S, I, J, Kc;       // I: lanes' extent; J: columns' extent (gradient); Kc: inner (product)
     int64_t glimit;               // rows the gathered matrix has
     const int32_t *rowptr, *rows;
-    int gather;                   // product: 1 = B's rows; gradient: 1 = A's, 2 = B's
+    int gather;                   // product: B's rows come through rows
     int vec;                      // out, z and res allow 16-byte vectors
     const __nv_bfloat16 *ga, *gb; // the operands' matrices, for the loader warps
     int pa, pb;                   // F32: coordinate from an operand's plane to the next (A of a product: experts)
@@ -101,7 +101,6 @@ struct TcArgs {
 __host__ __device__ inline uint32_t stage_size(int bn_max) { return kABytes + (uint32_t)((bn_max / 2 + 31) / 32) * 4096u; }
 
 struct TcCtl {
-    int idx[kLoaders / 32][kAhead * 16];          // a loader warp's rows, -1: none
     uint64_t full[kMaxStages], empty[kMaxStages], rows[kMaxStages], go[kMaxStages];
     uint64_t tfull[2], tempty[2], done;
     uint32_t tmem, fills;
@@ -466,23 +465,23 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                                 tma_2d(sB + (uint32_t)x * 4096u, &mB, full, kb * 64, r0 + 32 * x);
                     } else {
                         const bool tail = T.hi - T.lo - kb * 64 < 64;
-                        const bool ta = !tail && P.gather != 1, tb = !tail && P.gather != 2;
                         const int pa = T.lo + kb * 64 + plane * P.pa, pb = T.lo + kb * 64 + plane * P.pb;
                         if (rank == 0)
                             mbar_expect_tx(smem_u32(&ctl->full[stage]),
-                                           2u * ((ta ? kABytes : 0u) + (tb ? (uint32_t)nb * kBox : 0u)));
-                        if (rank == 0 && ta && tb)             // no rows to load: their arrivals
+                                           tail ? 0u : 2u * (kABytes + (uint32_t)nb * kBox));
+                        if (rank == 0 && !tail)                // no rows to load: their arrivals
                             mbar_arrive_count(smem_u32(&ctl->full[stage]), 2);
-                        if (tail && !P.gather) mbar_arrive_count(smem_u32(&ctl->go[stage]), 1);
-                        if (ta && P.a_pair) {
+                        if (tail) {                            // the loaders' turn
+                            mbar_arrive_count(smem_u32(&ctl->go[stage]), 1);
+                        } else if (P.a_pair) {
                             tma_3d(sA, &mA, full, 0, pa, a0 / 64);
-                        } else if (ta) {
+                        } else {
                             tma_2d(sA, &mA, full, a0, pa);
                             tma_2d(sA + kBox, &mA, full, a0 + 64, pa);
                         }
-                        if (tb && nb == 2 && P.b_pair)
+                        if (!tail && nb == 2 && P.b_pair)
                             tma_3d(sB, &mBig, full, 0, pb, bj0 / 64);
-                        else if (tb)
+                        else if (!tail)
                             for (int x = 0; x < nb; ++x)
                                 tma_2d(sB + (uint32_t)x * kBox, &mB, full, bj0 + 64 * x, pb);
                     }
@@ -736,74 +735,33 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 }
                 continue;
             }
-            // gradient: rows lw*4 + sub + 16*n (n < 4) of every step, both operands
+            // gradient: rows lw*4 + sub + 16*n (n < 4) of the group's last step,
+            // both operands.  The copy thread, which waits for every stage,
+            // says when: a wait for the stage's own barrier could be laps of
+            // the ring early, the steps between not being waited for here.
             const int64_t ca = (int64_t)T.i0 + rank * 128 + c8 * 8, cb = (int64_t)T.j0 + rank * bh + c8 * 8;
             const uint32_t qa[2] = {bytes_at(ca, P.I), bytes_at(ca + 64, P.I)};
             const uint32_t qb[2] = {bytes_at(cb, P.J), nb == 2 ? bytes_at(cb + 64, P.J) : 0u};
-            int ahead[kAhead * 16 / kWarp];
-            // the warp's row indices of steps k0 .. k0 + kAhead - 1, -1 where none
-            auto fetch = [&](int k0) {
-#pragma unroll
-                for (int n = 0; n < kAhead * 16 / kWarp; ++n) {
-                    const int q = n * kWarp + lane, r = q % 16;
-                    const int64_t p = (int64_t)T.lo + (k0 + q / 16) * 64 + lw * 4 + (r / 4) * 16 + r % 4;
-                    ahead[n] = p < T.hi ? __ldg(P.rows + p) - P.base : -1;
-                    if (p < T.hi && (ahead[n] < 0 || ahead[n] >= P.glimit)) {
-                        bad = true;
-                        ahead[n] = -1;
-                    }
-                }
-            };
-            if (P.gather) fetch(T.kb0);
             for (int k = T.kb0 * kPlanes; k < T.kb1 * kPlanes; ++k) {
                 const int kb = k / kPlanes, plane = k - kb * kPlanes;
-                // (without gather only a group's last step is loaded; the copy
-                // thread, which waits for every stage, says when: a wait for
-                // the stage's own barrier could be laps of the ring early)
-                // the indices of kAhead steps are kept in shared memory, the
-                // next ones' loads already on their way: a load in every step
-                // would wait for the step's copies before it
-                const bool tail = T.hi - T.lo - kb * 64 < 64;
-                const bool la = tail || P.gather == 1, lb = tail || P.gather == 2;
-                const int ka = (kb - T.kb0) % kAhead;
-                if (P.gather && ka == 0) {
-                    __syncwarp();
-#pragma unroll
-                    for (int n = 0; n < kAhead * 16 / kWarp; ++n) ctl->idx[lw][n * kWarp + lane] = ahead[n];
-                    __syncwarp();
-                    if (kb + kAhead < T.kb1) fetch(kb + kAhead);
-                }
-                if (!la && !lb) {
-                    if (++stage == P.stages) { stage = 0; pe ^= 1u; }
+                if (T.hi - T.lo - kb * 64 >= 64) {
+                    if (++stage == P.stages) stage = 0;
                     continue;
                 }
-                int sg[4], sp[4];                         // gathered and plain rows
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const int p = T.lo + kb * 64 + lw * 4 + n * 16 + sub;
-                    sp[n] = p < T.hi ? p : -1;
-                    sg[n] = P.gather ? ctl->idx[lw][ka * 16 + n * 4 + sub] : sp[n];
-                }
-                if (!(P.gather ? tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)
-                               : tc_wait_warp(smem_u32(&ctl->go[stage]), pgo >> stage & 1u, abort_flag))) {
-                    ok = false;
-                    break;
-                }
+                if (!tc_wait_warp(smem_u32(&ctl->go[stage]), pgo >> stage & 1u, abort_flag)) { ok = false; break; }
                 pgo ^= 1u << stage;               // a bit a stage: its next go comes after its release
                 const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + at0;
 #pragma unroll
                 for (int op = 0; op < 2; ++op) {
-                    if (!(op ? lb : la)) continue;
                     const int64_t ld = op ? P.ldb_ : P.lda, col = op ? cb : ca;
                     const __nv_bfloat16 *m = (op ? P.gb : P.ga) + (int64_t)plane * (op ? P.pb : P.pa) * ld;
-                    const bool g = P.gather == 1 + op;
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        const int sr = g ? sg[n] : sp[n];
-                        const __nv_bfloat16 *src = m + (int64_t)sr * ld + col;
+                        const int p = T.lo + kb * 64 + lw * 4 + n * 16 + sub;
+                        const __nv_bfloat16 *src = m + (int64_t)p * ld + col;
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const uint32_t q = sr >= 0 ? (op ? qb[x] : qa[x]) : 0u;
+                            const uint32_t q = p < T.hi ? (op ? qb[x] : qa[x]) : 0u;
                             if (op == 0 || x < nb)
                                 copy16(dst + (op ? kABytes : 0u) + (uint32_t)x * kBox + (uint32_t)n * 2048u,
                                        q ? src + 64 * x : m, q);
@@ -812,7 +770,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 }
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->rows[stage]))
                              : "memory");
-                if (++stage == P.stages) { stage = 0; pe ^= 1u; }
+                if (++stage == P.stages) stage = 0;
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -831,7 +789,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         Tile T;
         for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
             for (int k = T.kb0 * kPlanes; k < T.kb1 * kPlanes; ++k) {
-                if (!GRAD || P.gather || T.hi - T.lo - k / kPlanes * 64 < 64) {
+                if (!GRAD || T.hi - T.lo - k / kPlanes * 64 < 64) {
                     if (!tc_wait_warp(smem_u32(&ctl->rows[stage]), (pr >> stage) & 1u, abort_flag)) { ok = false; break; }
                     pr ^= 1u << stage;
                     if (lane == 0) {
@@ -1127,10 +1085,7 @@ int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     P.b_pair = b_pair;
     P.pa = (int)ar;
     P.pb = (int)br;
-    P.glimit = g.T;
     P.rowptr = g.rowptr;
-    P.rows = g.rows;
-    P.gather = g.rows ? (row ? 2 : 1) : 0;
     P.ga = (const __nv_bfloat16 *)ap;
     P.lda = lda;
     P.gb = (const __nv_bfloat16 *)bp;

@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(kThreads) route_count(const int32_t *__restric
                                                         int base, int E,
                                                         int32_t *__restrict__ hist) {
     extern __shared__ int32_t cnt[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (int e = threadIdx.x; e < E; e += kThreads) cnt[e] = 0;
     __syncthreads();
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
@@ -62,15 +63,23 @@ route_place(const int32_t *__restrict__ ids, int64_t n, int k, int base, int E,
     uint16_t *wh = reinterpret_cast<uint16_t *>(mine + E);   // kWarps x E: the warps' counts
     __shared__ int32_t wsum[kWarps];
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    for (int i = threadIdx.x; i < kWarps * E; i += kThreads) wh[i] = 0;
+    for (int i = threadIdx.x; i < kWarps * E / 2; i += kThreads) reinterpret_cast<uint32_t *>(wh)[i] = 0;
     __syncthreads();
-    // ranks inside the warp, in entry order
+    // ranks inside the warp, in entry order (a dropped entry is expert -1: all
+    // bits set, which no expert below 2^bits - 1 has)
+    const int bits = 32 - __clz(E);
     int ex[kPer], rank[kPer];
     uint16_t *my = wh + warp * E;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
         ex[r] = expert_of(ids, entry_index(warp, r, lane), n, base, E);
-        const unsigned same = __match_any_sync(0xffffffffu, ex[r]);
+        // lanes of the same expert, a ballot a bit (match.any takes a step for
+        // each distinct value, up to 32 here)
+        unsigned same = 0xffffffffu;
+        for (int b = 0; b < bits; ++b) {
+            const unsigned set = __ballot_sync(0xffffffffu, ex[r] >> b & 1);
+            same &= ex[r] >> b & 1 ? set : ~set;
+        }
         const int before = __popc(same & ((1u << lane) - 1u));
         int have = 0;
         if (ex[r] >= 0) have = my[ex[r]];
@@ -80,27 +89,50 @@ route_place(const int32_t *__restrict__ ids, int64_t n, int k, int base, int E,
         rank[r] = have + before;
     }
     __syncthreads();
-    // counts over the warps become each warp's offset inside the chunk
-    for (int e = threadIdx.x; e < E; e += kThreads) {
-        int run = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            const int c = wh[w * E + e];
-            wh[w * E + e] = (uint16_t)run;
-            run += c;
+    // counts over the warps become each warp's offset inside the chunk; with
+    // several chunks, kThreads / E threads an expert add up the chunks' counts
+    // (four neighbouring threads an expert, eight warps each)
+    for (int i = threadIdx.x; i < 4 * E; i += kThreads) {
+        const int e = i / 4, w0 = (i & 3) * (kWarps / 4);
+        int c[kWarps / 4], sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps / 4; ++w) sum += c[w] = wh[(w0 + w) * E + e];
+        const unsigned peers = 0xfu << (lane & ~3);
+        int run = 0, all = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int s = __shfl_sync(peers, sum, (lane & ~3) + q);
+            if (q < (i & 3)) run += s;
+            all += s;
         }
-        int all = run, before = 0;
-        if (hist) {
-            all = 0;
-            for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+        for (int w = 0; w < kWarps / 4; ++w) {
+            wh[(w0 + w) * E + e] = (uint16_t)run;
+            run += c[w];
+        }
+        if ((i & 3) == 0) {
+            tot[e] = hist ? 0 : all;
+            mine[e] = 0;
+        }
+    }
+    __syncthreads();
+    if (hist) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // the chunks' counts are complete
+        const int per = E < kThreads ? kThreads / E : 1;
+        for (int i = threadIdx.x; i < per * E; i += kThreads) {
+            const int e = i % E, p = i / E;
+            int all = 0, before = 0;
+#pragma unroll 8
+            for (int c = p; c < chunks; c += per) {
                 const int h = __ldg(hist + (int64_t)c * E + e);
                 if (c < (int)blockIdx.x) before += h;
                 all += h;
             }
+            atomicAdd(&tot[e], all);              // integers: the same in any order
+            atomicAdd(&mine[e], before);
         }
-        tot[e] = all;
-        mine[e] = before;
+        __syncthreads();
     }
-    __syncthreads();
     // exclusive scan of tot over the experts, kThreads at a time
     int carry = 0;
     for (int e0 = 0; e0 < E; e0 += kThreads) {
@@ -150,40 +182,35 @@ route_place(const int32_t *__restrict__ ids, int64_t n, int k, int base, int E,
 }
 
 // ------------------------------------------------------------ value access
-template <typename T>
-struct Val;
-template <>
-struct Val<float> {
-    static constexpr int kVec = 4;
-    static __device__ __forceinline__ float get(const float *p) { return __ldg(p); }
-    static __device__ __forceinline__ void put(float *p, float v) { *p = v; }
-    static __device__ __forceinline__ void load(const float *p, float *v) {
-        const float4 q = __ldg(reinterpret_cast<const float4 *>(p));
-        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+// V neighbouring values (16 bytes, or one) as they lie in memory, so that
+// several rows' loads can wait in few registers.
+template <typename T, int V>
+struct Raw {
+    uint4 q;
+    T one;
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (V == 1) one = *p;
+        else q = __ldg(reinterpret_cast<const uint4 *>(p));
     }
-    static __device__ __forceinline__ void store(float *p, const float *v) {
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    }
-};
-template <>
-struct Val<__nv_bfloat16> {
-    static constexpr int kVec = 8;
-    static __device__ __forceinline__ float get(const __nv_bfloat16 *p) {
-        return __bfloat162float(*p);
-    }
-    static __device__ __forceinline__ void put(__nv_bfloat16 *p, float v) {
-        *p = __float2bfloat16_rn(v);
-    }
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float *v) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (V == 1) {
+            if constexpr (sizeof(T) == 2) return __bfloat162float(one);
+            else return one;
+        } else {
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+            if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+            else return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
         }
     }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float *v) {
+};
+template <typename T, int V>
+__device__ __forceinline__ void store_values(T *p, const float (&v)[V]) {
+    if constexpr (V == 1) {
+        if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v[0]);
+        else *p = v[0];
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -192,11 +219,14 @@ struct Val<__nv_bfloat16> {
         }
         *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-};
+}
 
 // y[t] = sum_j g[t, j] z[slot[t, j]] in the order of j, fp32 sums rounded
 // once to the value type.  V columns a thread (16 bytes, or one when the
 // layout is not aligned); blockDim = (column threads, tokens).
+constexpr int kRowsAhead = 4;
+template <int V>
+constexpr int kColsAhead = V == 1 ? 4 : 2;     // column groups a thread has under way
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 combine_rows(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__restrict__ slot,
@@ -205,27 +235,42 @@ combine_rows(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *_
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (t >= T_) return;
     const int32_t *sl = slot + t * k;
-    for (int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V; c < N;
-         c += (int64_t)gridDim.y * blockDim.x * V) {
-        float acc[V];
+    constexpr int C = kColsAhead<V>;
+    const int64_t step = (int64_t)blockDim.x * V;       // from one of a thread's column groups to the next
+    for (int64_t c = (int64_t)blockIdx.y * step * C + threadIdx.x * V; c < N; c += (int64_t)gridDim.y * step * C) {
+        float acc[C][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-        for (int j = 0; j < k; ++j) {
-            const int64_t p = (int64_t)__ldg(sl + j) - base;
-            if (p < 0) continue;                  // dropped entry
-            if (p >= S) {
-                dev_error(DEV_ERR_BOUNDS);
-                continue;
+        for (int x = 0; x < C; ++x)
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[x][i] = 0.0f;
+        for (int j0 = 0; j0 < k; j0 += kRowsAhead) {      // their loads on the way together
+            Raw<T, V> v[kRowsAhead][C];
+            float w[kRowsAhead];
+            bool use[kRowsAhead];
+#pragma unroll
+            for (int q = 0; q < kRowsAhead; ++q) {
+                const int j = j0 + q;
+                const int64_t p = j < k ? (int64_t)__ldg(sl + j) - base : -1;
+                use[q] = p >= 0 && p < S;                 // a dropped entry has no slot
+                if (p >= S) dev_error(DEV_ERR_BOUNDS);
+                if (use[q]) {
+                    w[q] = g ? __ldg(g + t * k + j) : 1.0f;
+#pragma unroll
+                    for (int x = 0; x < C; ++x)
+                        if (c + x * step < N) v[q][x].load(z + p * ldz + c + x * step);
+                }
             }
-            const float w = g ? __ldg(g + t * k + j) : 1.0f;
-            float v[V];
-            if (V == 1) v[0] = Val<T>::get(z + p * ldz + c);
-            else Val<T>::load(z + p * ldz + c, v);
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+            for (int q = 0; q < kRowsAhead; ++q)
+                if (use[q])
+#pragma unroll
+                    for (int x = 0; x < C; ++x)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) acc[x][i] = fmaf(w[q], v[q][x].get(i), acc[x][i]);
         }
-        if (V == 1) Val<T>::put(y + t * ldy + c, acc[0]);
-        else Val<T>::store(y + t * ldy + c, acc);
+#pragma unroll
+        for (int x = 0; x < C; ++x)
+            if (c + x * step < N) store_values<T, V>(y + t * ldy + c + x * step, acc[x]);
     }
 }
 
@@ -248,42 +293,50 @@ combine_bwd(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__
         end = end < 0 ? 0 : end > S ? S : end;
         for (int64_t p = end + (t - T_); p < S; p += (int64_t)gridDim.x - T_)
             for (int64_t c = (int64_t)threadIdx.x; c < N; c += kBwdThreads)
-                Val<T>::put(dz + p * lddz + c, 0.0f);
+                dz[p * lddz + c] = T(0.0f);
         return;
     }
     for (int j0 = 0; j0 < k; j0 += kBwdJ) {
-        int64_t p[kBwdJ];
+        int p[kBwdJ];                              // slots, -1: none
         float w[kBwdJ], dot[kBwdJ];
 #pragma unroll
         for (int j = 0; j < kBwdJ; ++j) {
             p[j] = -1;
             w[j] = dot[j] = 0.0f;
             if (j0 + j < k) {
-                p[j] = (int64_t)__ldg(slot + t * k + j0 + j) - base;
+                const int64_t s = (int64_t)__ldg(slot + t * k + j0 + j) - base;
                 w[j] = g ? __ldg(g + t * k + j0 + j) : 1.0f;
-                if (p[j] >= S) {
-                    dev_error(DEV_ERR_BOUNDS);
-                    p[j] = -1;
-                }
+                if (s >= S) dev_error(DEV_ERR_BOUNDS);
+                p[j] = s < 0 || s >= S ? -1 : (int)s;
             }
         }
-        for (int64_t c = (int64_t)threadIdx.x * V; c < N; c += kBwdThreads * V) {
-            float d[V];
-            if (V == 1) d[0] = Val<T>::get(dy + t * lddy + c);
-            else Val<T>::load(dy + t * lddy + c, d);
+        constexpr int C = V == 1 ? 4 : 1;                 // column groups a thread has under way
+        for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < N; c0 += kBwdThreads * V * C) {
+            Raw<T, V> d[C], v[kBwdJ][C];
 #pragma unroll
-            for (int j = 0; j < kBwdJ; ++j) {
-                if (p[j] < 0) continue;
-                float v[V], o[V];
-                if (V == 1) v[0] = Val<T>::get(z + p[j] * ldz + c);
-                else Val<T>::load(z + p[j] * ldz + c, v);
+            for (int x = 0; x < C; ++x) {
+                const int64_t c = c0 + x * kBwdThreads * V;
+                if (c >= N) continue;
+                d[x].load(dy + t * lddy + c);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    dot[j] = fmaf(d[i], v[i], dot[j]);
-                    o[i] = w[j] * d[i];
+                for (int j = 0; j < kBwdJ; ++j)
+                    if (p[j] >= 0) v[j][x].load(z + (int64_t)p[j] * ldz + c);
+            }
+#pragma unroll
+            for (int x = 0; x < C; ++x) {
+                const int64_t c = c0 + x * kBwdThreads * V;
+                if (c >= N) continue;
+#pragma unroll
+                for (int j = 0; j < kBwdJ; ++j) {
+                    if (p[j] < 0) continue;
+                    float o[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        dot[j] = fmaf(d[x].get(i), v[j][x].get(i), dot[j]);
+                        o[i] = w[j] * d[x].get(i);
+                    }
+                    store_values<T, V>(dz + (int64_t)p[j] * lddz + c, o);
                 }
-                if (V == 1) Val<T>::put(dz + p[j] * lddz + c, o[0]);
-                else Val<T>::store(dz + p[j] * lddz + c, o);
             }
         }
         if (dg) {
@@ -343,9 +396,20 @@ extern "C" JLB_API int jlb_route(void *stream, int idx_base, int64_t T, int64_t 
     if (smem > 48 * 1024)
         JLB_CUDA(cudaFuncSetAttribute(route_place, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)smem));
-    route_place<<<chunks, kThreads, smem, st>>>(ids, n, (int)(k > 0 ? k : 1), idx_base, (int)E,
-                                                hist, chunks, rowptr, source, slot);
-    JLB_LAUNCH_CHECK("route_place");
+    // starts while the counts are being made and waits for them after its own
+    // ranks; alone it is an ordinary launch
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)chunks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = hist ? 1 : 0;
+    JLB_CUDA(cudaLaunchKernelEx(&cfg, route_place, ids, n, (int)(k > 0 ? k : 1), idx_base, (int)E,
+                                (const int32_t *)hist, chunks, rowptr, source, slot));
     return ok();
 }
 
@@ -364,10 +428,9 @@ int check_combine(int dtype, int idx_base, int64_t T, int64_t k, int64_t S, int6
 template <typename T>
 int run_combine(cudaStream_t st, int64_t Tn, int64_t k, int64_t S, int64_t N, int base,
                 const int32_t *slot, const float *g, const T *z, int64_t ldz, T *y, int64_t ldy) {
-    using routing::Val;
-    constexpr int V = Val<T>::kVec;
+    constexpr int V = 16 / (int)sizeof(T);
     const bool vec = N % V == 0 && ldz % V == 0 && ldy % V == 0 && aligned16(z) && aligned16(y);
-    const int64_t items = vec ? N / V : N;
+    const int64_t items = vec ? ceil_div(N / V, routing::kColsAhead<V>) : ceil_div(N, routing::kColsAhead<1>);
     int tx = 32;
     while (tx < 256 && tx < items) tx *= 2;
     const int ty = 256 / tx;
@@ -386,8 +449,7 @@ template <typename T>
 int run_combine_bwd(cudaStream_t st, int64_t Tn, int64_t k, int64_t S, int64_t N, int base,
                     const int32_t *slot, const int32_t *live_end, const float *g, const T *z,
                     int64_t ldz, const T *dy, int64_t lddy, T *dz, int64_t lddz, float *dg) {
-    using routing::Val;
-    constexpr int V = Val<T>::kVec;
+    constexpr int V = 16 / (int)sizeof(T);
     const bool vec = N % V == 0 && ldz % V == 0 && lddy % V == 0 && lddz % V == 0 &&
                      aligned16(z) && aligned16(dy) && aligned16(dz);
     const unsigned grid = (unsigned)(Tn + 148);   // 148 CTAs for the rows of no slot
