@@ -39,15 +39,18 @@
 // 8192 x 4096 x 16384 product against 1007 us without the gather.)
 //
 // Work split: a persistent grid of CTA pairs; pair c takes tiles c, c + G, ...
-// numbered group by group from rowptr on the device (each warp role walks 32
-// groups at a time), inside a group in column blocks of 8 tiles for L2 reuse.
+// numbered group by group from rowptr on the device, inside a group in column
+// blocks of 8 tiles for L2 reuse.  One warp of a CTA finds the tiles, 32
+// groups at a time, up to four ahead, and passes them to the other roles
+// through a ring in shared memory: found by each role at its tile's start, the
+// tensor cores stood still for some 1500 cycles a tile.
 // The tiles that do not fill a last round of the G pairs (all of them, when
 // there are few) are split along the inner dimension among the pairs; their
 // fp32 parts go to the workspace and finish_tc adds them in order and applies
 // the epilogue.
 // Roles: warp 0 copies, warp 1 of the leader issues products, warps 2-9 read
-// TMEM and store, warps 10-13 (only in launches that need them) load rows and
-// warp 14 reports their stages to the leader; two TMEM accumulators, so a tile's epilogue
+// TMEM and store, warp 10 finds the tiles, warps 11-14 (only in launches that
+// need them) load rows and warp 15 reports their stages to the leader; two TMEM accumulators, so a tile's epilogue
 // overlaps the next tile's products.  Every wait is bounded: on expiry the
 // device error word is raised and all roles leave.
 #include "expert_mm.cuh"
@@ -65,8 +68,10 @@ namespace emm {
 using namespace tc;
 
 constexpr int kEpiWarps = 8;                            // two for each quarter of TMEM's lanes
-constexpr int kTcThreads = 64 + kEpiWarps * 32;         // without the loaders
-constexpr int kLoadWarp = 2 + kEpiWarps, kLoaders = 128;  // the loader warps
+constexpr int kFindWarp = 2 + kEpiWarps;                // finds the tiles
+constexpr int kTcThreads = 32 + kFindWarp * 32;         // without the loaders
+constexpr int kLoadWarp = kFindWarp + 1, kLoaders = 128;  // the loader warps
+constexpr int kTileRing = 4;                            // tiles found ahead
 constexpr int kForward = 32;                            // the warp that reports the loaders' stages
 constexpr int kPitch = 36;                              // words a pair of columns takes in the epilogue's turn
 constexpr uint32_t kTurnBytes = kEpiWarps * 16 * kPitch * 4;
@@ -100,9 +105,18 @@ struct TcArgs {
 // A pipeline stage: A's half and, in 32-row boxes, B's.
 __host__ __device__ inline uint32_t stage_size(int bn_max) { return kABytes + (uint32_t)((bn_max / 2 + 31) / 32) * 4096u; }
 
+struct Tile {
+    int e, lo, hi;      // group and its rows
+    int i0, j0, bn;     // first lane, first column (product: relative to lo), columns of the instruction
+    int kb0, kb1;       // 64-wide steps of the inner dimension
+    int part;           // where a split tile's sums go, or -1
+};
+
 struct TcCtl {
     uint64_t full[kMaxStages], empty[kMaxStages], rows[kMaxStages], go[kMaxStages];
     uint64_t tfull[2], tempty[2], done;
+    uint64_t sfull[kTileRing], sempty[kTileRing];
+    Tile ring[kTileRing];
     uint32_t tmem, fills;
     int abort;
 };
@@ -133,13 +147,6 @@ __device__ __forceinline__ void tc_drain(uint32_t bar, uint32_t parity) {
             return;
         }
 }
-
-struct Tile {
-    int e, lo, hi;      // group and its rows
-    int i0, j0, bn;     // first lane, first column (product: relative to lo), columns of the instruction
-    int kb0, kb1;       // 64-wide steps of the inner dimension
-    int part;           // where a split tile's sums go, or -1
-};
 
 // width of a group's column tiles: equal shares rounded up to 32
 __host__ __device__ __forceinline__ int col_width(int r, int bn_max) {
@@ -263,6 +270,21 @@ struct Walk {
     }
 };
 
+// A role's view of the ring of tiles its CTA's finding warp fills; a tile of
+// no columns ends it.
+struct TileReader {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ bool next(TcCtl *ctl, Tile &T, volatile int *abort_flag) {
+        if (!tc_wait_warp(smem_u32(&ctl->sfull[slot]), phase, abort_flag)) return false;
+        T = ctl->ring[slot];
+        __syncwarp();
+        if (threadIdx.x % kWarp == 0) mbar_arrive_count(smem_u32(&ctl->sempty[slot]), 1);
+        if (++slot == kTileRing) { slot = 0; phase ^= 1u; }
+        return T.bn != 0;
+    }
+};
+
 // cp.async of up to 16 bytes; the rest of the 16 is zeroed (bytes == 0: all).
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -383,7 +405,8 @@ __device__ __forceinline__ void store_tile(const TcArgs &P, uint32_t taddr, uint
 template <bool A_MN, bool GRAD, typename T_>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads + kLoaders + kForward, 1)
 product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB,
-           const __grid_constant__ CUtensorMap mBig, const __grid_constant__ TcArgs P) {
+           const __grid_constant__ CUtensorMap mBig, const __grid_constant__ CUtensorMap mMid,
+           const __grid_constant__ TcArgs P) {
     constexpr bool F32 = sizeof(T_) == 4;
     constexpr int kPlanes = F32 ? 3 : 1;
     extern __shared__ uint8_t smem_raw[];
@@ -411,6 +434,11 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             mbar_init(smem_u32(&ctl->tempty[b]), 2 * kEpiWarps);
         }
         mbar_init(smem_u32(&ctl->done), 1);
+        for (int b = 0; b < kTileRing; ++b) {
+            mbar_init(smem_u32(&ctl->sfull[b]), 1);
+            // the warps that read it: copies, epilogue, the leader's products, loaders and their report
+            mbar_init(smem_u32(&ctl->sempty[b]), 1 + kEpiWarps + (rank == 0 ? 1 : 0) + (loaders ? (kLoaders + kForward) / kWarp : 0));
+        }
         ctl->abort = 0;
         ctl->fills = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -431,10 +459,9 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         bool ok = true, bad = false;
         if (blockIdx.x == 0)
             for (int64_t e = lane; e < P.E; e += kWarp) bad |= group_bad(P.rowptr, P.base, P.S, e);
-        Walk<GRAD> walk;
-        walk.init(P);
+        TileReader tiles;
         Tile T;
-        for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
+        while (ok && tiles.next(ctl, T, abort_flag)) {
             const int a0 = T.i0 + (int)rank * 128;
             const int bh = T.bn / 2, boxes = (bh + 31) / 32;           // product: B's rows, in 32-row boxes
             const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
@@ -458,11 +485,11 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                             tma_3d(sA, &mA, full, a0, kb * 64, e);
                             tma_3d(sA + kBox, &mA, full, a0 + 64, kb * 64, e);
                         }
-                        if (boxes == 4 && !P.gather)
-                            tma_2d(sB, &mBig, full, kb * 64, r0);
-                        else if (!P.gather)
-                            for (int x = 0; x < boxes; ++x)
-                                tma_2d(sB + (uint32_t)x * 4096u, &mB, full, kb * 64, r0 + 32 * x);
+                        if (!P.gather) {                       // few copies: each costs the issuing thread
+                            if (boxes == 4) tma_2d(sB, &mBig, full, kb * 64, r0);
+                            else if (boxes >= 2) tma_2d(sB, &mMid, full, kb * 64, r0);
+                            if (boxes & 1) tma_2d(sB + (uint32_t)(boxes - 1) * 4096u, &mB, full, kb * 64, r0 + 32 * (boxes - 1));
+                        }
                     } else {
                         const bool tail = T.hi - T.lo - kb * 64 < 64;
                         const int pa = T.lo + kb * 64 + plane * P.pa, pb = T.lo + kb * 64 + plane * P.pb;
@@ -512,10 +539,9 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             bool ok = true;
             const uint64_t a_desc = operand_desc(tiles_u32, A_MN ? kBox : 16u, 1024u);
             const uint64_t b_desc = operand_desc(tiles_u32 + kABytes, GRAD ? kBox : 16u, 1024u);
-            Walk<GRAD> walk;
-            walk.init(P);
+            TileReader tiles;
             Tile T;
-            for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
+            while (ok && tiles.next(ctl, T, abort_flag)) {
                 if (T.kb0 == T.kb1) continue;                 // the epilogue writes zeros
                 const uint32_t idesc = instr_desc(256, (uint32_t)T.bn, A_MN, GRAD);
                 auto mma = [&](uint32_t a_off, uint32_t b_off, uint32_t first) {
@@ -570,7 +596,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             if (lane == 0) commit_pair(smem_u32(&ctl->done));
             __syncwarp();
         }
-    } else if (warp < kLoadWarp) {
+    } else if (warp < kFindWarp) {
         // ----------------------------------------------------------- epilogue
         const int qd = warp & 3;
         const int first = (warp - 2) / 4;                 // the 32-column chunks of this parity
@@ -588,10 +614,9 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                     if (P.z) ((T_ *)P.z)[r * P.ldz + c] = from_f32<T_>(0.0f);
                 }
         }
-        Walk<GRAD> walk;
-        walk.init(P);
+        TileReader tiles;
         Tile T;
-        for (int t = pair; walk.find(P, t, T); t += pairs) {
+        while (tiles.next(ctl, T, abort_flag)) {
             const int64_t ib = (int64_t)T.i0 + rank * 128 + qd * 32;
             // column 0's row of the output, and its columns
             const int64_t row0 = GRAD ? T.j0 : (int64_t)T.lo + T.j0;
@@ -675,6 +700,24 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             if (lane == 0) mbar_arrive_cluster(te0 + (uint32_t)buf * 8u);
             buf ^= 1;
         }
+    } else if (warp == kFindWarp) {
+        // ------------------------------------------------------------- tiles
+        Walk<GRAD> walk;
+        walk.init(P);
+        int slot = 0;
+        uint32_t ph = 1u;
+        for (int t = pair;; t += pairs) {
+            Tile T;
+            const bool have = walk.find(P, t, T);
+            if (!tc_wait_warp(smem_u32(&ctl->sempty[slot]), ph, abort_flag)) break;
+            if (lane == 0) {
+                if (!have) T.bn = 0;
+                ctl->ring[slot] = T;
+                mbar_arrive_count(smem_u32(&ctl->sfull[slot]), 1);
+            }
+            if (++slot == kTileRing) { slot = 0; ph ^= 1u; }
+            if (!have) break;
+        }
     } else if (warp < kLoadWarp + kLoaders / 32) {
         // ------------------------------------------------------ loader warps
         // Loader warp w of the CTA copies rows w*4 + 16*n + lane/8 of a stage,
@@ -687,28 +730,36 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         int stage = 0;
         uint32_t pe = 1u, pgo = 0u;
         bool ok = true, bad = false;
-        Walk<GRAD> walk;
-        walk.init(P);
+        TileReader tiles;
         Tile T;
-        for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
+        bool more = tiles.next(ctl, T, abort_flag);
+        int at[8];                                 // product: this lane's row indices of the tile to come
+        auto fetch = [&](const Tile &Q) {
+            const int b0 = Q.lo + Q.j0 + (int)rank * (Q.bn / 2);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int r = lw * 4 + n * 16 + sub;
+                at[n] = r < Q.bn / 2 && b0 + r < Q.hi ? __ldg(P.rows + b0 + r) : INT_MIN;
+            }
+        };
+        if (!GRAD && !F32 && more) fetch(T);
+        while (ok && more) {
+            Tile N;
             const int bh = T.bn / 2, nb = T.bn / 128;
             if (!GRAD && !F32) {
                 // the (at most 8) rows of B this lane copies 16 bytes of
-                const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
                 const __nv_bfloat16 *row[8];
                 uint32_t some = 0;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const int r = lw * 4 + n * 16 + sub;
                     row[n] = P.gb;
-                    if (r < bh && b0 + r < T.hi) {
-                        const int64_t s = (int64_t)__ldg(P.rows + b0 + r) - P.base;
-                        if (s >= 0 && s < P.glimit) {
-                            row[n] = P.gb + s * P.ldb_ + c8 * 8;
-                            some |= 1u << n;
-                        } else {
-                            bad = true;
-                        }
+                    if (at[n] == INT_MIN) continue;          // no row of the tile
+                    const int64_t s = (int64_t)at[n] - P.base;
+                    if (s >= 0 && s < P.glimit) {
+                        row[n] = P.gb + s * P.ldb_ + c8 * 8;
+                        some |= 1u << n;
+                    } else {
+                        bad = true;
                     }
                 }
                 const int rows = (bh - lw * 4 + 15) / 16;       // bh is a multiple of 16: all lanes alike
@@ -716,23 +767,25 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                     if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
                     const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + kABytes + at0;
                     const uint32_t bytes = bytes_at((int64_t)kb * 64 + c8 * 8, P.Kc);
-                    if (rows == 8) {
 #pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            const uint32_t q = some >> n & 1u ? bytes : 0u;
-                            copy16(dst + (uint32_t)n * 2048u, q ? row[n] + kb * 64 : P.gb, q);
-                        }
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            const uint32_t q = some >> n & 1u ? bytes : 0u;
-                            if (n < rows) copy16(dst + (uint32_t)n * 2048u, q ? row[n] + kb * 64 : P.gb, q);
-                        }
+                    for (int n = 0; n < 8; ++n) {
+                        const uint32_t q = some >> n & 1u ? bytes : 0u;
+                        if (n < rows) copy16(dst + (uint32_t)n * 2048u, q ? row[n] + kb * 64 : P.gb, q);
                     }
                     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->rows[stage]))
                                  : "memory");
                     if (++stage == P.stages) { stage = 0; pe ^= 1u; }
+                    // the next tile's row indices, while this one's copies run
+                    if (kb - T.kb0 == min(2, T.kb1 - T.kb0 - 1)) {
+                        more = tiles.next(ctl, N, abort_flag);
+                        if (more) fetch(N);
+                    }
                 }
+                if (T.kb0 == T.kb1) {
+                    more = tiles.next(ctl, N, abort_flag);
+                    if (more) fetch(N);
+                }
+                T = N;
                 continue;
             }
             // gradient: rows lw*4 + sub + 16*n (n < 4) of the group's last step,
@@ -772,6 +825,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                              : "memory");
                 if (++stage == P.stages) stage = 0;
             }
+            more = tiles.next(ctl, T, abort_flag);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (bad) dev_error(DEV_ERR_BOUNDS);
@@ -784,10 +838,9 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         int stage = 0;
         uint32_t pr = 0;                          // the phase of each stage's rows barrier, a bit each
         bool ok = true;
-        Walk<GRAD> walk;
-        walk.init(P);
+        TileReader tiles;
         Tile T;
-        for (int t = pair; ok && walk.find(P, t, T); t += pairs) {
+        while (ok && tiles.next(ctl, T, abort_flag)) {
             for (int k = T.kb0 * kPlanes; k < T.kb1 * kPlanes; ++k) {
                 if (!GRAD || T.hi - T.lo - k / kPlanes * 64 < 64) {
                     if (!tc_wait_warp(smem_u32(&ctl->rows[stage]), (pr >> stage) & 1u, abort_flag)) { ok = false; break; }
@@ -963,7 +1016,8 @@ static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, int64_t steps) {
 }
 
 template <bool A_MN, bool GRAD, typename T_>
-static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &big, TcArgs &P,
+static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &big,
+                     const CUtensorMap &mid, TcArgs &P,
                      const TcPlan &plan, void *ws, bool loaders) {
     const size_t extra = 1024 + kTurnBytes + sizeof(TcCtl);
     const uint32_t stage = stage_size(plan.bn_max);
@@ -977,7 +1031,7 @@ static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b
     if (P.stages > kMaxStages) P.stages = kMaxStages;
     const size_t smem = (size_t)P.stages * stage + extra;
     JLB_CUDA(cudaFuncSetAttribute(product_tc<A_MN, GRAD, T_>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    product_tc<A_MN, GRAD, T_><<<(unsigned)(2 * P.pairs), kTcThreads + (loaders ? kLoaders + kForward : 0), smem, st>>>(a, b, big, P);
+    product_tc<A_MN, GRAD, T_><<<(unsigned)(2 * P.pairs), kTcThreads + (loaders ? kLoaders + kForward : 0), smem, st>>>(a, b, big, mid, P);
     JLB_LAUNCH_CHECK("product_tc");
     if (plan.finish) {
         cudaLaunchConfig_t cfg{};
@@ -1018,7 +1072,7 @@ size_t tc_gradient_workspace(const Gradient &G) { return plan_gradient(G).part_b
 // and [3][E] matrices, bias, res, z and y are F32.
 int tc_product(cudaStream_t st, const Product &p, void *ws) {
     const int planes = p.dtype == JLB_F32 ? 3 : 1;
-    CUtensorMap a, b, big;
+    CUtensorMap a, b, big, mid;
     const bool mn = p.w_order == JLB_ROW_MAJOR;
     const int64_t experts = p.E * planes, w_stride = experts > 1 ? p.w_stride : (mn ? p.K : p.N) * p.ldw;
     const bool pair = mn && make_pair_map(&a, p.w, p.N, p.K, p.ldw, experts, w_stride);
@@ -1026,6 +1080,7 @@ int tc_product(cudaStream_t st, const Product &p, void *ws) {
                       : make_map(&a, p.w, p.K, p.N, p.ldw, experts, w_stride, 128)))
         return -1;
     if (!make_map(&b, p.x, p.K, p.T * planes, p.ldx, 0, 0, 32) ||
+        !make_map(&mid, p.x, p.K, p.T * planes, p.ldx, 0, 0, 64) ||
         !make_map(&big, p.x, p.K, p.T * planes, p.ldx, 0, 0, 128))
         return -1;
     TcArgs P{};
@@ -1056,10 +1111,10 @@ int tc_product(cudaStream_t st, const Product &p, void *ws) {
     const TcPlan plan = plan_product(p);
     if (plan.pairs < 1 || (p.rowptr ? p.E : 1) * ceil_div(p.N, 256) * ceil_div(p.S, 32) > INT32_MAX / 2) return -1;
     if (p.dtype == JLB_F32)
-        return mn ? launch_tc<true, false, float>(st, a, b, big, P, plan, ws, false)
-                  : launch_tc<false, false, float>(st, a, b, big, P, plan, ws, false);
-    return mn ? launch_tc<true, false, __nv_bfloat16>(st, a, b, big, P, plan, ws, p.rows)
-              : launch_tc<false, false, __nv_bfloat16>(st, a, b, big, P, plan, ws, p.rows);
+        return mn ? launch_tc<true, false, float>(st, a, b, big, mid, P, plan, ws, false)
+                  : launch_tc<false, false, float>(st, a, b, big, mid, P, plan, ws, false);
+    return mn ? launch_tc<true, false, __nv_bfloat16>(st, a, b, big, mid, P, plan, ws, p.rows)
+              : launch_tc<false, false, __nv_bfloat16>(st, a, b, big, mid, P, plan, ws, p.rows);
 }
 
 int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
@@ -1069,12 +1124,13 @@ int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     const void *ap = row ? g.dz : g.x, *bp = row ? g.x : g.dz;
     const int64_t ac = row ? g.N : g.K, ar = row ? g.S : g.T, lda = row ? g.lddz : g.ldx;
     const int64_t bc = row ? g.K : g.N, br = row ? g.T : g.S, ldb = row ? g.ldx : g.lddz;
-    CUtensorMap a, b, big;
+    CUtensorMap a, b, big, mid;
     const bool a_pair = make_pair_map(&a, ap, ac, ar * planes, lda, 0, 0),
                b_pair = make_pair_map(&big, bp, bc, br * planes, ldb, 0, 0);
     if ((!a_pair && !make_map(&a, ap, ac, ar * planes, lda, 0, 0, 64)) || !make_map(&b, bp, bc, br * planes, ldb, 0, 0, 64))
         return -1;
     if (!b_pair) big = b;
+    mid = b;
     TcArgs P{};
     P.base = g.base;
     P.E = g.E;
@@ -1095,8 +1151,8 @@ int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     P.ldo = g.lddw;
     P.out_stride = g.dw_stride;
     if (P.E * ceil_div(P.I, 256) * ceil_div(P.J, 128) > INT32_MAX / 2) return -1;
-    return g.dtype == JLB_F32 ? launch_tc<true, true, float>(st, a, b, big, P, plan_gradient(g), ws, true)
-                              : launch_tc<true, true, __nv_bfloat16>(st, a, b, big, P, plan_gradient(g), ws, true);
+    return g.dtype == JLB_F32 ? launch_tc<true, true, float>(st, a, b, big, mid, P, plan_gradient(g), ws, true)
+                              : launch_tc<true, true, __nv_bfloat16>(st, a, b, big, mid, P, plan_gradient(g), ws, true);
 }
 
 }  // namespace emm
