@@ -39,8 +39,8 @@
 // 8192 x 4096 x 16384 product against 1007 us without the gather.)
 //
 // Work split: a persistent grid of CTA pairs; pair c takes tiles c, c + G, ...
-// numbered group by group from rowptr on the device, inside a group in column
-// blocks of 8 tiles for L2 reuse.  One warp of a CTA finds the tiles, 32
+// numbered group by group from rowptr on the device, inside a group in blocks
+// of the column tiles whose B stays in L2 while A streams past.  One warp of a CTA finds the tiles, 32
 // groups at a time, up to four ahead, and passes them to the other roles
 // through a ring in shared memory: found by each role at its tile's start, the
 // tensor cores stood still for some 1500 cycles a tile.
@@ -78,7 +78,7 @@ constexpr uint32_t kTurnBytes = kEpiWarps * 16 * kPitch * 4;
 constexpr int kMaxStages = 10;
 constexpr uint32_t kABytes = 128 * 128;                 // 128 lanes x 64 inner, a CTA's half of A
 constexpr uint32_t kBox = 64 * 128;                     // 64 x 64 bf16
-constexpr int kJBlock = 8;                              // column tiles that share A's tiles in L2
+constexpr int64_t kL2Block = 24 << 20;                  // bytes of B that a block of column tiles keeps in L2
 constexpr long long kTcTimeout = 4000000000ll;          // ~2 s
 
 struct TcArgs {
@@ -95,7 +95,7 @@ struct TcArgs {
     int64_t ldb, ldr;
     void *z, *out;
     int64_t ldz, ldo, out_stride;
-    int stages, bn_max;
+    int stages, bn_max, jblock;
     int a_pair, b_pair;           // mA / mBig: both 64-wide boxes of an operand in one copy
     int pairs, max_splits;        // CTA pairs launched; parts a tile may be split into (> 1: rowptr decides)
     int full, splits;             // tiles not split and the parts of the others, when the host knows
@@ -252,15 +252,15 @@ struct Walk {
         T.lo = __shfl_sync(0xffffffffu, lo, src);
         T.hi = __shfl_sync(0xffffffffu, hi, src);
         const int l = want - __shfl_sync(0xffffffffu, first, src);
-        // column tiles j, in blocks of kJBlock, lane tiles i inside a block
+        // column tiles j, in blocks of jblock, lane tiles i inside a block
         const int cw = GRAD ? P.bn_max : col_width(T.hi - T.lo, P.bn_max);
         const int n = GRAD ? jt : (int)((unsigned)(T.hi - T.lo + cw - 1) / (unsigned)cw);
         int i = l, j = 0;
         if (n > 1) {
-            const int jb = n <= kJBlock ? 0 : (int)((unsigned)l / (unsigned)(kJBlock * it));
-            const int rem = l - jb * kJBlock * it, w = min(kJBlock, n - kJBlock * jb);
+            const int jb = n <= P.jblock ? 0 : (int)((unsigned)l / (unsigned)(P.jblock * it));
+            const int rem = l - jb * P.jblock * it, w = min(P.jblock, n - P.jblock * jb);
             i = (int)((unsigned)rem / (unsigned)w);
-            j = kJBlock * jb + rem - i * w;
+            j = P.jblock * jb + rem - i * w;
         }
         T.i0 = i * 256;
         T.j0 = j * cw;
@@ -1022,6 +1022,8 @@ static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b
     const size_t extra = 1024 + kTurnBytes + sizeof(TcCtl);
     const uint32_t stage = stage_size(plan.bn_max);
     P.bn_max = plan.bn_max;
+    const int64_t inner = GRAD ? P.S / P.E : P.Kc, tile = (inner > 0 ? inner : 1) * plan.bn_max * 2 * (sizeof(T_) == 4 ? 3 : 1);
+    P.jblock = (int)(kL2Block / tile < 4 ? 4 : kL2Block / tile > 64 ? 64 : kL2Block / tile);
     P.pairs = plan.pairs;
     P.max_splits = plan.max_splits;
     P.full = plan.full;
