@@ -404,137 +404,152 @@ static int check_act(int act) {
 }
 
 // ------------------------------------------------- copies for the tensor path
-// Rows of bf16 copied to a leading dimension of a multiple of 8: those whose
-// leading dimension or address TMA cannot take, and the gradient's gathered
-// rows (idx; an index outside the matrix: a row of zeros; rows from *live_end
-// on are of no group and left out).  A warp moves 256 neighbouring elements of
-// a row: 16 bytes a lane where the source is aligned, else 64 bytes a load.
-__global__ void __launch_bounds__(256)
-align_rows(int64_t experts, int64_t rows, int64_t cols, const uint16_t *__restrict__ src, int64_t ld,
-           int64_t stride, const int32_t *__restrict__ idx, int base, int64_t limit,
-           const int32_t *__restrict__ live_end, int vec, uint16_t *__restrict__ dst, int64_t ldd) {
-    const int64_t pieces = (cols + 255) / 256, all = experts * rows * pieces;
-    const int lane = threadIdx.x % kWarp;
-    const int64_t end = live_end ? (int64_t)__ldg(live_end) - base : rows;
-    bool outside = false;
-    for (int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / kWarp; w < all; w += (int64_t)gridDim.x * 8) {
-        const int64_t r = w / pieces, p0 = (w - r * pieces) * 256;
-        const int64_t e = r / rows;
-        int64_t sr = r - e * rows;
-        if (sr >= end) continue;
-        if (idx) {
-            sr = (int64_t)__ldg(idx + sr) - base;
-            if (sr < 0 || sr >= limit) {
-                sr = -1;
-                outside = true;
-            }
+static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+static size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
+static bool tma_rows(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+// Rows of one operand that the tensor path reads from a copy.
+struct Copy {
+    const void *src;              // experts matrices of rows x cols
+    int64_t experts, rows, cols, ld, stride;
+    const int32_t *idx;           // source row of each row, or null; an index outside [0, limit): a row of zeros
+    int64_t limit;
+    const int32_t *live_end;      // rows from *live_end on are of no group and hold nothing
+    int base, vec;                // vec: the source's rows are 16-byte aligned
+    void *dst;
+    int64_t ldd;
+    int64_t warps;                // pieces of rows, one a warp at a time
+};
+
+// Where piece w of a copy comes from: its row r of the copy and its source
+// row, null for a row of zeros.  False: nothing to do.
+template <typename T>
+__device__ __forceinline__ bool copy_source(const Copy &c, int64_t w, int per_piece, int64_t &r, int64_t &col,
+                                            const T *&s, bool &outside) {
+    const int64_t pieces = (c.cols + per_piece - 1) / per_piece;
+    r = w / pieces;
+    col = (w - r * pieces) * per_piece;
+    const int64_t e = r / c.rows;
+    int64_t sr = r - e * c.rows;
+    if (c.live_end && sr >= (int64_t)__ldg(c.live_end) - c.base) return false;
+    s = (const T *)c.src + e * c.stride;
+    if (c.idx) {
+        sr = (int64_t)__ldg(c.idx + sr) - c.base;
+        if (sr < 0 || sr >= c.limit) {
+            outside = true;
+            s = nullptr;
+            return true;
         }
-        const uint16_t *s = src + e * stride + (sr < 0 ? 0 : sr) * ld;
-        uint16_t *d = dst + r * ldd;
-        if (vec && p0 + 256 <= cols) {
-            const uint4 z = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4 *>(d + p0 + 8 * lane) =
-                sr < 0 ? z : __ldg(reinterpret_cast<const uint4 *>(s + p0 + 8 * lane));
-            continue;
-        }
-        const int64_t c0 = p0 + lane;
-        uint16_t v[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = sr >= 0 && c0 + q * 32 < cols ? s[c0 + q * 32] : (uint16_t)0;
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-            if (c0 + q * 32 < cols) d[c0 + q * 32] = v[q];
     }
-    if (outside) dev_error(DEV_ERR_BOUNDS);
+    s += sr * c.ld;
+    return true;
+}
+
+// Rows of bf16 to a leading dimension of a multiple of 8: those whose leading
+// dimension or address TMA cannot take, and the gradient's gathered rows.  A
+// warp moves 256 neighbouring elements of a row: 16 bytes a lane where the
+// source is aligned, else 64 bytes a load.
+constexpr int kAlignPiece = 256;
+__device__ __forceinline__ void align_piece(const Copy &c, int64_t w, bool &outside) {
+    const int lane = threadIdx.x % kWarp;
+    int64_t r, p0;
+    const uint16_t *s;
+    if (!copy_source(c, w, kAlignPiece, r, p0, s, outside)) return;
+    uint16_t *d = (uint16_t *)c.dst + r * c.ldd;
+    if (c.vec && p0 + kAlignPiece <= c.cols) {
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4 *>(d + p0 + 8 * lane) = s ? __ldg(reinterpret_cast<const uint4 *>(s + p0 + 8 * lane)) : z;
+        return;
+    }
+    const int64_t c0 = p0 + lane;
+    uint16_t v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = s && c0 + q * 32 < c.cols ? s[c0 + q * 32] : (uint16_t)0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+        if (c0 + q * 32 < c.cols) d[c0 + q * 32] = v[q];
 }
 
 // F32 rows as three bf16 planes, h + m + l = the value: h holds its upper 8
 // bits, m the next 8 and l the last 8.  Truncated, not rounded, so that h
 // cannot overflow and the three have one sign (an overflow stays an infinity).
-// Rows come through `rows` when given (an index outside the matrix: zeros).
 // An infinity or NaN goes to l, whose only partner is the other operand's h
 // (never 0 for a value of 2^-133 or more, +-1 for an infinity), with h = +-1
 // for an infinity there; in h it would meet zero m and l planes.
-__global__ void __launch_bounds__(256)
-split_rows(int64_t experts, int64_t rows, int64_t cols, const float *__restrict__ src, int64_t ld, int64_t stride,
-           const int32_t *__restrict__ idx, int base, int64_t limit, const int32_t *__restrict__ live_end,
-           __nv_bfloat16 *__restrict__ dst, int64_t ldd) {
-    const int64_t pieces = (cols + 127) / 128, all = experts * rows * pieces, plane = experts * rows * ldd;
+constexpr int kSplitPiece = 128;
+__device__ __forceinline__ void split_piece(const Copy &c, int64_t w, bool &outside) {
     const int lane = threadIdx.x % kWarp;
-    const int64_t end = live_end ? (int64_t)__ldg(live_end) - base : rows;
+    int64_t r, p0;
+    const float *s;
+    if (!copy_source(c, w, kSplitPiece, r, p0, s, outside)) return;
+    __nv_bfloat16 *dst = (__nv_bfloat16 *)c.dst + r * c.ldd;
+    const int64_t plane = c.experts * c.rows * c.ldd, c0 = p0 + 2 * lane;
+    float v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int64_t k = c0 + (q / 2) * 64 + q % 2;
+        v[q] = s && k < c.cols ? s[k] : 0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q += 2) {
+        const int64_t k = c0 + (q / 2) * 64;
+        if (k >= c.cols) continue;
+        float h[2], m[2], l[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t u = __float_as_uint(v[q + x]);
+            h[x] = __uint_as_float(u & 0xffff0000u);
+            const float rest = v[q + x] - h[x];
+            m[x] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+            l[x] = rest - m[x];
+            if ((u & 0x7f800000u) == 0x7f800000u) {
+                h[x] = copysignf(1.0f, v[q + x]);
+                m[x] = 0.0f;
+                l[x] = v[q + x];
+            }
+        }
+        *reinterpret_cast<__nv_bfloat162 *>(dst + k) = __floats2bfloat162_rn(h[0], h[1]);
+        *reinterpret_cast<__nv_bfloat162 *>(dst + plane + k) = __floats2bfloat162_rn(m[0], m[1]);
+        *reinterpret_cast<__nv_bfloat162 *>(dst + 2 * plane + k) = __floats2bfloat162_rn(l[0], l[1]);
+    }
+}
+
+// One or two operands' copies in one launch, their pieces in turn.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) copy_rows(const Copy a, const Copy b) {
     bool outside = false;
+    const int64_t all = a.warps + b.warps;
     for (int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x / kWarp; w < all; w += (int64_t)gridDim.x * 8) {
-        const int64_t r = w / pieces, c0 = (w - r * pieces) * 128 + 2 * lane;
-        const int64_t e = r / rows;
-        int64_t sr = r - e * rows;
-        const bool live = sr < end;               // rows of no group hold anything
-        if (idx && live) {
-            sr = (int64_t)__ldg(idx + sr) - base;
-            if (sr < 0 || sr >= limit) {
-                sr = -1;
-                outside = true;
-            }
-        }
-        const float *s = live && sr >= 0 ? src + e * stride + sr * ld : nullptr;
-        float v[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int64_t c = c0 + (q / 2) * 64 + q % 2;
-            v[q] = s && c < cols ? s[c] : 0.0f;
-        }
-#pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-            const int64_t c = c0 + (q / 2) * 64;
-            if (c >= cols) continue;
-            __nv_bfloat162 o[3];
-            float h[2], m[2], l[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const uint32_t u = __float_as_uint(v[q + x]);
-                h[x] = __uint_as_float(u & 0xffff0000u);
-                const float rest = v[q + x] - h[x];
-                m[x] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-                l[x] = rest - m[x];
-                if ((u & 0x7f800000u) == 0x7f800000u) {
-                    h[x] = copysignf(1.0f, v[q + x]);
-                    m[x] = 0.0f;
-                    l[x] = v[q + x];
-                }
-            }
-            o[0] = __floats2bfloat162_rn(h[0], h[1]);
-            o[1] = __floats2bfloat162_rn(m[0], m[1]);
-            o[2] = __floats2bfloat162_rn(l[0], l[1]);
-#pragma unroll
-            for (int x = 0; x < 3; ++x) *reinterpret_cast<__nv_bfloat162 *>(dst + x * plane + r * ldd + c) = o[x];
-        }
+        const bool first = w < a.warps;
+        if (SPLIT) split_piece(first ? a : b, first ? w : w - a.warps, outside);
+        else align_piece(first ? a : b, first ? w : w - a.warps, outside);
     }
     if (outside) dev_error(DEV_ERR_BOUNDS);
 }
 
-static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
-static size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
-static bool tma_rows(const void *p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
-
-static int align_copy(cudaStream_t st, int64_t experts, int64_t rows, int64_t cols, const void *src, int64_t ld,
-                      int64_t stride, const int32_t *idx, int base, int64_t limit, const int32_t *live_end,
-                      void *dst) {
-    const int64_t warps = experts * rows * ceil_div(cols, 256), blocks = ceil_div(warps, 8);
-    const int vec = tma_rows(src, ld) && (experts == 1 || stride % 8 == 0);
-    align_rows<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(
-        experts, rows, cols, (const uint16_t *)src, ld, stride, idx, base, limit, live_end, vec, (uint16_t *)dst,
-        pad8(cols));
-    JLB_LAUNCH_CHECK("align_rows");
-    return JLB_OK;
+static Copy make_copy(bool split, const void *src, int64_t experts, int64_t rows, int64_t cols, int64_t ld,
+                      int64_t stride, void *dst) {
+    Copy c{};
+    c.src = src;
+    c.experts = experts;
+    c.rows = rows;
+    c.cols = cols;
+    c.ld = ld;
+    c.stride = stride;
+    c.vec = tma_rows(src, ld) && (experts == 1 || stride % 8 == 0);
+    c.dst = dst;
+    c.ldd = pad8(cols);
+    c.warps = experts * rows * ceil_div(cols, split ? kSplitPiece : kAlignPiece);
+    return c;
 }
 
-static int split_copy(cudaStream_t st, int64_t experts, int64_t rows, int64_t cols, const void *src, int64_t ld,
-                      int64_t stride, const int32_t *idx, int base, int64_t limit, const int32_t *live_end,
-                      void *dst) {
-    const int64_t warps = experts * rows * ceil_div(cols, 128), blocks = ceil_div(warps, 8);
-    split_rows<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(
-        experts, rows, cols, (const float *)src, ld, stride, idx, base, limit, live_end, (__nv_bfloat16 *)dst,
-        pad8(cols));
-    JLB_LAUNCH_CHECK("split_rows");
+static int launch_copies(cudaStream_t st, bool split, const Copy &a, const Copy &b) {
+    const int64_t blocks = ceil_div(a.warps + b.warps, 8);
+    if (blocks == 0) return JLB_OK;
+    const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+    if (split) copy_rows<true><<<grid, 256, 0, st>>>(a, b);
+    else copy_rows<false><<<grid, 256, 0, st>>>(a, b);
+    JLB_LAUNCH_CHECK("copy_rows");
     return JLB_OK;
 }
 
@@ -580,21 +595,21 @@ static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_by
             return fail(JLB_ERR_WORKSPACE, "the product needs %zu workspace bytes", q.bytes);
         const bool row = P.w_order == JLB_ROW_MAJOR;
         char *base = (char *)ws;
-        int r = JLB_OK;
-        if (q.split) {
-            r = split_copy(st, 1, P.S, P.K, P.x, P.ldx, 0, P.rows, P.base, P.T, P.rowptr ? P.rowptr + P.E : nullptr,
-                           base + q.x_at);
-            if (!r)
-                r = split_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride, nullptr, 0, 0, nullptr,
-                               base + q.w_at);
-            q.p.rows = nullptr;
-            q.p.T = P.S;
-        } else {
-            if (q.copy_x) r = align_copy(st, 1, P.T, P.K, P.x, P.ldx, 0, nullptr, 0, 0, nullptr, base + q.x_at);
-            if (!r && q.copy_w)
-                r = align_copy(st, P.E, row ? P.K : P.N, row ? P.N : P.K, P.w, P.ldw, P.w_stride, nullptr, 0, 0, nullptr,
-                               base + q.w_at);
+        Copy x{}, w{};
+        if (q.copy_x) {
+            x = make_copy(q.split, P.x, 1, q.split ? P.S : P.T, P.K, P.ldx, 0, base + q.x_at);
+            if (q.split) {                        // planes of the rows already gathered
+                x.idx = P.rows;
+                x.limit = P.T;
+                x.base = P.base;
+                x.live_end = P.rowptr ? P.rowptr + P.E : nullptr;
+                q.p.rows = nullptr;
+                q.p.T = P.S;
+            }
         }
+        if (q.copy_w)
+            w = make_copy(q.split, P.w, P.E, row ? P.K : P.N, row ? P.N : P.K, P.ldw, P.w_stride, base + q.w_at);
+        int r = launch_copies(st, q.split, x, w);
         if (r) return r;
         if (q.copy_x) q.p.x = base + q.x_at;
         if (q.copy_w) q.p.w = base + q.w_at;
@@ -647,19 +662,18 @@ static int run_gradient(cudaStream_t st, const Gradient &G, void *ws, size_t ws_
         if (q.bytes && (!ws || ws_bytes < q.bytes))
             return fail(JLB_ERR_WORKSPACE, "the gradient needs %zu workspace bytes", q.bytes);
         char *base = (char *)ws;
-        const int32_t *end = G.rowptr ? G.rowptr + G.E : nullptr;
-        int r = JLB_OK;
-        if (q.split) {
-            r = split_copy(st, 1, G.S, G.K, G.x, G.ldx, 0, G.rows, G.base, G.T, end, base + q.x_at);
-            if (!r) r = split_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, nullptr, G.base, 0, end, base + q.d_at);
-        } else {
-            if (q.copy_x) r = align_copy(st, 1, G.S, G.K, G.x, G.ldx, 0, G.rows, G.base, G.T, end, base + q.x_at);
-            if (!r && q.copy_d) r = align_copy(st, 1, G.S, G.N, G.dz, G.lddz, 0, nullptr, 0, 0, nullptr, base + q.d_at);
-        }
+        Copy x{}, d{};
         if (q.copy_x) {
+            x = make_copy(q.split, G.x, 1, G.S, G.K, G.ldx, 0, base + q.x_at);
+            x.idx = G.rows;
+            x.limit = G.T;
             q.g.rows = nullptr;
             q.g.T = G.S;
         }
+        if (q.copy_d) d = make_copy(q.split, G.dz, 1, G.S, G.N, G.lddz, 0, base + q.d_at);
+        x.base = d.base = G.base;
+        x.live_end = d.live_end = G.rowptr ? G.rowptr + G.E : nullptr;
+        int r = launch_copies(st, q.split, x, d);
         if (r) return r;
         if (q.copy_x) q.g.x = base + q.x_at;
         if (q.copy_d) q.g.dz = base + q.d_at;

@@ -457,3 +457,92 @@ def test_layer_of_experts_end_to_end():
     for got, want in ((y, out), (dx, xt.grad), (dw1, w1t.grad), (dw2, w2t.grad), (dg, gt.grad)):
         want = want.detach().numpy()
         assert np.abs(R.f64(got) - want).max() <= 512 * R.SUM_ULP * max(1.0, np.abs(want).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_zero_extents(dtype):
+    w, b = weights(3, 8, 16, dtype, "row", 1), randn((3, 16), dtype, 2)
+    none = torch.empty(0, 8, dtype=dtype, device=DEV)
+    assert J.grouped_matmul(none, w, dev_i32([0, 0, 0, 0]), bias=b).shape == (0, 16)
+    dx, dw, db = J.grouped_matmul_backward(torch.empty(0, 16, dtype=dtype, device=DEV), none, w,
+                                           dev_i32([0, 0, 0, 0]), bias=True)
+    assert dx.shape == (0, 8) and not dw.any() and not db.any()
+    # no inner dimension: the bias alone; no columns: nothing
+    x0, w0 = torch.empty(5, 0, dtype=dtype, device=DEV), torch.empty(3, 0, 16, dtype=dtype, device=DEV)
+    y = J.grouped_matmul(x0, w0, dev_i32([0, 2, 2, 5]), bias=b, act="relu")
+    want = b.clamp_min(0)[[0, 0, 2, 2, 2]]
+    assert torch.equal(y, want)
+    assert J.fused_matmul(randn((5, 8), dtype, 1), torch.empty(8, 0, dtype=dtype, device=DEV)).shape == (5, 0)
+    # every row's index outside x
+    y = J.grouped_matmul(none, w, dev_i32([0, 1, 1, 2]), rows=dev_i32([4, -1]))
+    with pytest.raises(J.NonCanonicalStorage):
+        J.device_status()
+    assert not y.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E,S,K,N", [(40, 300, 64, 264), (1000, 700, 72, 136), (2, 3000, 512, 64)])
+def test_many_groups_and_split_tiles_match_one_group_at_a_time(dtype, E, S, K, N):
+    """More groups than a warp looks at together, and tiles split along the
+    inner dimension, against the dense product of each group."""
+    rng = np.random.default_rng(E)
+    cuts = np.sort(rng.integers(0, S + 1, size=E - 1))
+    ptr = np.concatenate([[0], cuts, [S]])
+    x, w, dy = randn((S, K), dtype, 1), weights(E, K, N, dtype, "row", 2), randn((S, N), dtype, 3)
+    y = J.grouped_matmul(x, w, dev_i32(ptr), act="silu")
+    dx, dw, db = J.grouped_matmul_backward(dy, x, w, dev_i32(ptr), bias=True)
+    J.device_status()
+    ry, _, by, _ = R.forward(R.f64(x), R.f64(w), ptr, name="silu")
+    ref, bound = R.backward(R.f64(dy), R.f64(x), R.f64(w), ptr, dtype=dtype)
+    R.check(y, ry, by, dtype, "y")
+    for got, r, b, what in zip((dx, dw, db), ref, bound, ("dx", "dw", "db")):
+        R.check(got, r, b, dtype, what)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_graph_of_a_training_step(dtype):
+    """route, the products (few tiles, so split ones too), combine and every
+    gradient captured once and replayed on new values."""
+    T, k, E, D, H = 333, 2, 4, 512, 264
+    ids = dev_i32(random_ids(T, k, E, 4))
+    x, w = randn((T, D), dtype, 1), weights(E, D, H, dtype, "row", 2)
+    g, dy = torch.softmax(randn((T, k), F32, 5), 1), randn((T, H), dtype, 6)
+
+    def step():
+        r = J.route(ids, E)
+        y, z = J.grouped_matmul(x, w, r.rowptr, rows=r.source, act="gelu", keep_preact=True)
+        out = J.combine(y, r, g)
+        do, dg = J.combine_backward(dy, y, r, g)
+        dxs, dw, db = J.grouped_matmul_backward(do, x, w, r.rowptr, rows=r.source, z=z, act="gelu",
+                                                bias=True)
+        return out, dg, J.combine(dxs, r), dw, db
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    ids.copy_(dev_i32(random_ids(T, k, E, 9, 0.2)))
+    x.copy_(randn((T, D), dtype, 11))
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(kept, step()):
+        assert torch.equal(a, b)
+    J.device_status()
+
+
+@pytest.mark.parametrize("M,K,N", [(20, 256, 64), (200, 512, 264), (4, 128, 96)])
+def test_f32_infinities_and_large_values_keep_their_places(M, K, N):
+    """F32 runs as planes of bf16: an infinity, a NaN or a value near the
+    type's largest gives what the products and sums of fp32 give."""
+    x, w = randn((M, K), F32, 1), randn((K, N), F32, 2, K ** -0.5)
+    inf = float("inf")
+    x[0, 3], x[1, 4], x[1, 5], x[2, 6] = inf, inf, -inf, float("nan")
+    w[3, 1], w[3, 2], w[7, 3], w[8, 4] = 0.0, -inf, inf, float("nan")
+    x[3, 9], w[9, :] = 3.4028e38, 1e-3
+    y, want = J.fused_matmul(x, w).cpu(), (x.cpu().double() @ w.cpu().double())
+    assert torch.equal(y.isnan(), want.isnan())
+    assert torch.equal(y.isinf(), want.isinf()) and torch.equal(y[y.isinf()].sign(), want[want.isinf()].sign())
+    ok = want.isfinite()
+    scale = (x.cpu().double().abs().nan_to_num(0, 0, 0) @ w.cpu().double().abs().nan_to_num(0, 0, 0))
+    assert ((y - want).abs()[ok] <= (K + 8) * R.SUM_ULP * scale[ok] + 1e-37).all()
