@@ -427,9 +427,9 @@ template <typename T>
 __device__ __forceinline__ bool copy_source(const Copy &c, int64_t w, int per_piece, int64_t &r, int64_t &col,
                                             const T *&s, bool &outside) {
     const int64_t pieces = (c.cols + per_piece - 1) / per_piece;
-    r = w / pieces;
+    r = pieces == 1 ? w : w / pieces;
     col = (w - r * pieces) * per_piece;
-    const int64_t e = r / c.rows;
+    const int64_t e = c.experts == 1 ? 0 : r / c.rows;
     int64_t sr = r - e * c.rows;
     if (c.live_end && sr >= (int64_t)__ldg(c.live_end) - c.base) return false;
     s = (const T *)c.src + e * c.stride;
@@ -447,27 +447,42 @@ __device__ __forceinline__ bool copy_source(const Copy &c, int64_t w, int per_pi
 
 // Rows of bf16 to a leading dimension of a multiple of 8: those whose leading
 // dimension or address TMA cannot take, and the gradient's gathered rows.  A
-// warp moves 256 neighbouring elements of a row: 16 bytes a lane where the
-// source is aligned, else 64 bytes a load.
-constexpr int kAlignPiece = 256;
+// warp moves 1024 neighbouring elements of a row, its loads on the way
+// together: 16 bytes a lane where the source is aligned, else 64 bytes a load.
+constexpr int kAlignPiece = 1024;
 __device__ __forceinline__ void align_piece(const Copy &c, int64_t w, bool &outside) {
     const int lane = threadIdx.x % kWarp;
     int64_t r, p0;
     const uint16_t *s;
     if (!copy_source(c, w, kAlignPiece, r, p0, s, outside)) return;
     uint16_t *d = (uint16_t *)c.dst + r * c.ldd;
-    if (c.vec && p0 + kAlignPiece <= c.cols) {
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4 *>(d + p0 + 8 * lane) = s ? __ldg(reinterpret_cast<const uint4 *>(s + p0 + 8 * lane)) : z;
+    const int n = (int)(c.cols - p0 < kAlignPiece ? c.cols - p0 : kAlignPiece);
+    if (c.vec) {
+        uint4 v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int k = q * 256 + 8 * lane;
+            v[q] = make_uint4(0, 0, 0, 0);
+            if (s && k + 8 <= n) v[q] = __ldg(reinterpret_cast<const uint4 *>(s + p0 + k));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int k = q * 256 + 8 * lane;
+            if (k + 8 <= n) *reinterpret_cast<uint4 *>(d + p0 + k) = v[q];
+        }
+        const int k = (n & ~7) + lane;            // the row's last elements
+        if (lane < 8 && k < n) d[p0 + k] = s ? s[p0 + k] : (uint16_t)0;
         return;
     }
-    const int64_t c0 = p0 + lane;
-    uint16_t v[8];
+#pragma unroll 2
+    for (int q0 = 0; q0 < n; q0 += 512) {
+        uint16_t v[16];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = s && c0 + q * 32 < c.cols ? s[c0 + q * 32] : (uint16_t)0;
+        for (int q = 0; q < 16; ++q) v[q] = s && q0 + q * 32 + lane < n ? s[p0 + q0 + q * 32 + lane] : (uint16_t)0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-        if (c0 + q * 32 < c.cols) d[c0 + q * 32] = v[q];
+        for (int q = 0; q < 16; ++q)
+            if (q0 + q * 32 + lane < n) d[p0 + q0 + q * 32 + lane] = v[q];
+    }
 }
 
 // F32 rows as three bf16 planes, h + m + l = the value: h holds its upper 8
@@ -476,41 +491,56 @@ __device__ __forceinline__ void align_piece(const Copy &c, int64_t w, bool &outs
 // An infinity or NaN goes to l, whose only partner is the other operand's h
 // (never 0 for a value of 2^-133 or more, +-1 for an infinity), with h = +-1
 // for an infinity there; in h it would meet zero m and l planes.
-constexpr int kSplitPiece = 128;
+constexpr int kSplitPiece = 512;
 __device__ __forceinline__ void split_piece(const Copy &c, int64_t w, bool &outside) {
     const int lane = threadIdx.x % kWarp;
     int64_t r, p0;
     const float *s;
     if (!copy_source(c, w, kSplitPiece, r, p0, s, outside)) return;
-    __nv_bfloat16 *dst = (__nv_bfloat16 *)c.dst + r * c.ldd;
-    const int64_t plane = c.experts * c.rows * c.ldd, c0 = p0 + 2 * lane;
-    float v[4];
+    __nv_bfloat16 *dst = (__nv_bfloat16 *)c.dst + r * c.ldd + p0;
+    const int64_t plane = c.experts * c.rows * c.ldd;
+    const int n = (int)(c.cols - p0 < kSplitPiece ? c.cols - p0 : kSplitPiece);
+    float v[2][8];                                // a lane's 8 neighbours, twice
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int64_t k = c0 + (q / 2) * 64 + q % 2;
-        v[q] = s && k < c.cols ? s[k] : 0.0f;
+    for (int q = 0; q < 2; ++q) {
+        const int k = q * 256 + 8 * lane;
+        if (c.vec && s && k + 8 <= n) {
+            *reinterpret_cast<float4 *>(v[q]) = __ldg(reinterpret_cast<const float4 *>(s + p0 + k));
+            *reinterpret_cast<float4 *>(v[q] + 4) = __ldg(reinterpret_cast<const float4 *>(s + p0 + k + 4));
+        } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[q][x] = s && k + x < n ? s[p0 + k + x] : 0.0f;
+        }
     }
 #pragma unroll
-    for (int q = 0; q < 4; q += 2) {
-        const int64_t k = c0 + (q / 2) * 64;
-        if (k >= c.cols) continue;
-        float h[2], m[2], l[2];
+    for (int q = 0; q < 2; ++q) {
+        const int k = q * 256 + 8 * lane;
+        if (k >= n) continue;
+        __nv_bfloat162 o[3][4];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t u = __float_as_uint(v[q + x]);
-            h[x] = __uint_as_float(u & 0xffff0000u);
-            const float rest = v[q + x] - h[x];
-            m[x] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-            l[x] = rest - m[x];
-            if ((u & 0x7f800000u) == 0x7f800000u) {
-                h[x] = copysignf(1.0f, v[q + x]);
-                m[x] = 0.0f;
-                l[x] = v[q + x];
+        for (int x = 0; x < 8; x += 2) {
+            float h[2], m[2], l[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const float t = v[q][x + y];
+                const uint32_t u = __float_as_uint(t);
+                h[y] = __uint_as_float(u & 0xffff0000u);
+                const float rest = t - h[y];
+                m[y] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+                l[y] = rest - m[y];
+                if ((u & 0x7f800000u) == 0x7f800000u) {
+                    h[y] = copysignf(1.0f, t);
+                    m[y] = 0.0f;
+                    l[y] = t;
+                }
             }
+            o[0][x / 2] = __floats2bfloat162_rn(h[0], h[1]);
+            o[1][x / 2] = __floats2bfloat162_rn(m[0], m[1]);
+            o[2][x / 2] = __floats2bfloat162_rn(l[0], l[1]);
         }
-        *reinterpret_cast<__nv_bfloat162 *>(dst + k) = __floats2bfloat162_rn(h[0], h[1]);
-        *reinterpret_cast<__nv_bfloat162 *>(dst + plane + k) = __floats2bfloat162_rn(m[0], m[1]);
-        *reinterpret_cast<__nv_bfloat162 *>(dst + 2 * plane + k) = __floats2bfloat162_rn(l[0], l[1]);
+        // whole groups of 8: the copy's rows are padded to them
+#pragma unroll
+        for (int x = 0; x < 3; ++x) *reinterpret_cast<uint4 *>(dst + x * plane + k) = *reinterpret_cast<const uint4 *>(o[x]);
     }
 }
 

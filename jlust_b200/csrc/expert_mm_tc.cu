@@ -30,13 +30,16 @@
 // through shared memory as pairs of columns, so that a thread then holds 8
 // neighbouring i of two rows and stores 16-byte vectors.
 //
-// Gathered rows and ragged sums.  A product's rows fetched through `rows`, and
-// the gradient's last 64-row step of a group, which must not see the next
-// group's rows (they may hold NaN), are copied by four loader warps: 16-byte
-// cp.async into the swizzled places a TMA box would fill, absent rows
-// zero-filled.
+// Gathered rows.  A product's rows fetched through `rows` are copied by four
+// loader warps: 16-byte cp.async into the swizzled places a TMA box would fill,
+// absent rows zero-filled.
 // (TMA row gathers, four rows a copy, ran at 88 cycles a copy: 2549 us for the
 // 8192 x 4096 x 16384 product against 1007 us without the gather.)
+//
+// Ragged sums.  The gradient's last 64-row step of a group must not see the
+// next group's rows (they may hold NaN): the same warps wait for the step's
+// boxes, on a barrier of their own, and write zeros over its foreign rows
+// before the step is reported.
 //
 // Work split: a persistent grid of CTA pairs; pair c takes tiles c, c + G, ...
 // numbered group by group from rowptr on the device, inside a group in blocks
@@ -88,9 +91,9 @@ struct TcArgs {
     const int32_t *rowptr, *rows;
     int gather;                   // product: B's rows come through rows
     int vec;                      // out, z and res allow 16-byte vectors
-    const __nv_bfloat16 *ga, *gb; // the operands' matrices, for the loader warps
+    const __nv_bfloat16 *gb;      // the rows' matrix, for the loader warps
     int pa, pb;                   // F32: coordinate from an operand's plane to the next (A of a product: experts)
-    int64_t lda, ldb_;
+    int64_t ldb_;
     const void *bias, *res;       // of the value type
     int64_t ldb, ldr;
     void *z, *out;
@@ -118,6 +121,7 @@ struct TcCtl {
     uint64_t sfull[kTileRing], sempty[kTileRing];
     Tile ring[kTileRing];
     uint32_t tmem, fills;
+    uint32_t tails, tail_phase;                   // stages a last step used, and their go barriers' phases, a bit each
     int abort;
 };
 
@@ -290,6 +294,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t b
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ void zero16(uint32_t dst) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+}
+
 // Bytes of the 16 at element `at` of a row of `cols` elements.
 __device__ __forceinline__ uint32_t bytes_at(int64_t at, int64_t cols) {
     const int64_t left = cols - at;
@@ -441,6 +449,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         }
         ctl->abort = 0;
         ctl->fills = 0;
+        ctl->tails = ctl->tail_phase = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) alloc_pair(smem_u32(&ctl->tmem), 512);
@@ -491,26 +500,31 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                             if (boxes & 1) tma_2d(sB + (uint32_t)(boxes - 1) * 4096u, &mB, full, kb * 64, r0 + 32 * (boxes - 1));
                         }
                     } else {
+                        // a group's last step goes through the loader warps' hands
                         const bool tail = T.hi - T.lo - kb * 64 < 64;
+                        const uint32_t to = tail ? smem_u32(&ctl->go[stage]) : full;
+                        const uint32_t bytes = kABytes + (uint32_t)nb * kBox;
                         const int pa = T.lo + kb * 64 + plane * P.pa, pb = T.lo + kb * 64 + plane * P.pb;
-                        if (rank == 0)
-                            mbar_expect_tx(smem_u32(&ctl->full[stage]),
-                                           tail ? 0u : 2u * (kABytes + (uint32_t)nb * kBox));
-                        if (rank == 0 && !tail)                // no rows to load: their arrivals
+                        if (rank == 0) mbar_expect_tx(smem_u32(&ctl->full[stage]), tail ? 0u : 2u * bytes);
+                        if (rank == 0 && !tail)                // no hands: their arrivals
                             mbar_arrive_count(smem_u32(&ctl->full[stage]), 2);
-                        if (tail) {                            // the loaders' turn
-                            mbar_arrive_count(smem_u32(&ctl->go[stage]), 1);
-                        } else if (P.a_pair) {
-                            tma_3d(sA, &mA, full, 0, pa, a0 / 64);
-                        } else {
-                            tma_2d(sA, &mA, full, a0, pa);
-                            tma_2d(sA + kBox, &mA, full, a0 + 64, pa);
+                        if (tail) {
+                            mbar_expect_tx(to, bytes);
+                            ctl->tails |= 1u << stage;
+                            ctl->tail_phase ^= 1u << stage;
                         }
-                        if (!tail && nb == 2 && P.b_pair)
-                            tma_3d(sB, &mBig, full, 0, pb, bj0 / 64);
-                        else if (!tail)
+                        if (P.a_pair) {
+                            tma_3d(sA, &mA, to, 0, pa, a0 / 64);
+                        } else {
+                            tma_2d(sA, &mA, to, a0, pa);
+                            tma_2d(sA + kBox, &mA, to, a0 + 64, pa);
+                        }
+                        if (nb == 2 && P.b_pair) {
+                            tma_3d(sB, &mBig, to, 0, pb, bj0 / 64);
+                        } else {
                             for (int x = 0; x < nb; ++x)
-                                tma_2d(sB + (uint32_t)x * kBox, &mB, full, bj0 + 64 * x, pb);
+                                tma_2d(sB + (uint32_t)x * kBox, &mB, to, bj0 + 64 * x, pb);
+                        }
                     }
                 }
                 ++fills;
@@ -788,41 +802,22 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 T = N;
                 continue;
             }
-            // gradient: rows lw*4 + sub + 16*n (n < 4) of the group's last step,
-            // both operands.  The copy thread, which waits for every stage,
-            // says when: a wait for the stage's own barrier could be laps of
-            // the ring early, the steps between not being waited for here.
-            const int64_t ca = (int64_t)T.i0 + rank * 128 + c8 * 8, cb = (int64_t)T.j0 + rank * bh + c8 * 8;
-            const uint32_t qa[2] = {bytes_at(ca, P.I), bytes_at(ca + 64, P.I)};
-            const uint32_t qb[2] = {bytes_at(cb, P.J), nb == 2 ? bytes_at(cb + 64, P.J) : 0u};
+            // gradient: zeros over the rows of a group's last step that are not
+            // its own; this lane has rows lw*4 + sub + 16*n of every box
             for (int k = T.kb0 * kPlanes; k < T.kb1 * kPlanes; ++k) {
-                const int kb = k / kPlanes, plane = k - kb * kPlanes;
-                if (T.hi - T.lo - kb * 64 >= 64) {
-                    if (++stage == P.stages) stage = 0;
-                    continue;
+                const int left = T.hi - T.lo - k / kPlanes * 64;
+                if (left < 64) {
+                    if (!tc_wait_warp(smem_u32(&ctl->go[stage]), pgo >> stage & 1u, abort_flag)) { ok = false; break; }
+                    pgo ^= 1u << stage;           // a bit a stage: its next use comes after its release
+                    const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + at0;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        if (lw * 4 + sub + 16 * n >= left)
+                            for (int x = 0; x < 2 + nb; ++x)
+                                zero16(dst + (uint32_t)x * kBox + (uint32_t)n * 2048u);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive_count(smem_u32(&ctl->rows[stage]), 1);
                 }
-                if (!tc_wait_warp(smem_u32(&ctl->go[stage]), pgo >> stage & 1u, abort_flag)) { ok = false; break; }
-                pgo ^= 1u << stage;               // a bit a stage: its next go comes after its release
-                const uint32_t dst = tiles_u32 + (uint32_t)stage * stage_bytes + at0;
-#pragma unroll
-                for (int op = 0; op < 2; ++op) {
-                    const int64_t ld = op ? P.ldb_ : P.lda, col = op ? cb : ca;
-                    const __nv_bfloat16 *m = (op ? P.gb : P.ga) + (int64_t)plane * (op ? P.pb : P.pa) * ld;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int p = T.lo + kb * 64 + lw * 4 + n * 16 + sub;
-                        const __nv_bfloat16 *src = m + (int64_t)p * ld + col;
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t q = p < T.hi ? (op ? qb[x] : qa[x]) : 0u;
-                            if (op == 0 || x < nb)
-                                copy16(dst + (op ? kABytes : 0u) + (uint32_t)x * kBox + (uint32_t)n * 2048u,
-                                       q ? src + 64 * x : m, q);
-                        }
-                    }
-                }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->rows[stage]))
-                             : "memory");
                 if (++stage == P.stages) stage = 0;
             }
             more = tiles.next(ctl, T, abort_flag);
@@ -831,7 +826,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         if (bad) dev_error(DEV_ERR_BOUNDS);
     } else {
         // ------------------------------------------------- the loaders' report
-        // A stage whose rows have landed: the copies (generic proxy) are made
+        // A stage whose rows are in place: the copies (generic proxy) are made
         // visible to the tensor cores' reads (async proxy), then the leader's
         // barrier gets this CTA's arrival.
         const uint32_t full0 = map_rank(smem_u32(&ctl->full[0]), 0);
@@ -861,6 +856,8 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
     // TMEM go (after an abort some may still be on their way)
     if (threadIdx.x == 0) {
         tc_drain(smem_u32(&ctl->done), 0);
+        for (int s = 0; s < P.stages; ++s)
+            if (ctl->tails >> s & 1u) tc_drain(smem_u32(&ctl->go[s]), (ctl->tail_phase >> s & 1u) ^ 1u);
         if (rank == 0 && ctl->abort)
             for (uint32_t s = 0; s < (uint32_t)P.stages && s < ctl->fills; ++s)
                 tc_drain(smem_u32(&ctl->full[s]), ((ctl->fills - 1 - s) / (uint32_t)P.stages) & 1u);
@@ -994,10 +991,11 @@ static int device_sms() {
 struct TcPlan {
     int bn_max, pairs, max_splits, full, splits;
     bool finish;
+    int rest;                      // split tiles, at most
     size_t part_bytes;
 };
 static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, int64_t steps) {
-    TcPlan p{bn_max, device_sms() / 2, 1, INT32_MAX, 1, false, 0};
+    TcPlan p{bn_max, device_sms() / 2, 1, INT32_MAX, 1, false, 0, 0};
     if (tiles > INT32_MAX / 2) return p;           // the launch refuses
     // at least four steps a part; and finish_tc's launch is worth it only when
     // a partly filled last round can be a sixth of the work
@@ -1006,9 +1004,11 @@ static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, int64_t steps) {
     if (exact) {
         split_schedule((int)tiles, p.pairs, (int)most, p.full, p.splits);
         p.finish = p.splits > 1;
+        p.rest = (int)tiles - p.full;
     } else if (most > 1) {
         p.max_splits = (int)most;
         p.finish = true;
+        p.rest = p.pairs / 2;                      // a split tile has two parts at least
     }
     if (p.finish) p.part_bytes = (size_t)p.pairs * 256 * bn_max * 4;
     else if (tiles < p.pairs) p.pairs = (int)tiles;
@@ -1040,7 +1040,7 @@ static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.gridDim = dim3((unsigned)ceil_div(P.bn_max, kFinish), (unsigned)(P.pairs / 2));   // a split tile has two parts at least
+        cfg.gridDim = dim3((unsigned)ceil_div(P.bn_max, kFinish), (unsigned)plan.rest);
         cfg.blockDim = dim3(256);
         cfg.stream = st;
         cfg.attrs = at;
@@ -1144,10 +1144,6 @@ int tc_gradient(cudaStream_t st, const Gradient &g, void *ws) {
     P.pa = (int)ar;
     P.pb = (int)br;
     P.rowptr = g.rowptr;
-    P.ga = (const __nv_bfloat16 *)ap;
-    P.lda = lda;
-    P.gb = (const __nv_bfloat16 *)bp;
-    P.ldb_ = ldb;
     P.vec = tma_matrix(g.dw, g.lddw) && (g.E == 1 || g.dw_stride % 8 == 0);
     P.out = g.dw;
     P.ldo = g.lddw;
