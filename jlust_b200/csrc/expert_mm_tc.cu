@@ -357,6 +357,12 @@ __device__ __forceinline__ void store32_f32(const float (&v)[32], float *out, in
         if (c < n) o[c * ld] = v[c];
 }
 
+template <int ACT>
+__device__ __forceinline__ void act32_f32(float (&v)[32]) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = act_value<float>(v[c], ACT);
+}
+
 // The epilogue of 32 columns of F32 sums.
 template <bool GRAD>
 __device__ __forceinline__ void finish32_f32(const TcArgs &P, float (&v)[32], int64_t row0, int n, int64_t i,
@@ -365,8 +371,14 @@ __device__ __forceinline__ void finish32_f32(const TcArgs &P, float (&v)[32], in
 #pragma unroll
         for (int c = 0; c < 32; ++c) v[c] += bias;
         if (P.z) store32_f32(v, (float *)P.z, P.ldz, row0, n, i, P.I);
-#pragma unroll 4
-        for (int c = 0; c < 32; ++c) v[c] = act_value<float>(v[c], P.act);
+        // unrolled: an index that the compiler does not know would put the sums
+        // in local memory for the whole kernel
+        switch (P.act) {
+            case JLB_ACT_RELU: act32_f32<JLB_ACT_RELU>(v); break;
+            case JLB_ACT_SILU: act32_f32<JLB_ACT_SILU>(v); break;
+            case JLB_ACT_GELU: act32_f32<JLB_ACT_GELU>(v); break;
+            default: break;
+        }
         if (P.res && i < P.I) {
             const float *q = (const float *)P.res + row0 * P.ldr + i;
 #pragma unroll
