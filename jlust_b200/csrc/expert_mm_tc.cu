@@ -476,7 +476,7 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         // ------------------------------------------------------------ copies
         const uint32_t full0 = map_rank(smem_u32(&ctl->full[0]), 0);
         int stage = 0;
-        uint32_t pe = 1u, fills = 0;
+        uint32_t pe = 1u, fills = 0, tails = 0, tail_phase = 0;
         bool ok = true, bad = false;
         if (blockIdx.x == 0)
             for (int64_t e = lane; e < P.E; e += kWarp) bad |= group_bad(P.rowptr, P.base, P.S, e);
@@ -487,62 +487,59 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             const int bh = T.bn / 2, boxes = (bh + 31) / 32;           // product: B's rows, in 32-row boxes
             const int64_t b0 = (int64_t)T.lo + T.j0 + rank * bh;
             const int nb = T.bn / 128, bj0 = T.j0 + (int)rank * bh;    // gradient: B's 64-column boxes
-            for (int k = T.kb0 * kPlanes; lane == 0 && k < T.kb1 * kPlanes; ++k) {
+            for (int k = T.kb0 * kPlanes; k < T.kb1 * kPlanes; ++k) {
                 const int kb = k / kPlanes, plane = k - kb * kPlanes;
-                if (!tc_wait(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
-                {
-                    const uint32_t sA = tiles_u32 + (uint32_t)stage * stage_bytes, sB = sA + kABytes;
-                    const uint32_t full = full0 + (uint32_t)stage * 8u;
-                    if (!GRAD) {
-                        const int e = T.e + plane * P.pa, r0 = (int)b0 + plane * P.pb;
-                        if (rank == 0)
-                            mbar_expect_tx(smem_u32(&ctl->full[stage]),
-                                           2u * (kABytes + (P.gather ? 0u : (uint32_t)boxes * 4096u)));
-                        if (!A_MN) {
-                            tma_3d(sA, &mA, full, kb * 64, a0, e);
-                        } else if (P.a_pair) {
-                            tma_4d(sA, &mA, full, 0, kb * 64, a0 / 64, e);
-                        } else {
-                            tma_3d(sA, &mA, full, a0, kb * 64, e);
-                            tma_3d(sA + kBox, &mA, full, a0 + 64, kb * 64, e);
-                        }
-                        if (!P.gather) {                       // few copies: each costs the issuing thread
-                            if (boxes == 4) tma_2d(sB, &mBig, full, kb * 64, r0);
-                            else if (boxes >= 2) tma_2d(sB, &mMid, full, kb * 64, r0);
-                            if (boxes & 1) tma_2d(sB + (uint32_t)(boxes - 1) * 4096u, &mB, full, kb * 64, r0 + 32 * (boxes - 1));
-                        }
+                if (!tc_wait_warp(smem_u32(&ctl->empty[stage]), pe, abort_flag)) { ok = false; break; }
+                const uint32_t sA = tiles_u32 + (uint32_t)stage * stage_bytes, sB = sA + kABytes;
+                const uint32_t full = full0 + (uint32_t)stage * 8u;
+                if (!GRAD) {
+                    const int e = T.e + plane * P.pa, r0 = (int)b0 + plane * P.pb;
+                    if (rank == 0)
+                        mbar_expect_tx(smem_u32(&ctl->full[stage]),
+                                       2u * (kABytes + (P.gather ? 0u : (uint32_t)boxes * 4096u)));
+                    if (!A_MN) {
+                        tma_3d(sA, &mA, full, kb * 64, a0, e);
+                    } else if (P.a_pair) {
+                        tma_4d(sA, &mA, full, 0, kb * 64, a0 / 64, e);
                     } else {
-                        // a group's last step goes through the loader warps' hands
-                        const bool tail = T.hi - T.lo - kb * 64 < 64;
-                        const uint32_t to = tail ? smem_u32(&ctl->go[stage]) : full;
-                        const uint32_t bytes = kABytes + (uint32_t)nb * kBox;
-                        const int pa = T.lo + kb * 64 + plane * P.pa, pb = T.lo + kb * 64 + plane * P.pb;
-                        if (rank == 0) mbar_expect_tx(smem_u32(&ctl->full[stage]), tail ? 0u : 2u * bytes);
-                        if (rank == 0 && !tail)                // no hands: their arrivals
-                            mbar_arrive_count(smem_u32(&ctl->full[stage]), 2);
-                        if (tail) {
-                            mbar_expect_tx(to, bytes);
-                            ctl->tails |= 1u << stage;
-                            ctl->tail_phase ^= 1u << stage;
-                        }
-                        if (P.a_pair) {
-                            tma_3d(sA, &mA, to, 0, pa, a0 / 64);
-                        } else {
-                            tma_2d(sA, &mA, to, a0, pa);
-                            tma_2d(sA + kBox, &mA, to, a0 + 64, pa);
-                        }
-                        if (nb == 2 && P.b_pair) {
-                            tma_3d(sB, &mBig, to, 0, pb, bj0 / 64);
-                        } else {
-                            for (int x = 0; x < nb; ++x)
-                                tma_2d(sB + (uint32_t)x * kBox, &mB, to, bj0 + 64 * x, pb);
-                        }
+                        tma_3d(sA, &mA, full, a0, kb * 64, e);
+                        tma_3d(sA + kBox, &mA, full, a0 + 64, kb * 64, e);
+                    }
+                    if (!P.gather) {                       // few copies: each costs the issuing thread
+                        if (boxes == 4) tma_2d(sB, &mBig, full, kb * 64, r0);
+                        else if (boxes >= 2) tma_2d(sB, &mMid, full, kb * 64, r0);
+                        if (boxes & 1) tma_2d(sB + (uint32_t)(boxes - 1) * 4096u, &mB, full, kb * 64, r0 + 32 * (boxes - 1));
+                    }
+                } else {
+                    // a group's last step goes through the loader warps' hands
+                    const bool tail = T.hi - T.lo - kb * 64 < 64;
+                    const uint32_t to = tail ? smem_u32(&ctl->go[stage]) : full;
+                    const uint32_t bytes = kABytes + (uint32_t)nb * kBox;
+                    const int pa = T.lo + kb * 64 + plane * P.pa, pb = T.lo + kb * 64 + plane * P.pb;
+                    if (rank == 0) mbar_expect_tx(smem_u32(&ctl->full[stage]), tail ? 0u : 2u * bytes);
+                    if (rank == 0 && !tail)                // no hands: their arrivals
+                        mbar_arrive_elect(smem_u32(&ctl->full[stage]), 2);
+                    if (tail) {
+                        mbar_expect_tx(to, bytes);
+                        tails |= 1u << stage;
+                        tail_phase ^= 1u << stage;
+                    }
+                    if (P.a_pair) {
+                        tma_3d(sA, &mA, to, 0, pa, a0 / 64);
+                    } else {
+                        tma_2d(sA, &mA, to, a0, pa);
+                        tma_2d(sA + kBox, &mA, to, a0 + 64, pa);
+                    }
+                    if (nb == 2 && P.b_pair) {
+                        tma_3d(sB, &mBig, to, 0, pb, bj0 / 64);
+                    } else {
+                        for (int x = 0; x < nb; ++x)
+                            tma_2d(sB + (uint32_t)x * kBox, &mB, to, bj0 + 64 * x, pb);
                     }
                 }
                 ++fills;
                 if (++stage == P.stages) { stage = 0; pe ^= 1u; }
             }
-            ok = __all_sync(0xffffffffu, ok);
         }
         // every stage's last release has arrived: none can reach this CTA later
         if (lane == 0)
@@ -556,7 +553,11 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             }
         __syncwarp();
         if (bad) dev_error(DEV_ERR_BOUNDS);
-        if (lane == 0) ctl->fills = fills;
+        if (lane == 0) {
+            ctl->fills = fills;
+            ctl->tails = tails;
+            ctl->tail_phase = tail_phase;
+        }
     } else if (warp == 1) {
         // ------------------------------------------- products (leader's warp)
         if (rank == 0) {
@@ -579,26 +580,27 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                     if (!tc_wait_warp(smem_u32(&ctl->tempty[buf]), te[buf], abort_flag)) break;
                     te[buf] ^= 1u;
                     fence_after();
-                    if (lane == 0)
-                        for (int kb = T.kb0; kb < T.kb1; ++kb) {
-                            if (!tc_wait(smem_u32(&ctl->full[stage]), pf, abort_flag)) { ok = false; break; }
-                            fence_after();
-                            const uint32_t off = ((uint32_t)stage * stage_bytes) >> 4;
-                            mma(off, off, (uint32_t)(kb - T.kb0));
-                            commit_pair(smem_u32(&ctl->empty[stage]));
-                            if (++stage == P.stages) { stage = 0; pf ^= 1u; }
-                        }
-                    if (lane == 0 && ok) commit_pair(smem_u32(&ctl->tfull[buf]));
+                    // the whole warp goes through the loop: converged, its
+                    // operands stay in uniform registers
+                    for (int kb = T.kb0; kb < T.kb1; ++kb) {
+                        if (!tc_wait_warp(smem_u32(&ctl->full[stage]), pf, abort_flag)) { ok = false; break; }
+                        fence_after();
+                        const uint32_t off = ((uint32_t)stage * stage_bytes) >> 4;
+                        mma(off, off, (uint32_t)(kb - T.kb0));
+                        commit_pair(smem_u32(&ctl->empty[stage]));
+                        if (++stage == P.stages) { stage = 0; pf ^= 1u; }
+                    }
+                    if (ok) commit_pair(smem_u32(&ctl->tfull[buf]));
                     buf ^= 1;
-                } else if (lane == 0) {
+                } else {
                     // a 64-wide step: its three planes' stages, then six products into a fresh accumulator
                     for (int kb = T.kb0; ok && kb < T.kb1; ++kb) {
-                        ok = tc_wait(smem_u32(&ctl->tempty[buf]), te[buf], abort_flag);
+                        ok = tc_wait_warp(smem_u32(&ctl->tempty[buf]), te[buf], abort_flag);
                         te[buf] ^= 1u;
                         uint32_t off[3], bar[3];
 #pragma unroll
                         for (int q = 0; q < 3; ++q) {
-                            ok = ok && tc_wait(smem_u32(&ctl->full[stage]), pf, abort_flag);
+                            ok = ok && tc_wait_warp(smem_u32(&ctl->full[stage]), pf, abort_flag);
                             off[q] = ((uint32_t)stage * stage_bytes) >> 4;
                             bar[q] = smem_u32(&ctl->empty[stage]);
                             if (++stage == P.stages) { stage = 0; pf ^= 1u; }
@@ -617,10 +619,9 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                         buf ^= 1;
                     }
                 }
-                ok = __all_sync(0xffffffffu, ok);
             }
-            if (lane == 0) commit_pair(smem_u32(&ctl->done));
             __syncwarp();
+            commit_pair(smem_u32(&ctl->done));
         }
     } else if (warp < kFindWarp) {
         // ----------------------------------------------------------- epilogue

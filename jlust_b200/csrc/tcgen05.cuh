@@ -33,8 +33,16 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_elect(uint32_t bar, uint32_t count) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e mbarrier.arrive.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(count)
+        : "memory");
 }
 // `count` arrivals on a barrier of this CTA.
 __device__ __forceinline__ void mbar_arrive_count(uint32_t bar, uint32_t count) {
@@ -60,33 +68,40 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 }
 
 // Copies whose completion is counted on `bar`, a barrier of either CTA of the
-// pair (shared::cluster address); the destination is in this CTA.
+// pair (shared::cluster address); the destination is in this CTA.  Issued, like
+// the arrivals below, by one elected lane of a converged warp, so that their
+// operands stay in uniform registers (from a branch of one lane each product
+// took some 75 cycles to issue).
 __device__ __forceinline__ void tma_2d(uint32_t dst, const void *map, uint32_t bar, int x, int y) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
 __device__ __forceinline__ void tma_3d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }__device__ __forceinline__ void tma_4d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z, int w) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// Arrives, once this thread's products so far are done, on the barrier at
-// this offset in both CTAs of the pair.
+// Arrives, once the elected lane's products so far are done, on the barrier at
+// this offset in both CTAs of the pair; called by a converged warp.
 __device__ __forceinline__ void commit_pair(uint32_t bar) {
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
         "h"((uint16_t)3)
         : "memory");
 }
@@ -111,26 +126,28 @@ __device__ __forceinline__ uint32_t instr_desc(uint32_t m, uint32_t n, bool a_mn
            ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-// Four products of 16 inner elements each, from one asm block: the
-// descriptors' low (address) words advance by a_step and b_step (16-byte
-// units, no carry: addresses stay below 256 KB).  first == 0 overwrites D.
+// Four products of 16 inner elements each, issued by one elected lane of a
+// converged warp: the descriptors' low (address) words advance by a_step and
+// b_step (16-byte units, no carry: addresses stay below 256 KB).  first == 0
+// overwrites D.
 template <int A_STEP, int B_STEP>
 __device__ __forceinline__ void mma_pair_k64(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
                                              uint32_t idesc, uint32_t first) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t.reg .b32 t, u;\n\t"
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t.reg .b32 t, u;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
         "setp.ne.b32 p, %5, 0;\n\t"
         "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, p;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, p;\n\t"
         "add.u32 t, %1, %7;\n\tadd.u32 u, %3, %8;\n\t"
         "mov.b64 a, {t, %2};\n\tmov.b64 b, {u, %4};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t"
         "add.u32 t, t, %7;\n\tadd.u32 u, u, %8;\n\t"
         "mov.b64 a, {t, %2};\n\tmov.b64 b, {u, %4};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t"
         "add.u32 t, t, %7;\n\tadd.u32 u, u, %8;\n\t"
         "mov.b64 a, {t, %2};\n\tmov.b64 b, {u, %4};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t}" ::"r"(d),
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %6, 1;\n\t}" ::"r"(d),
         "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(first), "r"(idesc), "n"(A_STEP), "n"(B_STEP)
         : "memory");
 }
