@@ -235,6 +235,110 @@ exclusive_scan_noalloc!(out::CuVector{Int32}, counts::CuVector{Int32}, base::Int
                   (Ptr{Cvoid}, Int64, CuPtr{Int32}, CuPtr{Int32}, Cint),
                   _stream(), length(counts), counts, out, Cint(base))); out)
 
+# ------------------------------------------------- a layer of experts
+# No counterpart in JLUST.  Matrices are CuMatrix of Float32 or BFloat16 whose
+# columns are tokens or slots (feature x token: row-major token x feature to the
+# library); W is a feature_out x feature_in x expert CuArray, i.e. row-major
+# in x out matrices.  Indices are 1-based; an id outside 1:E is dropped.
+_vt(::Type{Float32}) = Cint(0)
+_vt(::Type{T}) where {T} = sizeof(T) == 2 ? Cint(2) :
+    throw(JLUST.UnsupportedValueType(T, B200Backend()))
+_opt(x) = x === nothing ? CU_NULL : x
+_ld(x) = x === nothing ? Int64(0) : Int64(max(stride(x, 2), 1))
+
+# ids (k x tokens) -> rowptr (E + 1), source (k * tokens), slot (k x tokens)
+function route(ids::CuMatrix{Int32}, E::Integer)
+    k, T = size(ids)
+    rowptr = CuArray{Int32}(undef, E + 1)
+    source, slot = CuArray{Int32}(undef, k * T), similar(ids)
+    wsb = ccall((:jlb_route_workspace_size, lib), Csize_t, (Int64, Int64, Int64), T, k, E)
+    ws = CuArray{UInt8}(undef, Int(wsb))
+    _check(ccall((:jlb_route, lib), Cint,
+                 (Ptr{Cvoid}, Cint, Int64, Int64, Int64, CuPtr{Int32}, CuPtr{Int32}, CuPtr{Int32},
+                  CuPtr{Int32}, CuPtr{Cvoid}, Csize_t),
+                 _stream(), Cint(1), T, k, E, ids, rowptr, source, slot, ws, wsb))
+    rowptr, source, slot
+end
+
+# y[:, t] = sum_j g[j, t] z[:, slot[j, t]]
+function combine!(y::CuMatrix{V}, z::CuMatrix{V}, slot::CuMatrix{Int32}, g=nothing) where {V}
+    k, T = size(slot); N, S = size(z)
+    _check(ccall((:jlb_combine, lib), Cint,
+                 (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, Int64, CuPtr{Int32}, CuPtr{Float32},
+                  CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64),
+                 _stream(), _vt(V), Cint(1), T, k, S, N, slot, _opt(g), z, _ld(z), y, _ld(y)))
+    y
+end
+
+function combine_backward!(dz::CuMatrix{V}, dg::CuMatrix{Float32}, dy::CuMatrix{V}, z::CuMatrix{V},
+                           rowptr::CuVector{Int32}, slot::CuMatrix{Int32}, g=nothing) where {V}
+    k, T = size(slot); N, S = size(z)
+    _check(ccall((:jlb_combine_backward, lib), Cint,
+                 (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Int32},
+                  CuPtr{Int32}, CuPtr{Float32}, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
+                  CuPtr{Cvoid}, Int64, CuPtr{Float32}),
+                 _stream(), _vt(V), Cint(1), T, k, S, N, length(rowptr) - 1, rowptr, slot, _opt(g),
+                 z, _ld(z), dy, _ld(dy), dz, _ld(dz), dg))
+    dz, dg
+end
+
+# y[:, p] = act(x[:, rows[p]] W_e + b_e) + res[:, p], p in group e (jlb_grouped_mm);
+# rowptr === nothing: one group, the dense product.  transposed: W_e' (the gradient dx)
+function grouped_mm!(y::CuMatrix{V}, x::CuMatrix{V}, W::CuArray{V,3}, rowptr=nothing; rows=nothing,
+                     bias=nothing, act::Integer=0, res=nothing, z=nothing,
+                     transposed::Bool=false) where {V}
+    N, K = transposed ? (size(W, 2), size(W, 1)) : (size(W, 1), size(W, 2))
+    E, S, T = size(W, 3), size(y, 2), size(x, 2)
+    order, ldw, sw = Cint(transposed ? 1 : 0), stride(W, 2), stride(W, 3)
+    wsb = ccall((:jlb_grouped_mm_workspace_size, lib), Csize_t,
+                (Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
+                 Int64, Cint, Cint),
+                _vt(V), E, S, T, K, N, x, _ld(x), W, ldw, sw, order, Cint(rows !== nothing))
+    ws = CuArray{UInt8}(undef, Int(wsb))
+    _check(ccall((:jlb_grouped_mm, lib), Cint,
+                 (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Int32},
+                  CuPtr{Int32}, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64, Int64, Cint,
+                  CuPtr{Cvoid}, Int64, Cint, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
+                  CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Csize_t),
+                 _stream(), _vt(V), Cint(1), E, S, T, K, N, _opt(rowptr), _opt(rows), x, _ld(x), W,
+                 ldw, sw, order, _opt(bias), _ld(bias), Cint(act), _opt(res), _ld(res), _opt(z),
+                 _ld(z), y, _ld(y), ws, wsb))
+    y
+end
+
+# dW_e = sum over p in group e of x[:, rows[p]] dz[:, p]'
+function grouped_mm_wgrad!(dW::CuArray{V,3}, x::CuMatrix{V}, dz::CuMatrix{V}, rowptr=nothing;
+                           rows=nothing) where {V}
+    N, K, E = size(dW); S, T = size(dz, 2), size(x, 2)
+    wsb = ccall((:jlb_grouped_mm_wgrad_workspace_size, lib), Csize_t,
+                (Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
+                 Cint, Cint),
+                _vt(V), E, S, T, K, N, x, _ld(x), dz, _ld(dz), Cint(0), Cint(rows !== nothing))
+    ws = CuArray{UInt8}(undef, Int(wsb))
+    _check(ccall((:jlb_grouped_mm_wgrad, lib), Cint,
+                 (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Int32},
+                  CuPtr{Int32}, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
+                  Int64, Cint, CuPtr{Cvoid}, Csize_t),
+                 _stream(), _vt(V), Cint(1), E, S, T, K, N, _opt(rowptr), _opt(rows), x, _ld(x), dz,
+                 _ld(dz), dW, stride(dW, 2), stride(dW, 3), Cint(0), ws, wsb))
+    dW
+end
+
+# dz = dy .* act'(z) and db[:, e] = sum of group e's columns of dz
+function act_backward!(dz, db, dy::CuMatrix{V}, z, rowptr=nothing; act::Integer=0, E::Integer=1) where {V}
+    N, S = size(dy)
+    wsb = ccall((:jlb_act_backward_workspace_size, lib), Csize_t, (Int64, Int64, Int64, Cint),
+                E, S, N, Cint(db !== nothing))
+    ws = CuArray{UInt8}(undef, Int(wsb))
+    _check(ccall((:jlb_act_backward, lib), Cint,
+                 (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, CuPtr{Int32}, Cint, CuPtr{Cvoid},
+                  Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
+                  CuPtr{Cvoid}, Csize_t),
+                 _stream(), _vt(V), Cint(1), E, S, N, _opt(rowptr), Cint(act), dy, _ld(dy), _opt(z),
+                 _ld(z), _opt(dz), _ld(dz), _opt(db), _ld(db), ws, wsb))
+    dz, db
+end
+
 # --------------------------------------------------------- the drop-in policy
 const _CuUST = USTensor{T,I,N,VA} where {T,I,N,VA<:CuArray}
 JLUST.default_backend(::_CuUST, ::Type{<:Op{:SpMV}})  = B200Backend()

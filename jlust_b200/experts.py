@@ -203,12 +203,11 @@ def route(ids: torch.Tensor, n_experts: int, origin=0) -> Routing:
     L = _lib.load()
     wsb = L.jlb_route_workspace_size(T, k, E)
     ws = _workspace(wsb, dev)
-    n = T * k
-    # one allocation for the three index buffers
-    buf = ids.new_empty(2 * n + max(E, 0) + 1)
-    slot, source, rowptr = buf[:n].view(T, k), buf[n:2 * n], buf[2 * n:]
-    _lib.call("jlb_route", _stream(dev), base, T, k, E, _ptr(ids), _ptr(rowptr), _ptr(source),
-              _ptr(slot), _ptr(ws), wsb)
+    slot, source, rowptr = torch.empty_like(ids), ids.new_empty(T * k), ids.new_empty(max(E, 0) + 1)
+    st = L.jlb_route(_stream(dev), base, T, k, E, ids.data_ptr(), rowptr.data_ptr(),
+                     source.data_ptr(), slot.data_ptr(), _ptr(ws), wsb)
+    if st:
+        _lib.check(st, "jlb_route")
     r = Routing.__new__(Routing)
     r.rowptr, r.source, r.slot, r.origin = rowptr, source, slot, _origin(origin)
     return r
