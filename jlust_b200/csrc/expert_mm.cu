@@ -377,7 +377,7 @@ static int check_extents(int64_t E, int64_t S, int64_t T, int64_t K, int64_t N,
         return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "negative extent");
     if (!rowptr && E != 1)
         return fail(JLB_ERR_INVALID_ARGUMENT, "no row pointer: only one group has all the rows");
-    if (!rows && S != T)
+    if (!rows && S != T && S > 0)                 // an empty index buffer may have no address
         return fail(JLB_ERR_INCOMPATIBLE_EXTENTS, "x has %lld rows, the result %lld", (long long)T,
                     (long long)S);
     if (S > (int64_t)INT32_MAX - 1024 || T > (int64_t)INT32_MAX - 1024 ||

@@ -41,9 +41,12 @@
 // boxes, on a barrier of their own, and write zeros over its foreign rows
 // before the step is reported.
 //
-// Work split: a persistent grid of CTA pairs; pair c takes tiles c, c + G, ...
-// numbered group by group from rowptr on the device, inside a group in blocks
-// of the column tiles whose B stays in L2 while A streams past.  One warp of a CTA finds the tiles, 32
+// Work split: a persistent grid of CTA pairs over the tiles, numbered group by
+// group from rowptr on the device, inside a group in blocks of the column tiles
+// whose B stays in L2 while A streams past.  Pair c takes tile c and then c + G,
+// c + 2G, ... of equal tiles; ragged groups' tiles differ in cost, and there a
+// counter in the workspace hands out the next one (over random skewed groups
+// the last pair ends 8 % after the mean, in turn 17 %).  One warp of a CTA finds the tiles, 32
 // groups at a time, up to four ahead, and passes them to the other roles
 // through a ring in shared memory: found by each role at its tile's start, the
 // tensor cores stood still for some 1500 cycles a tile.
@@ -75,6 +78,7 @@ constexpr int kFindWarp = 2 + kEpiWarps;                // finds the tiles
 constexpr int kTcThreads = 32 + kFindWarp * 32;         // without the loaders
 constexpr int kLoadWarp = kFindWarp + 1, kLoaders = 128;  // the loader warps
 constexpr int kTileRing = 4;                            // tiles found ahead
+constexpr int kTickets = 4;                             // numbers on their way to the pair's other CTA
 constexpr int kForward = 32;                            // the warp that reports the loaders' stages
 constexpr int kPitch = 36;                              // words a pair of columns takes in the epilogue's turn
 constexpr uint32_t kTurnBytes = kEpiWarps * 16 * kPitch * 4;
@@ -103,6 +107,7 @@ struct TcArgs {
     int pairs, max_splits;        // CTA pairs launched; parts a tile may be split into (> 1: rowptr decides)
     int full, splits;             // tiles not split and the parts of the others, when the host knows
     float *part;                  // one 256 x bn_max fp32 tile for each part
+    int *counter;                 // tiles handed out beyond each pair's first; null: in turn
 };
 
 // A pipeline stage: A's half and, in 32-row boxes, B's.
@@ -118,7 +123,8 @@ struct Tile {
 struct TcCtl {
     uint64_t full[kMaxStages], empty[kMaxStages], rows[kMaxStages], go[kMaxStages];
     uint64_t tfull[2], tempty[2], done;
-    uint64_t sfull[kTileRing], sempty[kTileRing];
+    uint64_t sfull[kTileRing], sempty[kTileRing], tbar[kTickets], tack[kTickets];
+    int ticket[kTickets];
     Tile ring[kTileRing];
     uint32_t tmem, fills;
     uint32_t tails, tail_phase;                   // stages a last step used, and their go barriers' phases, a bit each
@@ -454,6 +460,10 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             mbar_init(smem_u32(&ctl->tempty[b]), 2 * kEpiWarps);
         }
         mbar_init(smem_u32(&ctl->done), 1);
+        for (int b = 0; b < kTickets; ++b) {
+            mbar_init(smem_u32(&ctl->tbar[b]), 1);
+            mbar_init(smem_u32(&ctl->tack[b]), 1);
+        }
         for (int b = 0; b < kTileRing; ++b) {
             mbar_init(smem_u32(&ctl->sfull[b]), 1);
             // the warps that read it: copies, epilogue, the leader's products, loaders and their report
@@ -731,9 +741,9 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
         // ------------------------------------------------------------- tiles
         Walk<GRAD> walk;
         walk.init(P);
-        int slot = 0;
-        uint32_t ph = 1u;
-        for (int t = pair;; t += pairs) {
+        int slot = 0, tk = 0;
+        uint32_t ph = 1u, tph = 0u;
+        for (int t = pair;;) {
             Tile T;
             const bool have = walk.find(P, t, T);
             if (!tc_wait_warp(smem_u32(&ctl->sempty[slot]), ph, abort_flag)) break;
@@ -744,6 +754,29 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             }
             if (++slot == kTileRing) { slot = 0; ph ^= 1u; }
             if (!have) break;
+            if (!P.counter) {
+                t += pairs;
+                continue;
+            }
+            // the next number, drawn by the leader and sent to the other CTA,
+            // which reports each ticket's place free again (groups without
+            // rows let one CTA's roles run ahead of the other's)
+            if (rank == 0) {
+                if (!tc_wait_warp(smem_u32(&ctl->tack[tk]), tph ^ 1u, abort_flag)) break;
+                if (lane == 0) {
+                    t = pairs + atomicAdd(P.counter, 1);
+                    store_remote(map_rank(smem_u32(&ctl->ticket[tk]), 1), (uint32_t)t, map_rank(smem_u32(&ctl->tbar[tk]), 1));
+                }
+                t = __shfl_sync(0xffffffffu, t, 0);
+            } else {
+                __syncwarp();
+                mbar_expect_tx(smem_u32(&ctl->tbar[tk]), 4);
+                if (!tc_wait_warp(smem_u32(&ctl->tbar[tk]), tph, abort_flag)) break;
+                t = *(volatile int *)&ctl->ticket[tk];
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&ctl->tack[tk]), 0));
+            }
+            if (++tk == kTickets) { tk = 0; tph ^= 1u; }
         }
     } else if (warp < kLoadWarp + kLoaders / 32) {
         // ------------------------------------------------------ loader warps
@@ -1001,14 +1034,15 @@ static int device_sms() {
 
 // Columns of the instruction a call needs at most, and how its tiles are
 // split: tiles is their number (product: an upper bound when rowptr decides).
+constexpr size_t kCounterBytes = 256;                   // the workspace's first bytes: the tile counter
 struct TcPlan {
     int bn_max, pairs, max_splits, full, splits;
-    bool finish;
+    bool finish, dynamic;
     int rest;                      // split tiles, at most
     size_t part_bytes;
 };
-static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, int64_t steps) {
-    TcPlan p{bn_max, device_sms() / 2, 1, INT32_MAX, 1, false, 0, 0};
+static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, bool ragged, int64_t steps) {
+    TcPlan p{bn_max, device_sms() / 2, 1, INT32_MAX, 1, false, false, 0, 0};
     if (tiles > INT32_MAX / 2) return p;           // the launch refuses
     // at least four steps a part; and finish_tc's launch is worth it only when
     // a partly filled last round can be a sixth of the work
@@ -1025,6 +1059,10 @@ static TcPlan tc_plan(int bn_max, int64_t tiles, bool exact, int64_t steps) {
     }
     if (p.finish) p.part_bytes = (size_t)p.pairs * 256 * bn_max * 4;
     else if (tiles < p.pairs) p.pairs = (int)tiles;
+    // handed out where tiles differ in cost and two rounds or more of them hide
+    // the counter's clearing (3.5 us): gradients of 8192 rows over 16 experts 375
+    // -> 365 us, a 32,044-row prefill 558 -> 544; decode steps' tiles are alike
+    p.dynamic = ragged && tiles > 2 * p.pairs;
     return p;
 }
 
@@ -1041,7 +1079,9 @@ static int launch_tc(cudaStream_t st, const CUtensorMap &a, const CUtensorMap &b
     P.max_splits = plan.max_splits;
     P.full = plan.full;
     P.splits = plan.splits;
-    P.part = (float *)ws;
+    P.part = (float *)((char *)ws + kCounterBytes);
+    P.counter = plan.dynamic ? (int *)ws : nullptr;
+    if (plan.dynamic) JLB_CUDA(cudaMemsetAsync(ws, 0, sizeof(int), st));
     P.stages = (int)((227 * 1024 - extra) / stage);
     if (P.stages > kMaxStages) P.stages = kMaxStages;
     const size_t smem = (size_t)P.stages * stage + extra;
@@ -1068,19 +1108,20 @@ static int widest(int dtype) { return dtype == JLB_F32 ? 128 : 256; }   // F32: 
 static TcPlan plan_product(const Product &p) {
     const int wide = widest(p.dtype), bn = p.S >= wide ? wide : (int)((p.S + 31) / 32 * 32);
     if (!p.rowptr)
-        return tc_plan(bn, col_tiles((int)p.S, bn) * ceil_div(p.N, 256), true, ceil_div(p.K, 64));
+        return tc_plan(bn, col_tiles((int)p.S, bn) * ceil_div(p.N, 256), true, false, ceil_div(p.K, 64));
     const int64_t cols = ceil_div(p.S, bn) + (p.E < p.S ? p.E : p.S);
-    return tc_plan(bn, cols * ceil_div(p.N, 256), false, ceil_div(p.K, 64));
+    return tc_plan(bn, cols * ceil_div(p.N, 256), false, p.S >= 64 * p.E, ceil_div(p.K, 64));
 }
 
 static TcPlan plan_gradient(const Gradient &g) {
     const int64_t J = g.w_order == JLB_ROW_MAJOR ? g.K : g.N, I = g.w_order == JLB_ROW_MAJOR ? g.N : g.K;
     const int bn = J > 128 ? widest(g.dtype) : 128;
-    return tc_plan(bn, g.E * ceil_div(I, 256) * ceil_div(J, bn), true, ceil_div(g.S / g.E, 64));
+    return tc_plan(bn, g.E * ceil_div(I, 256) * ceil_div(J, bn), true, g.E > 1 && g.S >= 64 * g.E, ceil_div(g.S / g.E, 64));
 }
 
-size_t tc_product_workspace(const Product &P) { return plan_product(P).part_bytes; }
-size_t tc_gradient_workspace(const Gradient &G) { return plan_gradient(G).part_bytes; }
+static size_t plan_bytes(const TcPlan &p) { return p.part_bytes || p.dynamic ? kCounterBytes + p.part_bytes : 0; }
+size_t tc_product_workspace(const Product &P) { return plan_bytes(plan_product(P)); }
+size_t tc_gradient_workspace(const Gradient &G) { return plan_bytes(plan_gradient(G)); }
 
 // Status, or -1 when the driver refuses a tensor map (the caller takes
 // another kernel).  F32: p.x and p.w are three bf16 planes each, [3][T][ldx]

@@ -44,6 +44,13 @@ __device__ __forceinline__ void mbar_arrive_elect(uint32_t bar, uint32_t count) 
         "@e mbarrier.arrive.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(count)
         : "memory");
 }
+// Stores one word in a CTA of the cluster and counts its 4 bytes on a barrier
+// there (both shared::cluster addresses).
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t value, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(value),
+                 "r"(bar)
+                 : "memory");
+}
 // `count` arrivals on a barrier of this CTA.
 __device__ __forceinline__ void mbar_arrive_count(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");

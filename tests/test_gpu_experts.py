@@ -467,6 +467,14 @@ def test_zero_extents(dtype):
     dx, dw, db = J.grouped_matmul_backward(torch.empty(0, 16, dtype=dtype, device=DEV), none, w,
                                            dev_i32([0, 0, 0, 0]), bias=True)
     assert dx.shape == (0, 8) and not dw.any() and not db.any()
+    # no slots, though x has rows
+    x1, no = randn((4, 8), dtype, 3), dev_i32([])
+    assert J.grouped_matmul(x1, w, dev_i32([0, 0, 0, 0]), rows=no).shape == (0, 16)
+    h = J.prepare(J.B200Backend(), J.GroupedMMOp, w, bias=b)
+    assert J.execute(h, x1, dev_i32([0, 0, 0, 0]), rows=no).shape == (0, 16)
+    dx, dw, db = J.grouped_matmul_backward(torch.empty(0, 16, dtype=dtype, device=DEV), x1, w,
+                                           dev_i32([0, 0, 0, 0]), rows=no, bias=True)
+    assert dx.shape == (0, 8) and not dw.any() and not db.any()
     # no inner dimension: the bias alone; no columns: nothing
     x0, w0 = torch.empty(5, 0, dtype=dtype, device=DEV), torch.empty(3, 0, 16, dtype=dtype, device=DEV)
     y = J.grouped_matmul(x0, w0, dev_i32([0, 2, 2, 5]), bias=b, act="relu")
