@@ -784,7 +784,7 @@ extern "C" JLB_API int jlb_mm_plan_destroy(jlb_mm_plan plan) {
 
 extern "C" JLB_API size_t jlb_mm_plan_workspace_size(jlb_mm_plan plan, int64_t S, int64_t T,
                                                      const void *x, int64_t ldx, int gather) {
-    if (!plan) return 0;
+    if (!plan || S < 0 || T < 0) return 0;
     emm::Product P = plan->p;
     P.S = S;
     P.T = T;
@@ -828,6 +828,7 @@ extern "C" JLB_API size_t jlb_grouped_mm_workspace_size(int dtype, int64_t E, in
                                                         int64_t K, int64_t N, const void *x,
                                                         int64_t ldx, const void *w, int64_t ldw,
                                                         int64_t w_stride, int w_order, int gather) {
+    if (E < 0 || K < 0 || N < 0) return 0;
     jlb_mm_plan_s h;
     h.p = emm::Product{};
     h.p.dtype = dtype;

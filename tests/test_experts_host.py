@@ -80,6 +80,22 @@ def test_product_statuses(kw, status):
     assert len(_lib.last_error()) > 0
 
 
+def test_size_queries_take_any_extents():
+    L = _lib.load()
+    for bad in (-1, -40, -2 ** 40):
+        for i in range(5):                      # E, S, T, K, N
+            a = [2, 64, 64, 64, 64]
+            a[i] = bad
+            assert L.jlb_grouped_mm_workspace_size(2, *a, P, 64, P, 64, 4096, 0, 0) == 0
+            assert L.jlb_grouped_mm_wgrad_workspace_size(2, *a, P, 64, P, 64, 0, 0) == 0
+    for a in ((0, 5, 5, 8, 8), (3, 0, 0, 8, 8), (3, 5, 5, 0, 8), (3, 5, 5, 8, 0), (3, 5, 0, 8, 8)):
+        for dtype in (0, 2):
+            L.jlb_grouped_mm_workspace_size(dtype, *a, P, 8, P, 8, 64, 0, 0)
+            L.jlb_grouped_mm_wgrad_workspace_size(dtype, *a, P, 8, P, 8, 0, 0)
+    assert L.jlb_act_backward_workspace_size(-1, 5, 8, 1) == 0
+    assert L.jlb_route_workspace_size(-1, 5, 8) == 0
+
+
 def test_other_statuses():
     L = _lib.load()
     assert L.jlb_route(None, 0, 4, 2, 4096, P, P, P, P, None, 0) == 1          # too many experts
