@@ -67,6 +67,25 @@ def test_route(T, k, E, drop, base):
     assert np.array_equal(r.source.cpu().numpy(), source)
 
 
+def test_route_of_millions_of_entries():
+    """More chunks than a CTA adds up by itself: the counts are scanned."""
+    for T, k, E in ((700_001, 2, 19), (400_000, 4, 2048), (40_000, 4, 700)):
+        ids = torch.randint(-1, E, (T, k), generator=torch.Generator().manual_seed(E), dtype=torch.int32)
+        r = J.route(ids.to(DEV), E, origin=0)
+        J.device_status()
+        flat = ids.view(-1).long()
+        order = torch.sort(torch.where(flat < 0, E, flat), stable=True).indices
+        n = int((flat >= 0).sum())
+        counts = torch.bincount(flat[flat >= 0], minlength=E)
+        assert torch.equal(r.rowptr.cpu().long(), torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]))
+        source = torch.full((T * k,), -1, dtype=torch.long)
+        source[:n] = order[:n] // k
+        slot = torch.full((T * k,), -1, dtype=torch.long)
+        slot[order[:n]] = torch.arange(n)
+        assert torch.equal(r.source.cpu().long(), source)
+        assert torch.equal(r.slot.cpu().long().view(-1), slot)
+
+
 def test_route_one_expert_takes_all_and_repeats():
     ids = torch.full((9001, 3), 5, dtype=torch.int32, device=DEV)
     a, b = J.route(ids, 9), J.route(ids, 9)
