@@ -246,18 +246,21 @@ __device__ __forceinline__ void store_values(T *p, const float (&v)[V]) {
 // y[t] = sum_j g[t, j] z[slot[t, j]] in the order of j, fp32 sums rounded
 // once to the value type.  V columns a thread (16 bytes, or one when the
 // layout is not aligned); blockDim = (column threads, tokens).
-constexpr int kRowsAhead = 4;
-template <int V>
-constexpr int kColsAhead = V == 1 ? 4 : 2;     // column groups a thread has under way
-template <typename T, int V>
-__global__ void __launch_bounds__(256)
+constexpr int kCombineThreads = 128;
+// R rows of C column groups are under way in a thread.  Bound by HBM: 8191
+// tokens x 4 rows of 4096 bf16 55 us (floor 52; 58 with R = 4, C = 2 and CTAs
+// of 256), 16,384 x 2 of 2048 36 us (floor 31; 46 with R = 4, C = 2), 8192 x 3
+// of 2048 24 us with R = 3 (27 with R = 2).  A value a load is bound by the
+// loads' number: 16,384 x 4 rows of 1001 bf16 59 us (floor 25; 71 with C = 4);
+// 16-byte blocks shifted into place took 52 us there and more elsewhere.
+template <typename T, int V, int R, int C>
+__global__ void __launch_bounds__(kCombineThreads)
 combine_rows(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__restrict__ slot,
              const float *__restrict__ g, const T *__restrict__ z, int64_t ldz,
              T *__restrict__ y, int64_t ldy) {
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (t >= T_) return;
     const int32_t *sl = slot + t * k;
-    constexpr int C = kColsAhead<V>;
     const int64_t step = (int64_t)blockDim.x * V;       // from one of a thread's column groups to the next
     for (int64_t c = (int64_t)blockIdx.y * step * C + threadIdx.x * V; c < N; c += (int64_t)gridDim.y * step * C) {
         float acc[C][V];
@@ -265,26 +268,31 @@ combine_rows(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *_
         for (int x = 0; x < C; ++x)
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[x][i] = 0.0f;
-        for (int j0 = 0; j0 < k; j0 += kRowsAhead) {      // their loads on the way together
-            Raw<T, V> v[kRowsAhead][C];
-            float w[kRowsAhead];
-            bool use[kRowsAhead];
+        for (int j0 = 0; j0 < k; j0 += R) {      // their loads on the way together
+            Raw<T, V> v[R][C];
+            float w[R];
+            int p[R];                                     // slots, -1: none
+            // all slots before any row, so that no row waits for the next slot
 #pragma unroll
-            for (int q = 0; q < kRowsAhead; ++q) {
-                const int j = j0 + q;
-                const int64_t p = j < k ? (int64_t)__ldg(sl + j) - base : -1;
-                use[q] = p >= 0 && p < S;                 // a dropped entry has no slot
-                if (p >= S) dev_error(DEV_ERR_BOUNDS);
-                if (use[q]) {
-                    w[q] = g ? __ldg(g + t * k + j) : 1.0f;
-#pragma unroll
-                    for (int x = 0; x < C; ++x)
-                        if (c + x * step < N) v[q][x].load(z + p * ldz + c + x * step);
+            for (int q = 0; q < R; ++q) {
+                p[q] = -1;
+                w[q] = 0.0f;
+                if (j0 + q < k) {
+                    const int64_t at = (int64_t)__ldg(sl + j0 + q) - base;
+                    w[q] = g ? __ldg(g + t * k + j0 + q) : 1.0f;
+                    if (at >= S) dev_error(DEV_ERR_BOUNDS);
+                    p[q] = at < 0 || at >= S ? -1 : (int)at;      // a dropped entry has no slot
                 }
             }
 #pragma unroll
-            for (int q = 0; q < kRowsAhead; ++q)
-                if (use[q])
+            for (int x = 0; x < C; ++x)
+                if (c + x * step < N)
+#pragma unroll
+                    for (int q = 0; q < R; ++q)
+                        if (p[q] >= 0) v[q][x].load(z + (int64_t)p[q] * ldz + c + x * step);
+#pragma unroll
+            for (int q = 0; q < R; ++q)
+                if (p[q] >= 0)
 #pragma unroll
                     for (int x = 0; x < C; ++x)
 #pragma unroll
@@ -296,33 +304,62 @@ combine_rows(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *_
     }
 }
 
+constexpr int kBwdThreads = 128;
+
+// Rows first, first + step, ... past the last slot.
+template <typename T>
+__device__ __forceinline__ void clear_rows(int64_t first, int64_t step,
+                                           const int32_t *__restrict__ live_end, int base, int64_t S,
+                                           int64_t N, T *__restrict__ dz, int64_t lddz) {
+    int64_t end = (int64_t)__ldg(live_end) - base;
+    end = end < 0 ? 0 : end > S ? S : end;
+    for (int64_t p = end + first; p < S; p += step)
+        for (int64_t c = (int64_t)threadIdx.x; c < N; c += kBwdThreads) dz[p * lddz + c] = T(0.0f);
+}
+
+// dg[j] = the CTA's sum of dot[j] for j < left, by a fixed tree.
+template <int J>
+__device__ __forceinline__ void write_dots(const float (&dot)[J], int left, float *__restrict__ dg,
+                                           float (&part)[kBwdThreads / kWarp][J]) {
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const float s = warp_sum(dot[j]);
+        if (lane == 0) part[warp][j] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < J && (int)threadIdx.x < left) {
+        float s = 0.0f;
+        for (int q = 0; q < kBwdThreads / kWarp; ++q) s += part[q][threadIdx.x];
+        dg[threadIdx.x] = s;
+    }
+}
+
 // dz[slot[t, j]] = g[t, j] dy[t] and dg[t, j] = <dy[t], z[slot[t, j]]>: one
-// CTA a token, dy read once for up to 8 entries.  Rows of dz past the last
+// CTA a token, dy read once for J entries.  Rows of dz past the last
 // slot are zeroed.  The dot product's terms are summed per thread, then by a
 // fixed tree over the CTA.
-constexpr int kBwdThreads = 128, kBwdJ = 8;
-template <typename T, int V>
+// J follows k, so that registers are left for C column groups under way:
+// 16,384 tokens x 2 rows of 2048 bf16 53 us (floor 52) against 83 with J = 8,
+// 8191 x 4 of 4096 92 against 101.
+template <typename T, int V, int J, int C>
 __global__ void __launch_bounds__(kBwdThreads)
 combine_bwd(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__restrict__ slot,
             const int32_t *__restrict__ live_end, const float *__restrict__ g,
             const T *__restrict__ z, int64_t ldz, const T *__restrict__ dy, int64_t lddy,
             T *__restrict__ dz, int64_t lddz, float *__restrict__ dg) {
-    __shared__ float part[kBwdThreads / kWarp][kBwdJ];
+    __shared__ float part[kBwdThreads / kWarp][J];
     const int64_t t = blockIdx.x;
-    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     if (t >= T_) {                                // the CTAs after the tokens: rows of no slot
-        int64_t end = (int64_t)__ldg(live_end) - base;
-        end = end < 0 ? 0 : end > S ? S : end;
-        for (int64_t p = end + (t - T_); p < S; p += (int64_t)gridDim.x - T_)
-            for (int64_t c = (int64_t)threadIdx.x; c < N; c += kBwdThreads)
-                dz[p * lddz + c] = T(0.0f);
+        clear_rows(t - T_, gridDim.x - T_, live_end, base, S, N, dz, lddz);
         return;
     }
-    for (int j0 = 0; j0 < k; j0 += kBwdJ) {
-        int p[kBwdJ];                              // slots, -1: none
-        float w[kBwdJ], dot[kBwdJ];
+    for (int j0 = 0; j0 < k; j0 += J) {
+        int p[J];                              // slots, -1: none
+        float w[J], dot[J];
 #pragma unroll
-        for (int j = 0; j < kBwdJ; ++j) {
+        for (int j = 0; j < J; ++j) {
             p[j] = -1;
             w[j] = dot[j] = 0.0f;
             if (j0 + j < k) {
@@ -332,16 +369,15 @@ combine_bwd(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__
                 p[j] = s < 0 || s >= S ? -1 : (int)s;
             }
         }
-        constexpr int C = V == 1 ? 4 : 1;                 // column groups a thread has under way
         for (int64_t c0 = (int64_t)threadIdx.x * V; c0 < N; c0 += kBwdThreads * V * C) {
-            Raw<T, V> d[C], v[kBwdJ][C];
+            Raw<T, V> d[C], v[J][C];
 #pragma unroll
             for (int x = 0; x < C; ++x) {
                 const int64_t c = c0 + x * kBwdThreads * V;
                 if (c >= N) continue;
                 d[x].load(dy + t * lddy + c);
 #pragma unroll
-                for (int j = 0; j < kBwdJ; ++j)
+                for (int j = 0; j < J; ++j)
                     if (p[j] >= 0) v[j][x].load(z + (int64_t)p[j] * ldz + c);
             }
 #pragma unroll
@@ -349,7 +385,7 @@ combine_bwd(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__
                 const int64_t c = c0 + x * kBwdThreads * V;
                 if (c >= N) continue;
 #pragma unroll
-                for (int j = 0; j < kBwdJ; ++j) {
+                for (int j = 0; j < J; ++j) {
                     if (p[j] < 0) continue;
                     float o[V];
 #pragma unroll
@@ -361,20 +397,7 @@ combine_bwd(int64_t T_, int k, int64_t S, int64_t N, int base, const int32_t *__
                 }
             }
         }
-        if (dg) {
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < kBwdJ; ++j) {
-                const float s = warp_sum(dot[j]);
-                if (lane == 0) part[warp][j] = s;
-            }
-            __syncthreads();
-            if (threadIdx.x < kBwdJ && j0 + (int)threadIdx.x < k) {
-                float s = 0.0f;
-                for (int q = 0; q < kBwdThreads / kWarp; ++q) s += part[q][threadIdx.x];
-                dg[t * k + j0 + threadIdx.x] = s;
-            }
-        }
+        if (dg) write_dots<J>(dot, k - j0, dg + t * k + j0, part);
     }
 }
 
@@ -465,17 +488,22 @@ int run_combine(cudaStream_t st, int64_t Tn, int64_t k, int64_t S, int64_t N, in
                 const int32_t *slot, const float *g, const T *z, int64_t ldz, T *y, int64_t ldy) {
     constexpr int V = 16 / (int)sizeof(T);
     const bool vec = N % V == 0 && ldz % V == 0 && ldy % V == 0 && aligned16(z) && aligned16(y);
-    const int64_t items = vec ? ceil_div(N / V, routing::kColsAhead<V>) : ceil_div(N, routing::kColsAhead<1>);
+    const bool two = k == 2 || k == 4;
+    const int64_t items = ceil_div(vec ? N / V : N, !vec ? 8 : k == 1 || two ? 4 : 2);
     int tx = 32;
-    while (tx < 256 && tx < items) tx *= 2;
-    const int ty = 256 / tx;
+    while (tx < routing::kCombineThreads && tx < items) tx *= 2;
+    const int ty = routing::kCombineThreads / tx;
     const dim3 block(tx, ty);
     const dim3 grid((unsigned)ceil_div(Tn, ty),
                     (unsigned)(ceil_div(items, tx) < 65535 ? ceil_div(items, tx) : 65535));
-    if (vec)
-        routing::combine_rows<T, V><<<grid, block, 0, st>>>(Tn, (int)k, S, N, base, slot, g, z, ldz, y, ldy);
-    else
-        routing::combine_rows<T, 1><<<grid, block, 0, st>>>(Tn, (int)k, S, N, base, slot, g, z, ldz, y, ldy);
+    // few rows leave registers for more columns; three rows at a time suit the
+    // other counts (a fourth would be idle in the last pass)
+    const auto kernel = vec ? (k == 1 ? routing::combine_rows<T, V, 1, 4>
+                               : two  ? routing::combine_rows<T, V, 2, 4>
+                                      : routing::combine_rows<T, V, 3, 2>)
+                            : (k == 1 ? routing::combine_rows<T, 1, 1, 8>
+                                      : routing::combine_rows<T, 1, 2, 8>);
+    kernel<<<grid, block, 0, st>>>(Tn, (int)k, S, N, base, slot, g, z, ldz, y, ldy);
     JLB_LAUNCH_CHECK("combine_rows");
     return ok();
 }
@@ -488,12 +516,16 @@ int run_combine_bwd(cudaStream_t st, int64_t Tn, int64_t k, int64_t S, int64_t N
     const bool vec = N % V == 0 && ldz % V == 0 && lddy % V == 0 && lddz % V == 0 &&
                      aligned16(z) && aligned16(dy) && aligned16(dz);
     const unsigned grid = (unsigned)(Tn + 148);   // 148 CTAs for the rows of no slot
-    if (vec)
-        routing::combine_bwd<T, V><<<grid, routing::kBwdThreads, 0, st>>>(
-            Tn, (int)k, S, N, base, slot, live_end, g, z, ldz, dy, lddy, dz, lddz, dg);
-    else
-        routing::combine_bwd<T, 1><<<grid, routing::kBwdThreads, 0, st>>>(
-            Tn, (int)k, S, N, base, slot, live_end, g, z, ldz, dy, lddy, dz, lddz, dg);
+    const auto kernel =
+        vec ? (k == 1   ? routing::combine_bwd<T, V, 1, 2>
+               : k == 2 ? routing::combine_bwd<T, V, 2, 2>
+               : k <= 4 ? routing::combine_bwd<T, V, 4, 2>
+                        : routing::combine_bwd<T, V, 8, 1>)
+            : (k <= 2   ? routing::combine_bwd<T, 1, 2, 4>
+               : k <= 4 ? routing::combine_bwd<T, 1, 4, 4>
+                        : routing::combine_bwd<T, 1, 8, 4>);
+    kernel<<<grid, routing::kBwdThreads, 0, st>>>(Tn, (int)k, S, N, base, slot, live_end, g, z, ldz,
+                                                  dy, lddy, dz, lddz, dg);
     JLB_LAUNCH_CHECK("combine_bwd");
     return ok();
 }
