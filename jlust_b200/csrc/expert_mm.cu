@@ -415,6 +415,8 @@ struct Copy {
     const int32_t *idx;           // source row of each row, or null; an index outside [0, limit): a row of zeros
     int64_t limit;
     const int32_t *live_end;      // rows from *live_end on are of no group and hold nothing
+    const int32_t *rowptr;        // matrices whose group has none of the S rows are not read, or null: all are
+    int64_t S;
     int base, vec;                // vec: the source's rows are 16-byte aligned
     void *dst;
     int64_t ldd;
@@ -432,6 +434,11 @@ __device__ __forceinline__ bool copy_source(const Copy &c, int64_t w, int per_pi
     const int64_t e = c.experts == 1 ? 0 : r / c.rows;
     int64_t sr = r - e * c.rows;
     if (c.live_end && sr >= (int64_t)__ldg(c.live_end) - c.base) return false;
+    if (c.rowptr) {
+        int lo, hi;
+        group_rows(c.rowptr, c.base, c.S, e, lo, hi);
+        if (lo == hi) return false;
+    }
     s = (const T *)c.src + e * c.stride;
     if (c.idx) {
         sr = (int64_t)__ldg(c.idx + sr) - c.base;
@@ -637,8 +644,12 @@ static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_by
                 q.p.T = P.S;
             }
         }
-        if (q.copy_w)
+        if (q.copy_w) {
             w = make_copy(q.split, P.w, P.E, row ? P.K : P.N, row ? P.N : P.K, P.ldw, P.w_stride, base + q.w_at);
+            w.rowptr = P.rowptr;
+            w.S = P.S;
+            w.base = P.base;
+        }
         int r = launch_copies(st, q.split, x, w);
         if (r) return r;
         if (q.copy_x) q.p.x = base + q.x_at;

@@ -3,7 +3,7 @@
 // costs, so the kernel is a stream over W with the rows' values beside it.
 //
 // A CTA takes one group and one tile of its columns; up to 8 rows at a time
-// sit in shared memory as fp32.  Row-major W: 8 lanes read 128 contiguous
+// (16 where F32 has more) sit in shared memory as fp32.  Row-major W: 8 lanes read 128 contiguous
 // bytes of one row of W, 32 rows of W a pass; a thread keeps sums[rows][8]
 // and each weight it loads meets every row.  Column-major W: 8 lanes read 128
 // bytes along K, a thread holds 4 columns.  The inner dimension is split over
@@ -32,7 +32,7 @@ constexpr int kSkCols = 4;                 // columns a thread holds for column-
 // Tile width: VEC values a lane (16 bytes, or one), LX lanes side by side.
 template <typename T, bool COL, int VEC>
 struct SkShape {
-    static constexpr int kLX = VEC > 1 ? 8 : 32;
+    static constexpr int kLX = VEC > 1 ? 8 : COL ? 32 / (int)sizeof(T) : 32;
     static constexpr int kTile = COL ? kSkCols * (32 / kLX) : kLX * VEC;
 };
 
@@ -82,27 +82,46 @@ __device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0
     for (int m = 0; m < MR; ++m)
 #pragma unroll
         for (int c = 0; c < NS; ++c) acc[m][c] = 0.0f;
+    // loads a thread has under way (column-major: times four)
+    constexpr int U = !COL ? MR <= 8 ? 8 : 4 : VEC == 1 ? 4 : MR <= 2 ? 2 : 1;
+    constexpr int kStep = U * (COL ? kSkWarps * LX * VEC : kSkThreads / LX);
+    static_assert(kSkK % kStep == 0, "a staged part is a whole number of steps");
+    int src[MR];                                   // the rows in x, -1: none
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+        src[m] = -1;
+        if (m < nrows) {
+            int64_t s = row + m;
+            if (P.rows) s = (int64_t)__ldg(P.rows + s) - P.base;
+            if (s < 0 || s >= P.T) bad = true;
+            else src[m] = (int)s;
+        }
+    }
     for (int64_t kc = k0; kc < k1; kc += kSkK) {
         const int kn = (int)(k1 - kc < kSkK ? k1 - kc : kSkK);
         __syncthreads();                           // the values of the step before are used
-        for (int q = threadIdx.x; q < MR * kn; q += kSkThreads) {
-            const int m = q / kn, k = q - m * kn;
-            float v = 0.0f;
-            if (m < nrows) {
-                int64_t s = row + m;
-                if (P.rows) s = (int64_t)__ldg(P.rows + s) - P.base;
-                if (s < 0 || s >= P.T) bad = true;
-                else v = to_f32(((const T *)P.x)[s * P.ldx + kc + k]);
+        // past kn the rows hold zeros, up to a whole step of the loops below
+        const int kp = min(kSkK, (kn + kStep - 1) / kStep * kStep);
+        for (int k = threadIdx.x; k < kp; k += kSkThreads) {
+            float v[MR];
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                v[m] = 0.0f;
+                if (src[m] >= 0 && k < kn) v[m] = to_f32(((const T *)P.x)[(int64_t)src[m] * P.ldx + kc + k]);
             }
-            xs[COL ? m * (kSkK + 8) + k : k * MR + m] = v;
+            if (!COL && MR % 4 == 0) {
+#pragma unroll
+                for (int m = 0; m < MR; m += 4)
+                    *reinterpret_cast<float4 *>(xs + k * MR + m) = make_float4(v[m], v[m + 1], v[m + 2], v[m + 3]);
+            } else {
+#pragma unroll
+                for (int m = 0; m < MR; ++m) xs[COL ? m * (kSkK + 8) + k : k * MR + m] = v[m];
+            }
         }
-        // a column-major step may read up to 16 bytes past kn: zeros there
-        if (COL && threadIdx.x < MR * VEC) xs[(threadIdx.x / VEC) * (kSkK + 8) + kn + threadIdx.x % VEC] = 0.0f;
         __syncthreads();
         // U loads are on their way before the first is used
         if (!COL) {
             constexpr int KY = kSkThreads / LX;    // rows of W a pass
-            constexpr int U = 8;
             const int ky = threadIdx.x / LX, n = (int)min((int64_t)VEC, P.N - (n0 + lx * VEC));
             const T *p = w + kc * P.ldw + n0 + lx * VEC;
             for (int kb = ky; kb < kn && n > 0; kb += U * KY) {
@@ -115,19 +134,24 @@ __device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int k = kb + u * KY;
-                    float v[VEC];
+                    float v[VEC], xv[MR];
                     sk_value<T, VEC>(raw[u], v);
+                    if constexpr (MR % 4 == 0) {
 #pragma unroll
-                    for (int m = 0; m < MR; ++m) {
-                        const float xv = k < kn ? xs[k * MR + m] : 0.0f;
+                        for (int m = 0; m < MR; m += 4)
+                            *reinterpret_cast<float4 *>(xv + m) = *reinterpret_cast<const float4 *>(xs + k * MR + m);
+                    } else {
 #pragma unroll
-                        for (int c = 0; c < VEC; ++c) acc[m][c] = fmaf(xv, v[c], acc[m][c]);
+                        for (int m = 0; m < MR; ++m) xv[m] = xs[k * MR + m];
                     }
+#pragma unroll
+                    for (int m = 0; m < MR; ++m)
+#pragma unroll
+                        for (int c = 0; c < VEC; ++c) acc[m][c] = fmaf(xv[m], v[c], acc[m][c]);
                 }
             }
         } else {
             constexpr int KP = LX * VEC;           // inner elements a warp's pass
-            constexpr int U = MR <= 2 ? 2 : 1;
             const T *p[kSkCols];
 #pragma unroll
             for (int c = 0; c < kSkCols; ++c) {
@@ -146,15 +170,20 @@ __device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int k = kb + u * kSkWarps * KP;
-                    if (k >= kn) break;
                     float v[kSkCols][VEC];
 #pragma unroll
                     for (int c = 0; c < kSkCols; ++c) sk_value<T, VEC>(raw[u][c], v[c]);
 #pragma unroll
                     for (int m = 0; m < MR; ++m) {
                         float xv[VEC];
+                        if constexpr (VEC % 4 == 0) {
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) xv[i] = xs[m * (kSkK + 8) + k + i];
+                            for (int i = 0; i < VEC; i += 4)
+                                *reinterpret_cast<float4 *>(xv + i) = *reinterpret_cast<const float4 *>(xs + m * (kSkK + 8) + k + i);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) xv[i] = xs[m * (kSkK + 8) + k + i];
+                        }
 #pragma unroll
                         for (int c = 0; c < kSkCols; ++c)
 #pragma unroll
@@ -222,6 +251,7 @@ product_skinny(const __grid_constant__ Product P, int splits) {
         if (nr == 1) sk_rows<T, COL, VEC, 1>(P, w, n0, row, nr, k0, k1, xs, red, bad);
         else if (MAXR == 2 || nr == 2) sk_rows<T, COL, VEC, 2>(P, w, n0, row, nr, k0, k1, xs, red, bad);
         else if (nr <= 4) sk_rows<T, COL, VEC, MAXR < 4 ? MAXR : 4>(P, w, n0, row, nr, k0, k1, xs, red, bad);
+        else if (MAXR <= 8 || nr <= 8) sk_rows<T, COL, VEC, MAXR < 8 ? MAXR : 8>(P, w, n0, row, nr, k0, k1, xs, red, bad);
         else sk_rows<T, COL, VEC, MAXR>(P, w, n0, row, nr, k0, k1, xs, red, bad);
         if (splits > 1) cluster.sync();
         else __syncthreads();
@@ -243,25 +273,42 @@ product_skinny(const __grid_constant__ Product P, int splits) {
 }
 
 // Few rows: one or two in bf16, where the tensor path is as fast from there
-// on; F32 up to 8 rows, or two a group, where
-// splitting W into planes for the tensor path costs more than its products.
+// on.  F32: the tensor path splits W into planes first, four times W's bytes,
+// and this one reads W once for each 16 rows of a group.  Measured, here
+// against there: 4096 x 4096, 17 rows 48 against 63 us and 32 rows 71 against
+// 64; 7296 x 6784, 17 rows 139 against 166 and 32 rows 204 against 167; 32
+// experts of 2048 x 1024, 8 rows each 119 against 228 and 24 rows each 252
+// against 233; 8 column-major experts of 1024 x 1001, 6 rows each 41 against
+// 40.  Fewer for groups than these show, because all rows may be in one.
 bool skinny_ok(const Product &P) {
     if (P.E > 65535 || P.K == 0) return false;
     if (P.dtype == JLB_BF16) return P.S <= 2;
-    return P.S <= (P.rowptr ? 2 * P.E : 8) && P.S <= 4096;
+    if (!P.rowptr) return P.S <= 24;
+    return P.S <= (P.w_order == JLB_ROW_MAJOR ? 8 : 4) * P.E && P.S <= 1024;
 }
 
 template <typename T, bool COL, int VEC, int MAXR>
 static int launch_skinny(cudaStream_t st, const Product &P) {
     using S = SkShape<T, COL, VEC>;
     const int64_t tiles = ceil_div(P.N, S::kTile);
-    // as many CTAs as are resident at once (4 an SM, 2 with 8 rows' sums), at
+    // as many CTAs as are resident at once (4 an SM, 2 with more rows' sums), at
     // least 128 inner elements each: 4096 x 4096 bf16 10.5 us, 8192 x 8192 28.4;
     // with half as many 11.6 and 37.2, with half as many again 10.5 and 37.1
     const int64_t live = tiles * (P.rowptr ? (P.E < P.S ? P.E : P.S) : 1);
     int64_t splits = (MAXR <= 2 ? 592 : 296) / (live > 0 ? live : 1);
     if (splits > P.K / 128) splits = P.K / 128;
     splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
+    if (MAXR > 2) {                                   // the fewest rounds a part's length, a part costs 3 %
+        const int64_t most = splits > 1 ? splits : P.K / 128 < 8 ? P.K / 128 : 8;
+        double best = 1e30;
+        for (int64_t q = 1; q <= most; ++q) {
+            const double cost = (double)ceil_div(live * q, 296) / q * (1.0 + 0.03 * q);
+            if (cost < best) {
+                best = cost;
+                splits = q;
+            }
+        }
+    }
     const size_t smem = (size_t)(MAXR * (kSkK + 8) + kSkWarps * MAXR * S::kTile) * 4;
     JLB_CUDA(cudaFuncSetAttribute(product_skinny<T, COL, VEC, MAXR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg{};
@@ -282,7 +329,12 @@ static int launch_skinny(cudaStream_t st, const Product &P) {
 
 template <typename T, bool COL, int VEC>
 static int skinny_rows(cudaStream_t st, const Product &P) {
-    return P.S <= 2 ? launch_skinny<T, COL, VEC, 2>(st, P) : launch_skinny<T, COL, VEC, 8>(st, P);
+    if (P.S <= 2) return launch_skinny<T, COL, VEC, 2>(st, P);
+    if constexpr (sizeof(T) == 4) {
+        if (P.S > (P.rowptr ? 4 * P.E : 8)) return launch_skinny<T, COL, VEC, 16>(st, P);
+        return launch_skinny<T, COL, VEC, 8>(st, P);
+    }
+    return fail(JLB_ERR_INVALID_ARGUMENT, "bf16 rows past two are the tensor path's");
 }
 
 template <typename T>
