@@ -3,9 +3,10 @@
 // costs, so the kernel is a stream over W with the rows' values beside it.
 //
 // A CTA takes one group and one tile of its columns; up to 8 rows at a time
-// (16 where F32 has more) sit in shared memory as fp32.  Row-major W: 8 lanes read 128 contiguous
-// bytes of one row of W, 32 rows of W a pass; a thread keeps sums[rows][8]
-// and each weight it loads meets every row.  Column-major W: 8 lanes read 128
+// (16 where F32 has more) sit in shared memory as fp32.  Row-major W: 8 lanes
+// read 128 contiguous bytes of one row of W, 32 rows of W a pass; a thread
+// keeps the sums of its 16 bytes of columns for all rows, and each weight it
+// loads meets every row.  Column-major W: 8 lanes read 128
 // bytes along K, a thread holds 4 columns.  The inner dimension is split over
 // the CTAs of a cluster when there are few tiles, and the parts are added
 // through distributed shared memory in rank order: one launch, no workspace,
@@ -83,7 +84,7 @@ __device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0
 #pragma unroll
         for (int c = 0; c < NS; ++c) acc[m][c] = 0.0f;
     // loads a thread has under way (column-major: times four)
-    constexpr int U = !COL ? MR <= 8 ? 8 : 4 : VEC == 1 ? 4 : MR <= 2 ? 2 : 1;
+    constexpr int U = !COL ? MR <= 8 ? 8 : 4 : VEC == 1 ? 4 : MR <= 4 ? 2 : 1;
     constexpr int kStep = U * (COL ? kSkWarps * LX * VEC : kSkThreads / LX);
     static_assert(kSkK % kStep == 0, "a staged part is a whole number of steps");
     int src[MR];                                   // the rows in x, -1: none
@@ -219,6 +220,43 @@ __device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0
     }
 }
 
+// The group of this CTA: the blockIdx.y-th of those with rows, or -1.  There
+// are as many grid rows as groups can have rows, so that a call of 2 rows over
+// 32 experts is not 16 times as many empty CTAs (2048 x 4096 bf16: 8.9
+// against 21 us).  One CTA looks at all the ranges and reports those that had
+// to be corrected.
+__device__ __forceinline__ int64_t sk_group(const Product &P, bool &bad) {
+    __shared__ int found, counts[kSkWarps];
+    const bool first = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    if (threadIdx.x == 0) found = -1;
+    int left = blockIdx.y;                            // groups with rows still to pass
+    bool done = false;
+    for (int64_t e0 = 0; e0 < P.E && (!done || first); e0 += kSkThreads) {
+        const int64_t e = e0 + threadIdx.x;
+        int lo = 0, hi = 0;
+        if (e < P.E) {
+            group_rows(P.rowptr, P.base, P.S, e, lo, hi);
+            if (first) bad |= group_bad(P.rowptr, P.base, P.S, e);
+        }
+        const unsigned mask = __ballot_sync(0xffffffffu, lo < hi);
+        __syncthreads();                              // the counts of the step before are read
+        if (lane == 0) counts[warp] = __popc(mask);
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int q = 0; q < kSkWarps; ++q) {
+            if (q < warp) before += counts[q];
+            all += counts[q];
+        }
+        if (!done && lo < hi && before + __popc(mask & ((1u << lane) - 1u)) == left) found = (int)e;
+        if (left < all) done = true;
+        else if (!done) left -= all;
+    }
+    __syncthreads();
+    return found;
+}
+
 // MAXR: rows taken at a time.
 template <typename T, bool COL, int VEC, int MAXR>
 __global__ void __launch_bounds__(kSkThreads, MAXR <= 2 ? 4 : 2)
@@ -228,14 +266,15 @@ product_skinny(const __grid_constant__ Product P, int splits) {
     extern __shared__ __align__(16) float sk_smem[];
     float *xs = sk_smem;                              // MAXR x (kSkK + 8)
     float *red = sk_smem + MAXR * (kSkK + 8);         // kSkWarps x MAXR x CT
-    const int64_t e = blockIdx.y, n0 = (int64_t)blockIdx.x * CT;
-    int lo, hi;
-    group_rows(P.rowptr, P.base, P.S, e, lo, hi);
-    bool bad = P.rowptr && group_bad(P.rowptr, P.base, P.S, e);
+    const int64_t n0 = (int64_t)blockIdx.x * CT;
+    bool bad = false;
+    const int64_t e = P.rowptr ? sk_group(P, bad) : 0;
+    int lo = 0, hi = 0;
+    if (e >= 0) group_rows(P.rowptr, P.base, P.S, e, lo, hi);
     if (P.rowptr && blockIdx.z == 0) {                // rows of no group are zero
         int a, end;
         group_rows(P.rowptr, P.base, P.S, P.E - 1, a, end);
-        for (int64_t r = (int64_t)end + e; r < P.S; r += P.E)
+        for (int64_t r = (int64_t)end + blockIdx.y; r < P.S; r += gridDim.y)
             for (int c = threadIdx.x; c < CT && n0 + c < P.N; c += kSkThreads) {
                 ((T *)P.y)[r * P.ldy + n0 + c] = from_f32<T>(0.0f);
                 if (P.z) ((T *)P.z)[r * P.ldz + n0 + c] = from_f32<T>(0.0f);
@@ -272,9 +311,14 @@ product_skinny(const __grid_constant__ Product P, int splits) {
     if (bad) dev_error(DEV_ERR_BOUNDS);
 }
 
-// Few rows: one or two in bf16, where the tensor path is as fast from there
-// on.  F32: the tensor path splits W into planes first, four times W's bytes,
-// and this one reads W once for each 16 rows of a group.  Measured, here
+// Few rows.  BF16: one or two; up to eight of a small W, four of row-major
+// experts, where the tensor path's start and second launch cost more than its
+// products save (here against there: 4 rows of 2048 x 2048 7.6 against 11.0 us,
+// of 8192 x 8192 45 against 31; 8 rows of 2049 x 1023 7.8 against 14.5; 4 rows
+// over 8 experts of 2048 x 1024 6.8 against 12.6, column-major ones up to
+// twice as long).
+// F32: the tensor path splits W into planes first, four times W's bytes, and
+// this one reads W once for each 16 rows of a group.  Measured, here
 // against there: 4096 x 4096, 17 rows 48 against 63 us and 32 rows 71 against
 // 64; 7296 x 6784, 17 rows 139 against 166 and 32 rows 204 against 167; 32
 // experts of 2048 x 1024, 8 rows each 119 against 228 and 24 rows each 252
@@ -282,7 +326,11 @@ product_skinny(const __grid_constant__ Product P, int splits) {
 // 40.  Fewer for groups than these show, because all rows may be in one.
 bool skinny_ok(const Product &P) {
     if (P.E > 65535 || P.K == 0) return false;
-    if (P.dtype == JLB_BF16) return P.S <= 2;
+    if (P.dtype == JLB_BF16) {
+        if (P.S <= 2) return true;
+        return P.rowptr ? P.S <= 4 && P.w_order == JLB_ROW_MAJOR
+                        : P.S <= 8 && P.K * P.N * P.S <= 1 << 25;
+    }
     if (!P.rowptr) return P.S <= 24;
     return P.S <= (P.w_order == JLB_ROW_MAJOR ? 8 : 4) * P.E && P.S <= 1024;
 }
@@ -291,22 +339,20 @@ template <typename T, bool COL, int VEC, int MAXR>
 static int launch_skinny(cudaStream_t st, const Product &P) {
     using S = SkShape<T, COL, VEC>;
     const int64_t tiles = ceil_div(P.N, S::kTile);
-    // as many CTAs as are resident at once (4 an SM, 2 with more rows' sums), at
-    // least 128 inner elements each: 4096 x 4096 bf16 10.5 us, 8192 x 8192 28.4;
-    // with half as many 11.6 and 37.2, with half as many again 10.5 and 37.1
-    const int64_t live = tiles * (P.rowptr ? (P.E < P.S ? P.E : P.S) : 1);
-    int64_t splits = (MAXR <= 2 ? 592 : 296) / (live > 0 ? live : 1);
-    if (splits > P.K / 128) splits = P.K / 128;
-    splits = splits < 1 ? 1 : splits > 8 ? 8 : splits;
-    if (MAXR > 2) {                                   // the fewest rounds a part's length, a part costs 3 %
-        const int64_t most = splits > 1 ? splits : P.K / 128 < 8 ? P.K / 128 : 8;
-        double best = 1e30;
-        for (int64_t q = 1; q <= most; ++q) {
-            const double cost = (double)ceil_div(live * q, 296) / q * (1.0 + 0.03 * q);
-            if (cost < best) {
-                best = cost;
-                splits = q;
-            }
+    const int64_t groups = P.rowptr && P.S < P.E ? P.S : P.E;       // that can have rows
+    const int64_t live = tiles * groups;
+    // Parts of the inner dimension, 1 to 8: the fewest rounds of resident CTAs
+    // (4 an SM, 2 with more rows' sums) for a part's length, each part at least
+    // 128 long and 3 % of overhead.  A power of two: clusters of 3 or 6 CTAs
+    // took twice as long (3 rows over 8 experts of 1024 x 1001 bf16 13.2 us,
+    // 4 rows 5.0).
+    int64_t splits = 1;
+    double best = 1e30;
+    for (int64_t q = 1; q <= 8 && (q == 1 || q <= P.K / 128); q *= 2) {
+        const double cost = (double)ceil_div(live * q, MAXR <= 2 ? 592 : 296) / q * (1.0 + 0.03 * q);
+        if (cost < best) {
+            best = cost;
+            splits = q;
         }
     }
     const size_t smem = (size_t)(MAXR * (kSkK + 8) + kSkWarps * MAXR * S::kTile) * 4;
@@ -317,7 +363,7 @@ static int launch_skinny(cudaStream_t st, const Product &P) {
     at[0].val.clusterDim.x = 1;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = (unsigned)splits;
-    cfg.gridDim = dim3((unsigned)tiles, (unsigned)P.E, (unsigned)splits);
+    cfg.gridDim = dim3((unsigned)tiles, (unsigned)groups, (unsigned)splits);
     cfg.blockDim = dim3(kSkThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -330,11 +376,10 @@ static int launch_skinny(cudaStream_t st, const Product &P) {
 template <typename T, bool COL, int VEC>
 static int skinny_rows(cudaStream_t st, const Product &P) {
     if (P.S <= 2) return launch_skinny<T, COL, VEC, 2>(st, P);
-    if constexpr (sizeof(T) == 4) {
+    if (sizeof(T) == 2 && P.S <= 4) return launch_skinny<T, COL, VEC, 4>(st, P);
+    if constexpr (sizeof(T) == 4)
         if (P.S > (P.rowptr ? 4 * P.E : 8)) return launch_skinny<T, COL, VEC, 16>(st, P);
-        return launch_skinny<T, COL, VEC, 8>(st, P);
-    }
-    return fail(JLB_ERR_INVALID_ARGUMENT, "bf16 rows past two are the tensor path's");
+    return launch_skinny<T, COL, VEC, 8>(st, P);
 }
 
 template <typename T>

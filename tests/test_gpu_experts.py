@@ -130,6 +130,30 @@ def test_combine(dtype, T, k, N, drop, base, weighted):
     R.check(dg, rg, bg * (N + 2) * R.SUM_ULP, F32, "dg")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [1, 40, 129, 1024, 4104])
+def test_combine_entries_a_token(dtype, N):
+    T, E = 70, 20
+    for k in (1, 2, 3, 4, 5, 6, 8, 9):
+        ids = random_ids(T, k, E, k, 0.1)
+        r = J.route(torch.from_numpy(ids).to(DEV), E)
+        z, g, dy = randn((T * k, N), dtype, 1), randn((T, k), F32, 2), randn((T, N), dtype, 4)
+        y = J.combine(z, r, g)
+        dz, dg = J.combine_backward(dy, z, r, g)
+        J.device_status()
+        slot = r.slot.cpu().numpy().astype(np.int64)
+        live = slot >= 0
+        rows = np.where(live[..., None], R.f64(z)[np.maximum(slot, 0)], 0.0)      # T x k x N
+        g64, dy64 = R.f64(g), R.f64(dy)
+        rz = np.zeros((T * k, N))
+        rz[slot[live]] = (g64[..., None] * dy64[:, None])[live]
+        R.check(y, np.einsum("tk,tkn->tn", g64, rows),
+                np.einsum("tk,tkn->tn", np.abs(g64), np.abs(rows)) * (k + 2) * R.SUM_ULP, dtype, "y")
+        R.check(dz, rz, np.abs(rz) * R.SUM_ULP, dtype, "dz")
+        R.check(dg, np.einsum("tn,tkn->tk", dy64, rows),
+                np.einsum("tn,tkn->tk", np.abs(dy64), np.abs(rows)) * (N + 2) * R.SUM_ULP, F32, "dg")
+
+
 def test_combine_strided_and_in_place_buffers():
     T, k, N, E = 50, 3, 72, 6
     r = J.route(torch.from_numpy(random_ids(T, k, E, 8)).to(DEV), E)
@@ -314,6 +338,45 @@ def test_strides_and_misaligned_buffers(dtype, M):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["row", "col"])
+@pytest.mark.parametrize("K,N", [(96, 136), (97, 133)])
+@pytest.mark.parametrize("sizes", [{255: 1}, {0: 1, 256: 2}, {3: 1, 511: 1, 512: 1, 699: 1}, {699: 4},
+                                   {0: 9, 300: 18, 640: 1}])
+def test_few_rows_among_many_experts(dtype, order, K, N, sizes):
+    """The other experts' weights (NaN here) are not used."""
+    E = 700
+    n = np.zeros(E, np.int64)
+    for e, c in sizes.items():
+        n[e] = c
+    S, ptr = int(n.sum()) + 1, pointers(n)
+    x, b = randn((S, K), dtype, 1), randn((E, N), dtype, 3)
+    w = torch.full((E, K, N) if order == "row" else (E, N, K), float("nan"), dtype=dtype, device=DEV)
+    w = w if order == "row" else w.transpose(1, 2)
+    for e in sizes:
+        w[e] = randn((K, N), dtype, 10 + e, K ** -0.5)
+    y = J.grouped_matmul(x, w, dev_i32(ptr), bias=b, act="silu")
+    J.device_status()
+    ry, _, by, _ = R.forward(R.f64(x), np.nan_to_num(R.f64(w)), ptr, None, R.f64(b), "silu")
+    ry[ptr[-1]:] = 0
+    R.check(y, ry, by, dtype, "y")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["row", "col"])
+@pytest.mark.parametrize("K,N", [(1024, 264), (1537, 129), (70, 40)])
+def test_fused_few_rows(dtype, order, K, N):
+    w, b = weights(1, K, N, dtype, order, 2)[0], randn((N,), dtype, 3)
+    for M in (1, 2, 3, 4, 5, 8, 9, 16, 17, 24, 25):
+        x, res = randn((M, K), dtype, M), randn((M, N), dtype, 5)
+        y, z = J.fused_matmul(x, w, bias=b, act="gelu", residual=res, keep_preact=True)
+        J.device_status()
+        ry, rz, by, bz = R.forward(R.f64(x), R.f64(w)[None], np.array([0, M]), None, R.f64(b)[None],
+                                   "gelu", R.f64(res))
+        R.check(z, rz, bz, dtype, "z")
+        R.check(y, ry, by, dtype, "y")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("sizes", [[3, 2], [40, 70, 33], [300, 0, 290]])
 def test_bad_values_stay_in_their_rows_and_groups(dtype, sizes):
     """An infinity or NaN in one row reaches that row alone, and a group's dw
@@ -361,6 +424,19 @@ def test_row_indices_outside_x_are_reported():
 def test_row_ranges_outside_the_rows_are_reported():
     x, w = randn((6, 64), BF, 1), weights(3, 64, 72, BF, "row", 2)
     J.grouped_matmul(x, w, dev_i32([0, 4, 2, 9]))
+    with pytest.raises(J.NonCanonicalStorage):
+        J.device_status()
+    J.device_status()
+
+
+def test_row_ranges_of_late_experts_are_reported():
+    x, w = randn((3, 64), F32, 1), weights(400, 64, 72, F32, "row", 2)
+    ptr = np.zeros(401, np.int64)
+    ptr[350:] = 2
+    J.grouped_matmul(x, w, dev_i32(ptr))
+    J.device_status()
+    ptr[390] = 1                                   # a range that runs backwards
+    J.grouped_matmul(x, w, dev_i32(ptr))
     with pytest.raises(J.NonCanonicalStorage):
         J.device_status()
     J.device_status()
