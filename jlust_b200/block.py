@@ -23,6 +23,8 @@ out of the assembled CSR and added by the patched SpMV kernel.
 """
 from __future__ import annotations
 
+import gc
+
 import numpy as np
 import torch
 
@@ -119,8 +121,16 @@ class _Graphed:
             self.spmv(x, y)          # first use outside the graph, then capture
             torch.cuda.current_stream(y.device).synchronize()
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
-                self.spmv(x, y)
+            # no cyclic collection meanwhile: one that frees another graph
+            # resets it, which invalidates the capture
+            collects = gc.isenabled()
+            gc.disable()
+            try:
+                with torch.cuda.graph(g):
+                    self.spmv(x, y)
+            finally:
+                if collects:
+                    gc.enable()
             self.graphs[key] = g
         g.replay()
 

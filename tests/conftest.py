@@ -1,4 +1,5 @@
 """Shared test set-up: the `gpu` marker, import paths and built libraries."""
+import gc
 import os
 import sys
 
@@ -20,6 +21,21 @@ def _built_libraries():
     b.build()
     from oracle import oracle as O
     O.build()
+    yield
+
+
+def pytest_collection_finish(session):
+    # what the imports made stays; later collections look at the tests' own
+    gc.collect()
+    gc.freeze()
+
+
+@pytest.fixture(autouse=True)
+def _no_garbage(request):
+    """Graphs that earlier tests left in cycles are freed before a test, not by
+    a collection in the middle of its capture, which that would invalidate."""
+    if request.node.get_closest_marker("gpu"):
+        gc.collect()
     yield
 
 
