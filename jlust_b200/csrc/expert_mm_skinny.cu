@@ -2,15 +2,15 @@
 // (decode steps, single tokens): the weights are read once and nothing else
 // costs, so the kernel is a stream over W with the rows' values beside it.
 //
-// A CTA takes one group and one tile of its columns; up to 8 rows at a time
-// (16 where F32 has more) sit in shared memory as fp32.  Row-major W: 8 lanes
+// A CTA takes a run of up to 8 rows of one group (16 where F32 has more) and one
+// tile of columns; the rows sit in shared memory as fp32.  Row-major W: 8 lanes
 // read 128 contiguous bytes of one row of W, 32 rows of W a pass; a thread
 // keeps the sums of its 16 bytes of columns for all rows, and each weight it
-// loads meets every row.  Column-major W: 8 lanes read 128
-// bytes along K, a thread holds 4 columns.  The inner dimension is split over
-// the CTAs of a cluster when there are few tiles, and the parts are added
-// through distributed shared memory in rank order: one launch, no workspace,
-// the same order on every run.  Unaligned W is read one element a lane.
+// loads meets every row.  Column-major W: 8 lanes read 128 bytes along K, a
+// thread holds 4 columns.  The inner dimension is split over the CTAs of a
+// cluster when there are few tiles, and the parts are added through
+// distributed shared memory in rank order: one launch, no workspace, the same
+// order on every run.  Unaligned W is read one element a lane.
 //
 // Bound: HBM (L2 for repeated weights).  Sums are fp32 FMAs, one rounding to
 // the value type.
@@ -220,41 +220,55 @@ __device__ __forceinline__ void sk_rows(const Product &P, const T *w, int64_t n0
     }
 }
 
-// The group of this CTA: the blockIdx.y-th of those with rows, or -1.  There
-// are as many grid rows as groups can have rows, so that a call of 2 rows over
-// 32 experts is not 16 times as many empty CTAs (2048 x 4096 bf16: 8.9
-// against 21 us).  One CTA looks at all the ranges and reports those that had
-// to be corrected.
-__device__ __forceinline__ int64_t sk_group(const Product &P, bool &bad) {
-    __shared__ int found, counts[kSkWarps];
+// The rows of this CTA: the blockIdx.x-th run of up to MAXR rows, counted over
+// the groups in order; false when there are fewer.  A call of 2 rows over 32
+// experts launches two runs and not 32 groups (2048 x 4096 bf16: 8.9 against 21
+// us), and a group with many rows has them side by side.  One CTA looks at all
+// the ranges and reports those that had to be corrected.
+template <int MAXR>
+__device__ __forceinline__ bool sk_run(const Product &P, int64_t &e, int &row, int &nrows, bool &bad) {
+    __shared__ int found, counts[kSkWarps], its_row, its_rows;
     const bool first = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
     const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
     if (threadIdx.x == 0) found = -1;
-    int left = blockIdx.y;                            // groups with rows still to pass
+    int left = blockIdx.x;                            // runs still to pass
     bool done = false;
     for (int64_t e0 = 0; e0 < P.E && (!done || first); e0 += kSkThreads) {
-        const int64_t e = e0 + threadIdx.x;
+        const int64_t g = e0 + threadIdx.x;
         int lo = 0, hi = 0;
-        if (e < P.E) {
-            group_rows(P.rowptr, P.base, P.S, e, lo, hi);
-            if (first) bad |= group_bad(P.rowptr, P.base, P.S, e);
+        if (g < P.E) {
+            group_rows(P.rowptr, P.base, P.S, g, lo, hi);
+            if (first) bad |= group_bad(P.rowptr, P.base, P.S, g);
         }
-        const unsigned mask = __ballot_sync(0xffffffffu, lo < hi);
+        const int runs = (hi - lo + MAXR - 1) / MAXR;
+        int upto = runs;                              // of this warp's groups, this one's with them
+#pragma unroll
+        for (int o = 1; o < kWarp; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
         __syncthreads();                              // the counts of the step before are read
-        if (lane == 0) counts[warp] = __popc(mask);
+        if (lane == kWarp - 1) counts[warp] = upto;
         __syncthreads();
-        int before = 0, all = 0;
+        int before = upto - runs, all = 0;
 #pragma unroll
         for (int q = 0; q < kSkWarps; ++q) {
             if (q < warp) before += counts[q];
             all += counts[q];
         }
-        if (!done && lo < hi && before + __popc(mask & ((1u << lane) - 1u)) == left) found = (int)e;
+        if (!done && left >= before && left < before + runs) {
+            found = (int)g;
+            its_row = lo + (left - before) * MAXR;
+            its_rows = min(MAXR, hi - its_row);
+        }
         if (left < all) done = true;
         else if (!done) left -= all;
     }
     __syncthreads();
-    return found;
+    e = found;
+    row = its_row;
+    nrows = its_rows;
+    return found >= 0;
 }
 
 // MAXR: rows taken at a time.
@@ -266,15 +280,15 @@ product_skinny(const __grid_constant__ Product P, int splits) {
     extern __shared__ __align__(16) float sk_smem[];
     float *xs = sk_smem;                              // MAXR x (kSkK + 8)
     float *red = sk_smem + MAXR * (kSkK + 8);         // kSkWarps x MAXR x CT
-    const int64_t n0 = (int64_t)blockIdx.x * CT;
+    const int64_t n0 = (int64_t)blockIdx.y * CT;
     bool bad = false;
-    const int64_t e = P.rowptr ? sk_group(P, bad) : 0;
-    int lo = 0, hi = 0;
-    if (e >= 0) group_rows(P.rowptr, P.base, P.S, e, lo, hi);
+    int64_t e = 0;
+    int row = blockIdx.x * MAXR, nr = (int)min((int64_t)MAXR, P.S - row);
+    const bool live = P.rowptr ? sk_run<MAXR>(P, e, row, nr, bad) : true;
     if (P.rowptr && blockIdx.z == 0) {                // rows of no group are zero
         int a, end;
         group_rows(P.rowptr, P.base, P.S, P.E - 1, a, end);
-        for (int64_t r = (int64_t)end + blockIdx.y; r < P.S; r += gridDim.y)
+        for (int64_t r = (int64_t)end + blockIdx.x; r < P.S; r += gridDim.x)
             for (int c = threadIdx.x; c < CT && n0 + c < P.N; c += kSkThreads) {
                 ((T *)P.y)[r * P.ldy + n0 + c] = from_f32<T>(0.0f);
                 if (P.z) ((T *)P.z)[r * P.ldz + n0 + c] = from_f32<T>(0.0f);
@@ -285,8 +299,7 @@ product_skinny(const __grid_constant__ Product P, int splits) {
     const int64_t k0 = min(P.K, share * blockIdx.z), k1 = min(P.K, k0 + share);
     const T *w = (const T *)P.w + e * P.w_stride;
     cg::cluster_group cluster = cg::this_cluster();
-    for (int row = lo; row < hi; row += MAXR) {
-        const int nr = min(MAXR, hi - row);
+    if (live) {                                       // the same for a cluster's CTAs
         if (nr == 1) sk_rows<T, COL, VEC, 1>(P, w, n0, row, nr, k0, k1, xs, red, bad);
         else if (MAXR == 2 || nr == 2) sk_rows<T, COL, VEC, 2>(P, w, n0, row, nr, k0, k1, xs, red, bad);
         else if (nr <= 4) sk_rows<T, COL, VEC, MAXR < 4 ? MAXR : 4>(P, w, n0, row, nr, k0, k1, xs, red, bad);
@@ -311,45 +324,51 @@ product_skinny(const __grid_constant__ Product P, int splits) {
     if (bad) dev_error(DEV_ERR_BOUNDS);
 }
 
-// Few rows.  BF16: one or two; up to eight of a small W, four of row-major
-// experts, where the tensor path's start and second launch cost more than its
-// products save (here against there: 4 rows of 2048 x 2048 7.6 against 11.0 us,
-// of 8192 x 8192 45 against 31; 8 rows of 2049 x 1023 7.8 against 14.5; 4 rows
-// over 8 experts of 2048 x 1024 6.8 against 12.6, column-major ones up to
-// twice as long).
+// Few rows, measured here against the tensor path.  BF16: one or two; up to
+// eight over experts, where the tensor path starts slowly and joins its parts
+// in a second launch (8 rows over 8 experts of 2048 x 1024 9.5 against 14.5 us,
+// over 32 of 2048 x 4096 33 against 31, over 69 unaligned ones of 512 x 4093 27
+// against 52); more for a small W (16 rows over 64 experts of 512 x 1024 6.7
+// against 12.9; 4 dense rows of 2048 x 2048 7.5 against 11, 8 of 2049 x 1023
+// 7.8 against 14.5, but 4 of 8192 x 8192 45 against 31).
 // F32: the tensor path splits W into planes first, four times W's bytes, and
-// this one reads W once for each 16 rows of a group.  Measured, here
-// against there: 4096 x 4096, 17 rows 48 against 63 us and 32 rows 71 against
-// 64; 7296 x 6784, 17 rows 139 against 166 and 32 rows 204 against 167; 32
-// experts of 2048 x 1024, 8 rows each 119 against 228 and 24 rows each 252
-// against 233; 8 column-major experts of 1024 x 1001, 6 rows each 41 against
-// 40.  Fewer for groups than these show, because all rows may be in one.
+// this one reads W once for each 16 rows of a group: 4096 x 4096, 16 rows 37
+// against 63 us, 17 rows 59 and 32 rows 71 against 64; 7296 x 6784, 17 rows 125
+// against 166 and 32 rows 204 against 167; 32 experts of 2048 x 1024, 8 rows
+// each 105 and 12 rows each 128 against 230; 8 column-major ones of 1024 x 1001,
+// 12 rows each 27 against 40.  1024 rows of one expert out of 128, 512 x 1024,
+// take 88 us, 128 rows of one out of 32, 4096 x 4096, 230.
 bool skinny_ok(const Product &P) {
-    if (P.E > 65535 || P.K == 0) return false;
+    if (P.N > 65535 * 8 || P.K == 0 || P.E == 0) return false;    // a tile is 8 columns or more
     if (P.dtype == JLB_BF16) {
         if (P.S <= 2) return true;
-        return P.rowptr ? P.S <= 4 && P.w_order == JLB_ROW_MAJOR
-                        : P.S <= 8 && P.K * P.N * P.S <= 1 << 25;
+        return P.S <= (P.rowptr ? 16 : 8) && ((P.rowptr && P.S <= 8) || P.K * P.N * P.S <= 1 << 25);
     }
     if (!P.rowptr) return P.S <= 24;
-    return P.S <= (P.w_order == JLB_ROW_MAJOR ? 8 : 4) * P.E && P.S <= 1024;
+    return P.S <= 16 * P.E && P.S <= 1024;
 }
 
 template <typename T, bool COL, int VEC, int MAXR>
 static int launch_skinny(cudaStream_t st, const Product &P) {
     using S = SkShape<T, COL, VEC>;
     const int64_t tiles = ceil_div(P.N, S::kTile);
-    const int64_t groups = P.rowptr && P.S < P.E ? P.S : P.E;       // that can have rows
-    const int64_t live = tiles * groups;
+    // runs of rows that the groups can have, at most
+    const int64_t most = P.rowptr ? P.E + P.S / MAXR : ceil_div(P.S, MAXR), runs = most < P.S ? most : P.S;
+    const int64_t live = tiles * (P.rowptr && P.E < runs ? P.E : runs);
     // Parts of the inner dimension, 1 to 8: the fewest rounds of resident CTAs
     // (4 an SM, 2 with more rows' sums) for a part's length, each part at least
     // 128 long and 3 % of overhead.  A power of two: clusters of 3 or 6 CTAs
     // took twice as long (3 rows over 8 experts of 1024 x 1001 bf16 13.2 us,
-    // 4 rows 5.0).
+    // 4 rows 5.0).  Groups' parts have to be resident at once: among runs that
+    // turn out empty, clusters in several rounds took two to three times as long
+    // (8 F32 experts of 1024 x 1001, one row each, 24 against 8.6 us); a dense
+    // product gains by them (3 F32 rows of 7296 x 6784 column-major 64 against 83).
+    const int64_t slots = MAXR <= 2 ? 592 : 296;
     int64_t splits = 1;
     double best = 1e30;
     for (int64_t q = 1; q <= 8 && (q == 1 || q <= P.K / 128); q *= 2) {
-        const double cost = (double)ceil_div(live * q, MAXR <= 2 ? 592 : 296) / q * (1.0 + 0.03 * q);
+        if (P.rowptr && q > 1 && live * q > slots) break;
+        const double cost = (double)ceil_div(live * q, slots) / q * (1.0 + 0.03 * q);
         if (cost < best) {
             best = cost;
             splits = q;
@@ -363,7 +382,7 @@ static int launch_skinny(cudaStream_t st, const Product &P) {
     at[0].val.clusterDim.x = 1;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = (unsigned)splits;
-    cfg.gridDim = dim3((unsigned)tiles, (unsigned)groups, (unsigned)splits);
+    cfg.gridDim = dim3((unsigned)runs, (unsigned)tiles, (unsigned)splits);
     cfg.blockDim = dim3(kSkThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -376,9 +395,11 @@ static int launch_skinny(cudaStream_t st, const Product &P) {
 template <typename T, bool COL, int VEC>
 static int skinny_rows(cudaStream_t st, const Product &P) {
     if (P.S <= 2) return launch_skinny<T, COL, VEC, 2>(st, P);
-    if (sizeof(T) == 2 && P.S <= 4) return launch_skinny<T, COL, VEC, 4>(st, P);
-    if constexpr (sizeof(T) == 4)
+    if constexpr (sizeof(T) == 2) {
+        if (P.S <= 4) return launch_skinny<T, COL, VEC, 4>(st, P);
+    } else {
         if (P.S > (P.rowptr ? 4 * P.E : 8)) return launch_skinny<T, COL, VEC, 16>(st, P);
+    }
     return launch_skinny<T, COL, VEC, 8>(st, P);
 }
 
