@@ -212,7 +212,9 @@ __global__ void __launch_bounds__(kSimtThreads) gradient_simt(const Gradient G) 
 // one where the layout is not aligned) x 8 row lanes, four rows' loads on
 // their way at a time.  Sums of unrounded products in fp32: a lane's rows,
 // then the 8 lanes in order; sum_parts adds a group's CTAs in order.  Bound by
-// HBM.
+// HBM.  Row ranges that overlap (rowptr running backwards) have more tiles than
+// rows allow: the ones past the grid are left out, in sum_parts too, and
+// reported.
 constexpr int kSumRows = 128;
 template <typename T, int V>
 struct Values {                    // as they lie in memory, until they are used
@@ -280,6 +282,9 @@ act_backward(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restric
     __shared__ Found f;
     __shared__ float red[8][32 * V];
     find_row_tile(rowptr, base, S, E, kSumRows, blockIdx.y, &f);
+    if (blockIdx.x == 0)
+        for (int64_t e = (int64_t)blockIdx.y * 256 + threadIdx.x; e < E; e += (int64_t)gridDim.y * 256)
+            if (group_bad(rowptr, base, S, e)) dev_error(DEV_ERR_BOUNDS);
     __syncthreads();
     if (f.e < 0) return;
     const int cx = threadIdx.x % 32;
@@ -310,10 +315,11 @@ act_backward(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restric
     }
 }
 
+// part holds `parts` rows of N.
 template <typename T>
 __global__ void __launch_bounds__(256)
 sum_parts(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__ rowptr,
-          const float *__restrict__ part, T *__restrict__ db, int64_t lddb) {
+          const float *__restrict__ part, int64_t parts, T *__restrict__ db, int64_t lddb) {
     const int64_t e = blockIdx.y;
     __shared__ int64_t first_s;
     __shared__ int count_s;
@@ -329,8 +335,9 @@ sum_parts(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__
         if (threadIdx.x == 0) {
             int lo, hi;
             group_rows(rowptr, base, S, e, lo, hi);
+            const int64_t left = parts > first ? parts - first : 0, count = ceil_div(hi - lo, kSumRows);
             first_s = first;
-            count_s = (int)ceil_div(hi - lo, kSumRows);
+            count_s = (int)(count < left ? count : left);
         }
     }
     __syncthreads();
@@ -950,10 +957,10 @@ extern "C" JLB_API int jlb_act_backward(void *stream, int dtype, int idx_base, i
     if (db) {
         const dim3 grid((unsigned)ceil_div(N, 256), (unsigned)E);
         if (dtype == JLB_F32)
-            emm::sum_parts<float><<<grid, 256, 0, st>>>(E, S, N, idx_base, rowptr, part,
+            emm::sum_parts<float><<<grid, 256, 0, st>>>(E, S, N, idx_base, rowptr, part, tiles,
                                                         (float *)db, lddb);
         else
-            emm::sum_parts<__nv_bfloat16><<<grid, 256, 0, st>>>(E, S, N, idx_base, rowptr, part,
+            emm::sum_parts<__nv_bfloat16><<<grid, 256, 0, st>>>(E, S, N, idx_base, rowptr, part, tiles,
                                                                 (__nv_bfloat16 *)db, lddb);
         JLB_LAUNCH_CHECK("sum_parts");
     }

@@ -1,0 +1,63 @@
+"""Expert-layer operators at the edges of their contracts: row ranges that
+overlap, tails of the activations, extents past a launch's limits, and what
+has to be waited for before a kernel ends."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import jlust_b200 as J
+import _experts_ref as R
+from _helpers import DEV
+from jlust_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+TYPES = [pytest.param(BF, id="bf16"), pytest.param(F32, id="f32")]
+
+
+def randn(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def dev_i32(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(torch.int32).to(DEV)
+
+
+# ------------------------------------------------- row ranges that overlap
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [40, 41])
+def test_bias_sums_of_overlapping_ranges_stay_in_their_workspace(dtype, N):
+    """rowptr [0, S, 0, S, ...] gives every second group all rows: more row
+    tiles than the workspace has parts.  Past its bytes lies NaN, which no sum
+    may read; the first group's sums are those of its rows."""
+    L, S, E = _lib.load(), 1000, 9
+    dy, ptr = randn((S, N), dtype, 1), dev_i32([0, S] * 5)
+    wsb = L.jlb_act_backward_workspace_size(E, S, N, 1)
+    ws = torch.full((wsb // 4 + 64 * N,), float("nan"), device=DEV)
+    db = torch.full((E, N), float("nan"), dtype=dtype, device=DEV)
+    st = L.jlb_act_backward(torch.cuda.current_stream().cuda_stream, 0 if dtype == F32 else 2, 0, E, S, N,
+                            ptr.data_ptr(), 0, dy.data_ptr(), N, None, 0, None, 0, db.data_ptr(), N,
+                            ws.data_ptr(), wsb)
+    assert st == 0
+    with pytest.raises(J.NonCanonicalStorage):
+        J.device_status()
+    J.device_status()
+    assert db.isfinite().all() and not db[1].any()
+    dy64 = R.f64(dy)
+    R.check(db[0], dy64.sum(0), (S + 8) * R.SUM_ULP * np.abs(dy64).sum(0), dtype, "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ptr", [[0, 300, 0, 300], [0, 40, 20, 300], [5, 60, 400, 200], [0, 100, 200, -7]])
+def test_gradients_report_bad_ranges(dtype, ptr):
+    E, S, K, N = len(ptr) - 1, 300, 72, 136
+    x, w, z, dy = randn((S, K), dtype, 1), randn((E, K, N), dtype, 2), randn((S, N), dtype, 3), randn((S, N), dtype, 4)
+    for act in (None, "silu"):
+        J.grouped_matmul_backward(dy, x, w, dev_i32(ptr), z=z, act=act, bias=True)
+        with pytest.raises(J.NonCanonicalStorage):
+            J.device_status()
+        J.device_status()
