@@ -514,8 +514,10 @@ JLB_API int jlb_combine_backward(void *stream, int dtype, int idx_base, int64_t 
  * A row index outside x counts as a row of zeros, and row ranges that are not
  * ascending inside [0, S] are cut to it; both are reported by
  * jlb_device_status().  Where ranges overlap, the values of their rows and
- * groups are unspecified; nothing outside the buffers is touched.  `workspace` holds the bytes the size query returns
- * for the same operands (0: none needed).  Asynchronous.
+ * groups are unspecified; nothing outside the buffers is touched.
+ *
+ * `workspace` holds the bytes the size query returns for the same operands
+ * (0: none needed).  Asynchronous.
  *
  * A plan keeps the weight's side of the call (the buffers stay the caller's
  * and must outlive it; their values may change between calls). */

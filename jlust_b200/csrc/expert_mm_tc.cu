@@ -630,6 +630,11 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                     }
                 }
             }
+            // both accumulators' last releases have arrived: the other CTA's
+            // epilogue sends none to a CTA that is gone
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+                ok = ok && tc_wait_warp(smem_u32(&ctl->tempty[b]), te[b], abort_flag);
             __syncwarp();
             commit_pair(smem_u32(&ctl->done));
         }
@@ -778,6 +783,12 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
             }
             if (++tk == kTickets) { tk = 0; tph ^= 1u; }
         }
+        // the other CTA's reports of the last tickets have arrived
+        if (rank == 0 && P.counter)
+            for (int b = 0; b < kTickets; ++b) {
+                if (!tc_wait_warp(smem_u32(&ctl->tack[tk]), tph ^ 1u, abort_flag)) break;
+                if (++tk == kTickets) { tk = 0; tph ^= 1u; }
+            }
     } else if (warp < kLoadWarp + kLoaders / 32) {
         // ------------------------------------------------------ loader warps
         // Loader warp w of the CTA copies rows w*4 + 16*n + lane/8 of a stage,
@@ -909,7 +920,13 @@ product_tc(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUten
                 tc_drain(smem_u32(&ctl->full[s]), ((ctl->fills - 1 - s) / (uint32_t)P.stages) & 1u);
     }
     __syncthreads();
-    cluster_sync_relaxed();               // neither CTA's shared memory goes before the other is done
+    // neither CTA's shared memory goes before the other is done.  Arrivals on
+    // the other CTA's barriers have been waited for there (empty, tfull and done
+    // of commits; full, tempty and tack on the leader; tbar), unless a wait
+    // gave up: the role at the other end then gives up too, and its CTA's barrier
+    // is one that its arrivals come before.
+    if (ctl->abort) cluster_sync_released();
+    else cluster_sync_relaxed();
     if (warp == 1) {
         fence_after();
         dealloc_pair(tmem, 512);

@@ -22,6 +22,11 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// A cluster barrier before which every operation of this CTA is performed, its
+// arrivals on the other CTA's barriers among them.
+__device__ __forceinline__ void cluster_sync_released() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // A cluster barrier that orders no memory of its own: callers publish nothing
 // by it but what they have fenced (a releasing one waits for every store of
 // the epilogue, about 1 us at a kernel's end).
@@ -92,7 +97,8 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const void *map, uint32_t b
         "@e cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
-}__device__ __forceinline__ void tma_4d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z, int w) {
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z, int w) {
     asm volatile(
         "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
         "@e cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"

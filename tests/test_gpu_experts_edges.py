@@ -61,3 +61,23 @@ def test_gradients_report_bad_ranges(dtype, ptr):
         with pytest.raises(J.NonCanonicalStorage):
             J.device_status()
         J.device_status()
+
+
+# --------------------------------------- what a launch waits for at its end
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_products_back_to_back_with_few_and_many_tiles_a_pair(dtype):
+    """One, two, three and more tiles a CTA pair (each accumulator's last use
+    odd or even), empty groups, and tiles drawn from the counter with fewer and
+    more tickets than places: a launch that waited for an arrival that does not
+    come would report a timeout, and the next ones repeat its results."""
+    K, N = 128, 512
+    for sizes in ([300], [0, 40], [300] * 40, [0, 900, 33] * 50, [1] * 80, [256] * 300):
+        ptr, E, S = dev_i32(np.concatenate([[0], np.cumsum(sizes)])), len(sizes), sum(sizes)
+        x, w, dy = randn((S, K), dtype, 1), randn((E, K, N), dtype, 2), randn((S, N), dtype, 3)
+        first = None
+        for _ in range(20):
+            got = (J.grouped_matmul(x, w, ptr), *J.grouped_matmul_backward(dy, x, w, ptr)[:2])
+            first = first or got
+        J.device_status()
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
