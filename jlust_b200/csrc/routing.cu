@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kThreads) route_count(const int32_t *__restric
 // by expert (E x chunks; scans_counts).
 __global__ void __launch_bounds__(kThreads)
 route_place(const int32_t *__restrict__ ids, int64_t n, int k, int base, int E,
-            const int32_t *__restrict__ hist, const int32_t *__restrict__ at, int chunks,
+            const int32_t *hist, const int32_t *__restrict__ at, int chunks,
             int32_t *__restrict__ rowptr, int32_t *__restrict__ source, int32_t *__restrict__ slot) {
     extern __shared__ int32_t sm[];
     int32_t *tot = sm;                        // E: entries per expert, then their exclusive scan
@@ -137,7 +137,8 @@ route_place(const int32_t *__restrict__ ids, int64_t n, int k, int base, int E,
             int all = 0, before = 0;
 #pragma unroll 8
             for (int c = p; c < chunks; c += per) {
-                const int h = __ldg(hist + (int64_t)c * E + e);
+                // coherent: route_count writes them while this grid runs
+                const int h = __ldcg(hist + (int64_t)c * E + e);
                 if (c < (int)blockIdx.x) before += h;
                 all += h;
             }
