@@ -241,8 +241,15 @@ exclusive_scan_noalloc!(out::CuVector{Int32}, counts::CuVector{Int32}, base::Int
 # library); W is a feature_out x feature_in x expert CuArray, i.e. row-major
 # in x out matrices.  Indices are 1-based; an id outside 1:E is dropped.
 _vt(::Type{Float32}) = Cint(0)
-_vt(::Type{T}) where {T} = sizeof(T) == 2 ? Cint(2) :
+# BFloat16 by its name: Core's or a package's, no other 16-bit type
+_vt(::Type{T}) where {T} = nameof(T) === :BFloat16 ? Cint(2) :
     throw(JLUST.UnsupportedValueType(T, B200Backend()))
+# The library takes addresses: every buffer's type and size is checked here.
+_is(a, ::Type{V}, dims, what) where {V} = (a isa CuArray{V} && size(a) == dims) ? nothing :
+    throw(JLUST.IncompatibleExtents("$what must be a CuArray{$V} of size $dims"))
+_maybe(a, V, dims, what) = a === nothing ? nothing : _is(a, V, dims, what)
+# the row pointer of E groups, or nothing for one group
+_groups(rowptr, E) = rowptr === nothing && E == 1 ? nothing : _is(rowptr, Int32, (E + 1,), "rowptr")
 _opt(x) = x === nothing ? CU_NULL : x
 _ld(x) = x === nothing ? Int64(0) : Int64(max(stride(x, 2), 1))
 
@@ -263,6 +270,7 @@ end
 # y[:, t] = sum_j g[j, t] z[:, slot[j, t]]
 function combine!(y::CuMatrix{V}, z::CuMatrix{V}, slot::CuMatrix{Int32}, g=nothing) where {V}
     k, T = size(slot); N, S = size(z)
+    _is(y, V, (N, T), "y"); _maybe(g, Float32, (k, T), "g")
     _check(ccall((:jlb_combine, lib), Cint,
                  (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, Int64, CuPtr{Int32}, CuPtr{Float32},
                   CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64),
@@ -273,6 +281,8 @@ end
 function combine_backward!(dz::CuMatrix{V}, dg::CuMatrix{Float32}, dy::CuMatrix{V}, z::CuMatrix{V},
                            rowptr::CuVector{Int32}, slot::CuMatrix{Int32}, g=nothing) where {V}
     k, T = size(slot); N, S = size(z)
+    _is(dz, V, (N, S), "dz"); _is(dg, Float32, (k, T), "dg"); _is(dy, V, (N, T), "dy")
+    _is(rowptr, Int32, (max(length(rowptr), 1),), "rowptr"); _maybe(g, Float32, (k, T), "g")
     _check(ccall((:jlb_combine_backward, lib), Cint,
                  (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Int32},
                   CuPtr{Int32}, CuPtr{Float32}, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
@@ -289,6 +299,9 @@ function grouped_mm!(y::CuMatrix{V}, x::CuMatrix{V}, W::CuArray{V,3}, rowptr=not
                      transposed::Bool=false) where {V}
     N, K = transposed ? (size(W, 2), size(W, 1)) : (size(W, 1), size(W, 2))
     E, S, T = size(W, 3), size(y, 2), size(x, 2)
+    _is(y, V, (N, S), "y"); _is(x, V, (K, T), "x"); _groups(rowptr, E)
+    _maybe(rows, Int32, (S,), "rows"); _maybe(bias, V, (N, E), "bias")
+    _maybe(res, V, (N, S), "res"); _maybe(z, V, (N, S), "z")
     order, ldw, sw = Cint(transposed ? 1 : 0), stride(W, 2), stride(W, 3)
     wsb = ccall((:jlb_grouped_mm_workspace_size, lib), Csize_t,
                 (Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
@@ -310,6 +323,8 @@ end
 function grouped_mm_wgrad!(dW::CuArray{V,3}, x::CuMatrix{V}, dz::CuMatrix{V}, rowptr=nothing;
                            rows=nothing) where {V}
     N, K, E = size(dW); S, T = size(dz, 2), size(x, 2)
+    _is(dz, V, (N, S), "dz"); _is(x, V, (K, T), "x"); _groups(rowptr, E)
+    _maybe(rows, Int32, (S,), "rows")
     wsb = ccall((:jlb_grouped_mm_wgrad_workspace_size, lib), Csize_t,
                 (Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
                  Cint, Cint),
@@ -327,6 +342,8 @@ end
 # dz = dy .* act'(z) and db[:, e] = sum of group e's columns of dz
 function act_backward!(dz, db, dy::CuMatrix{V}, z, rowptr=nothing; act::Integer=0, E::Integer=1) where {V}
     N, S = size(dy)
+    _maybe(z, V, (N, S), "z"); _maybe(dz, V, (N, S), "dz"); _maybe(db, V, (N, E), "db")
+    _groups(rowptr, E)
     wsb = ccall((:jlb_act_backward_workspace_size, lib), Csize_t, (Int64, Int64, Int64, Cint),
                 E, S, N, Cint(db !== nothing))
     ws = CuArray{UInt8}(undef, Int(wsb))
