@@ -282,7 +282,7 @@ function combine_backward!(dz::CuMatrix{V}, dg::CuMatrix{Float32}, dy::CuMatrix{
                            rowptr::CuVector{Int32}, slot::CuMatrix{Int32}, g=nothing) where {V}
     k, T = size(slot); N, S = size(z)
     _is(dz, V, (N, S), "dz"); _is(dg, Float32, (k, T), "dg"); _is(dy, V, (N, T), "dy")
-    _is(rowptr, Int32, (max(length(rowptr), 1),), "rowptr"); _maybe(g, Float32, (k, T), "g")
+    _maybe(g, Float32, (k, T), "g")        # rowptr gives E (empty: -1, which the library refuses)
     _check(ccall((:jlb_combine_backward, lib), Cint,
                  (Ptr{Cvoid}, Cint, Cint, Int64, Int64, Int64, Int64, Int64, CuPtr{Int32},
                   CuPtr{Int32}, CuPtr{Float32}, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64,
