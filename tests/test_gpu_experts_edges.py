@@ -81,3 +81,34 @@ def test_products_back_to_back_with_few_and_many_tiles_a_pair(dtype):
             first = first or got
         J.device_status()
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+# -------------------------------------------------- tails of the activations
+
+def tail(dtype, M):
+    z = torch.linspace(-10, -3, M, dtype=torch.float64).to(dtype)
+    return z.view(M, 1).to(DEV), z.double().numpy()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [8, 40, 700])
+def test_gelu_keeps_its_negative_tail(dtype, M):
+    """Relative to the result, value and slope, against erfc in 64 bits.  F32:
+    the argument z / sqrt 2 is rounded twice (a unit and a half of 2^-24), which
+    erfc multiplies by z^2 + 1; erfcf's 4 units and the products' roundings are
+    a dozen more.  In the slope expf(-z^2 / 2) does the same and the difference
+    of the two terms is 0.8 of the larger at least.  BF16: 5e-6 of the fit, and
+    the same with the cheaper exponential's 60 units of 2^-23, below 1e-4 in
+    all, then the rounding."""
+    z, z64 = tail(dtype, M)
+    phi = np.array([0.5 * math.erfc(-v / math.sqrt(2)) for v in z64])
+    slope = phi + z64 * np.exp(-0.5 * z64 * z64) / math.sqrt(2 * math.pi)
+    one = torch.ones(1, 1, dtype=dtype, device=DEV)
+    y = J.fused_matmul(z, one, act="gelu")
+    dz, _, _ = J.fused_matmul_backward(torch.ones_like(z), z, one, z=z, act="gelu")
+    J.device_status()
+    rel = (3 * z64 * z64 + 32) * 2.0 ** -24 if dtype == F32 else 1e-4
+    for got, want in ((y, z64 * phi), (dz, slope)):
+        err = np.abs(R.f64(got)[:, 0] / want - 1)
+        lim = rel + R.HALF_ULP[dtype] * (1 + rel)
+        assert (err <= lim).all(), (z64[err > lim][0], err.max())
