@@ -9,6 +9,7 @@ import torch
 
 import jlust_b200 as J
 import _experts_ref as R
+from _planes import F32_NORM
 from _helpers import DEV
 from jlust_b200 import _lib
 
@@ -112,3 +113,27 @@ def test_gelu_keeps_its_negative_tail(dtype, M):
         err = np.abs(R.f64(got)[:, 0] / want - 1)
         lim = rel + R.HALF_ULP[dtype] * (1 + rel)
         assert (err <= lim).all(), (z64[err > lim][0], err.max())
+
+
+# ------------------------------------------------ how exact F32 products are
+
+@pytest.mark.parametrize("order", ["row", "col"])
+@pytest.mark.parametrize("K,N", [(320, 640), (520, 257), (1536, 264), (641, 72)])
+@pytest.mark.parametrize("sizes", [[130], [459], [260, 31, 0, 168], [1601, 70]])
+def test_f32_products_keep_three_planes(order, K, N, sizes):
+    """The forward product, dx and dw of shapes that run as planes of bf16, in
+    the norm: element by element, a bound for any values lets a lost third
+    plane through."""
+    ptr, E, S = np.concatenate([[0], np.cumsum(sizes)]), len(sizes), sum(sizes)
+    x, dy = randn((S, K), F32, 1), randn((S, N), F32, 3)
+    w = randn((E, K, N), F32, 2) if order == "row" else randn((E, N, K), F32, 2).transpose(1, 2)
+    y = J.grouped_matmul(x, w, dev_i32(ptr))
+    dx, dw, _ = J.grouped_matmul_backward(dy, x, w, dev_i32(ptr))
+    J.device_status()
+    ry, _, _, _ = R.forward(R.f64(x), R.f64(w), ptr)
+    (rdx, rdw, _), _ = R.backward(R.f64(dy), R.f64(x), R.f64(w), ptr)
+    for got, want, what in ((y, ry, "y"), (dx, rdx, "dx"), (dw, rdw, "dw")):
+        assert np.linalg.norm(R.f64(got) - want) <= F32_NORM * np.linalg.norm(want), what
+    if E == 1:
+        y = J.fused_matmul(x, w[0])
+        assert np.linalg.norm(R.f64(y) - ry) <= F32_NORM * np.linalg.norm(ry)
