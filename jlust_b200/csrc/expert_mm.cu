@@ -105,6 +105,14 @@ __device__ __forceinline__ void tile_product(const Operand<T> &A, int64_t m0, in
 
 __device__ __forceinline__ int tile_index(int t, int i) { return (i < 4 ? 0 : 64) + t * 4 + (i & 3); }
 
+// Grid extents y and z hold 65,535 CTAs each: numbers up to n lie in y and, past
+// that, in z (a loop in the kernel instead made act_backward 28 % slower).
+static dim3 in_yz(int64_t x, int64_t n) {
+    const int64_t y = n < 65535 ? n : 65535;
+    return dim3((unsigned)x, (unsigned)y, (unsigned)(y ? ceil_div(n, y) : 1));
+}
+__device__ __forceinline__ int64_t at_yz() { return (int64_t)blockIdx.z * gridDim.y + blockIdx.y; }
+
 // The group and first row of row tile `want`, tiles of `size` rows numbered
 // group by group; e = -1 past the last.  Warp 0 scans 32 groups at a time.
 struct Found {
@@ -137,17 +145,17 @@ __device__ void find_row_tile(const int32_t *rowptr, int base, int64_t S, int64_
 template <typename T>
 __global__ void __launch_bounds__(kSimtThreads) product_simt(const Product P) {
     __shared__ Found f;
-    find_row_tile(P.rowptr, P.base, P.S, P.E, kTile, blockIdx.y, &f);
+    const int64_t tile = at_yz(), tiles = (int64_t)gridDim.z * gridDim.y;
+    find_row_tile(P.rowptr, P.base, P.S, P.E, kTile, tile, &f);
     if (blockIdx.x == 0 && P.rowptr) {
-        for (int64_t e = (int64_t)blockIdx.y * kSimtThreads + threadIdx.x; e < P.E;
-             e += (int64_t)gridDim.y * kSimtThreads)
+        for (int64_t e = tile * kSimtThreads + threadIdx.x; e < P.E; e += tiles * kSimtThreads)
             if (group_bad(P.rowptr, P.base, P.S, e)) dev_error(DEV_ERR_BOUNDS);
     }
     // rows of no group are zero
     if (P.rowptr) {
         int lo, hi;
         group_rows(P.rowptr, P.base, P.S, P.E - 1, lo, hi);
-        for (int64_t r = hi + blockIdx.y; r < P.S; r += gridDim.y)
+        for (int64_t r = hi + tile; r < P.S; r += tiles)
             for (int64_t c = (int64_t)blockIdx.x * kSimtThreads + threadIdx.x; c < P.N;
                  c += (int64_t)gridDim.x * kSimtThreads) {
                 ((T *)P.y)[r * P.ldy + c] = from_f32<T>(0.0f);
@@ -184,26 +192,28 @@ __global__ void __launch_bounds__(kSimtThreads) product_simt(const Product P) {
 // column-major dw is computed as its transpose, the operands swapped.
 template <typename T>
 __global__ void __launch_bounds__(kSimtThreads) gradient_simt(const Gradient G) {
-    const int64_t e = blockIdx.z;
-    int lo, hi;
-    group_rows(G.rowptr, G.base, G.S, e, lo, hi);
-    if (group_bad(G.rowptr, G.base, G.S, e) && threadIdx.x == 0) dev_error(DEV_ERR_BOUNDS);
-    Operand<T> X{(const T *)G.x, G.ldx, false, G.rows, G.base, G.T, lo};
-    Operand<T> D{(const T *)G.dz, G.lddz, false, nullptr, 0, 0, lo};
     const bool col = G.w_order == JLB_COL_MAJOR;
-    const int64_t M = col ? G.N : G.K, N = col ? G.K : G.N;
-    const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
-    float acc[8][8];
-    tile_product<T>(col ? D : X, m0, M, col ? X : D, n0, N, hi - lo, acc);
+    const int64_t M = col ? G.N : G.K, N = col ? G.K : G.N, n0 = (int64_t)blockIdx.x * kTile;
     const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-    T *out = (T *)G.dw + e * G.dw_stride;
+    for (int64_t e = blockIdx.z; e < G.E; e += gridDim.z) {
+        int lo, hi;
+        group_rows(G.rowptr, G.base, G.S, e, lo, hi);
+        if (group_bad(G.rowptr, G.base, G.S, e) && threadIdx.x == 0) dev_error(DEV_ERR_BOUNDS);
+        Operand<T> X{(const T *)G.x, G.ldx, false, G.rows, G.base, G.T, lo};
+        Operand<T> D{(const T *)G.dz, G.lddz, false, nullptr, 0, 0, lo};
+        T *out = (T *)G.dw + e * G.dw_stride;
+        for (int64_t m0 = (int64_t)blockIdx.y * kTile; m0 < M; m0 += (int64_t)gridDim.y * kTile) {
+            float acc[8][8];
+            tile_product<T>(col ? D : X, m0, M, col ? X : D, n0, N, hi - lo, acc);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t r = m0 + tile_index(ty, i), c = n0 + tile_index(tx, j);
-            if (r < M && c < N) out[r * G.lddw + c] = from_f32<T>(acc[i][j]);
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t r = m0 + tile_index(ty, i), c = n0 + tile_index(tx, j);
+                    if (r < M && c < N) out[r * G.lddw + c] = from_f32<T>(acc[i][j]);
+                }
         }
+    }
 }
 
 // ------------------------------------------------- activation's gradient
@@ -276,14 +286,16 @@ __device__ __forceinline__ void act_rows(int lo, int hi, int64_t c, const T *__r
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256, 4)
-act_backward(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__ rowptr, int act,
+act_backward(int64_t tiles, int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__ rowptr, int act,
              const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z, int64_t ldz,
              T *__restrict__ dz, int64_t lddz, float *__restrict__ part) {
     __shared__ Found f;
     __shared__ float red[8][32 * V];
-    find_row_tile(rowptr, base, S, E, kSumRows, blockIdx.y, &f);
+    const int64_t tile = at_yz();
+    if (tile >= tiles) return;                     // part has no place for it
+    find_row_tile(rowptr, base, S, E, kSumRows, tile, &f);
     if (blockIdx.x == 0)
-        for (int64_t e = (int64_t)blockIdx.y * 256 + threadIdx.x; e < E; e += (int64_t)gridDim.y * 256)
+        for (int64_t e = tile * 256 + threadIdx.x; e < E; e += tiles * 256)
             if (group_bad(rowptr, base, S, e)) dev_error(DEV_ERR_BOUNDS);
     __syncthreads();
     if (f.e < 0) return;
@@ -311,7 +323,7 @@ act_backward(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restric
         float s = red[0][i];
 #pragma unroll
         for (int q = 1; q < 8; ++q) s += red[q][i];
-        part[(int64_t)blockIdx.y * N + col] = s;
+        part[tile * N + col] = s;
     }
 }
 
@@ -320,9 +332,10 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 sum_parts(int64_t E, int64_t S, int64_t N, int base, const int32_t *__restrict__ rowptr,
           const float *__restrict__ part, int64_t parts, T *__restrict__ db, int64_t lddb) {
-    const int64_t e = blockIdx.y;
+    const int64_t e = at_yz();
     __shared__ int64_t first_s;
     __shared__ int count_s;
+    if (e >= E) return;
     if (threadIdx.x < kWarp) {                 // the group's parts: after those of the groups before
         int64_t first = 0;
         for (int64_t i = threadIdx.x; i < e; i += kWarp) {
@@ -356,12 +369,12 @@ static int launch_act(cudaStream_t st, int64_t tiles, int64_t E, int64_t S, int6
     constexpr int V = 16 / (int)sizeof(T);
     const bool vec = N % V == 0 && lddy % V == 0 && aligned16(dy) && (!z || (ldz % V == 0 && aligned16(z))) &&
                      (!dz || (lddz % V == 0 && aligned16(dz)));
-    const dim3 grid((unsigned)ceil_div(N, vec ? 32 * V : 32), (unsigned)tiles);
+    const dim3 grid = in_yz(ceil_div(N, vec ? 32 * V : 32), tiles);
     if (vec)
-        act_backward<T, V><<<grid, 256, 0, st>>>(E, S, N, base, rowptr, act, (const T *)dy, lddy, (const T *)z, ldz,
+        act_backward<T, V><<<grid, 256, 0, st>>>(tiles, E, S, N, base, rowptr, act, (const T *)dy, lddy, (const T *)z, ldz,
                                                  (T *)dz, lddz, part);
     else
-        act_backward<T, 1><<<grid, 256, 0, st>>>(E, S, N, base, rowptr, act, (const T *)dy, lddy, (const T *)z, ldz,
+        act_backward<T, 1><<<grid, 256, 0, st>>>(tiles, E, S, N, base, rowptr, act, (const T *)dy, lddy, (const T *)z, ldz,
                                                  (T *)dz, lddz, part);
     JLB_LAUNCH_CHECK("act_backward");
     return JLB_OK;
@@ -665,8 +678,7 @@ static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_by
         if (r >= 0) return r;
     }
     const int64_t ntiles = ceil_div(P.N, kTile), rtiles = row_tiles_bound(P.E, P.S, P.rowptr, kTile);
-    if (rtiles > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "too many rows (%lld)", (long long)P.S);
-    const dim3 grid((unsigned)ntiles, (unsigned)rtiles);
+    const dim3 grid = in_yz(ntiles, rtiles);
     if (P.dtype == JLB_F32) product_simt<float><<<grid, kSimtThreads, 0, st>>>(P);
     else product_simt<__nv_bfloat16><<<grid, kSimtThreads, 0, st>>>(P);
     JLB_LAUNCH_CHECK("product_simt");
@@ -730,8 +742,7 @@ static int run_gradient(cudaStream_t st, const Gradient &G, void *ws, size_t ws_
     }
     const bool col = G.w_order == JLB_COL_MAJOR;
     const int64_t mt = ceil_div(col ? G.N : G.K, kTile), nt = ceil_div(col ? G.K : G.N, kTile);
-    if (mt > 65535 || G.E > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent too large");
-    const dim3 grid((unsigned)nt, (unsigned)mt, (unsigned)G.E);
+    const dim3 grid((unsigned)nt, (unsigned)(mt < 65535 ? mt : 65535), (unsigned)(G.E < 65535 ? G.E : 65535));
     if (G.dtype == JLB_F32) gradient_simt<float><<<grid, kSimtThreads, 0, st>>>(G);
     else gradient_simt<__nv_bfloat16><<<grid, kSimtThreads, 0, st>>>(G);
     JLB_LAUNCH_CHECK("gradient_simt");
@@ -946,7 +957,6 @@ extern "C" JLB_API int jlb_act_backward(void *stream, int dtype, int idx_base, i
     if (act == JLB_ACT_NONE) z = nullptr;
     cudaStream_t st = as_stream(stream);
     const int64_t tiles = emm::row_tiles_bound(E, S, rowptr, emm::kSumRows);
-    if (tiles > 65535 || E > 65535) return fail(JLB_ERR_UNSUPPORTED_INDEX_TYPE, "extent too large");
     float *part = db ? (float *)workspace : nullptr;
     if (tiles > 0) {
         r = dtype == JLB_F32 ? emm::launch_act<float>(st, tiles, E, S, N, idx_base, rowptr, act, dy, lddy, z, ldz, dz, lddz, part)
@@ -955,7 +965,7 @@ extern "C" JLB_API int jlb_act_backward(void *stream, int dtype, int idx_base, i
         if (r) return r;
     }
     if (db) {
-        const dim3 grid((unsigned)ceil_div(N, 256), (unsigned)E);
+        const dim3 grid = emm::in_yz(ceil_div(N, 256), E);
         if (dtype == JLB_F32)
             emm::sum_parts<float><<<grid, 256, 0, st>>>(E, S, N, idx_base, rowptr, part, tiles,
                                                         (float *)db, lddb);

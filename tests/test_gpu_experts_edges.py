@@ -137,3 +137,67 @@ def test_f32_products_keep_three_planes(order, K, N, sizes):
     if E == 1:
         y = J.fused_matmul(x, w[0])
         assert np.linalg.norm(R.f64(y) - ry) <= F32_NORM * np.linalg.norm(ry)
+
+
+# ------------------------------------------ extents past a launch's y and z
+
+def test_bias_sums_of_overlapping_ranges_past_the_grid():
+    """More tiles than grid y holds and ranges that overlap: the grid's last
+    layer has no part to write."""
+    L, S, E, N = _lib.load(), 65535 * 128 + 300, 3, 8
+    dy, ptr = torch.ones(S, N, dtype=BF, device=DEV), dev_i32([0, S, 0, S])
+    wsb = L.jlb_act_backward_workspace_size(E, S, N, 1)
+    ws = torch.full((wsb // 4 + (1 << 22),), float("nan"), device=DEV)
+    db = torch.empty(E, N, dtype=BF, device=DEV)
+    assert L.jlb_act_backward(torch.cuda.current_stream().cuda_stream, 2, 0, E, S, N, ptr.data_ptr(), 0,
+                              dy.data_ptr(), N, None, 0, None, 0, db.data_ptr(), N, ws.data_ptr(), wsb) == 0
+    with pytest.raises(J.NonCanonicalStorage):
+        J.device_status()
+    J.device_status()
+    assert ws[wsb // 4:].isnan().all() and db.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_more_rows_than_a_grid_has_tiles(dtype):
+    """65,535 tiles of 128 rows and more.  Ones in the last rows: their sums
+    are whole numbers, exact in either type."""
+    S, N, tail = 65535 * 128 + 300, 8, 200
+    dy, x = torch.zeros(S, N, dtype=dtype, device=DEV), torch.ones(S, N, dtype=dtype, device=DEV)
+    dy[-tail:] = 1
+    w = torch.eye(N, dtype=dtype, device=DEV)
+    for act in (None, "relu"):
+        assert J.fused_matmul(x, w, act=act).shape == (S, N)
+        dx, dw, db = J.fused_matmul_backward(dy, x, w, z=x, act=act, bias=True)
+        J.device_status()
+        assert torch.equal(dx, dy)
+        assert torch.equal(db, torch.full_like(db, tail)) and torch.equal(dw, torch.full_like(dw, tail))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_more_experts_than_a_grid_has_rows(dtype):
+    E, N = 70_000, 8
+    n = np.zeros(E, np.int64)
+    n[[3, 65_534, 65_535, 65_536, E - 1]] = [5, 2, 7, 1, 4]
+    ptr, S = dev_i32(np.concatenate([[0], np.cumsum(n)])), int(n.sum())
+    x, w = torch.ones(S, N, dtype=dtype, device=DEV), torch.ones(E, N, N, dtype=dtype, device=DEV)
+    z, dy = torch.ones_like(x), torch.ones_like(x)
+    y = J.grouped_matmul(x, w, ptr)
+    dx, dw, db = J.grouped_matmul_backward(dy, x, w, ptr, z=z, act="relu", bias=True)
+    J.device_status()
+    assert torch.equal(y, torch.full_like(y, N)) and torch.equal(dx, torch.full_like(dx, N))
+    want = torch.from_numpy(n).to(DEV).to(dtype)
+    assert torch.equal(db, want[:, None].expand(E, N)) and torch.equal(dw, want[:, None, None].expand(E, N, N))
+    # no rows at all: zeros
+    none = torch.empty(0, N, dtype=dtype, device=DEV)
+    dx, dw, db = J.grouped_matmul_backward(none, none, w, torch.zeros_like(ptr), bias=True)
+    J.device_status()
+    assert dx.shape == (0, N) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_products_without_an_inner_dimension_of_many_rows(dtype):
+    S, N = 65535 * 128 + 300, 8
+    b = randn((N,), dtype, 1)
+    y = J.fused_matmul(torch.empty(S, 0, dtype=dtype, device=DEV), torch.empty(0, N, dtype=dtype, device=DEV), bias=b)
+    J.device_status()
+    assert torch.equal(y, b.expand(S, N))
