@@ -517,7 +517,8 @@ JLB_API int jlb_combine_backward(void *stream, int dtype, int idx_base, int64_t 
  * groups are unspecified; nothing outside the buffers is touched.
  *
  * `workspace` holds the bytes the size query returns for the same operands
- * (0: none needed).  Asynchronous.
+ * (0: none needed) and starts on a 16-byte boundary, in every call of this
+ * section and the one before.  Asynchronous.
  *
  * A plan keeps the weight's side of the call (the buffers stay the caller's
  * and must outlive it; their values may change between calls). */

@@ -41,6 +41,11 @@ inline size_t dtype_size(int dtype) {
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// A workspace of `need` bytes that kernels store 16-byte vectors into.
+inline bool workspace_ok(const void *ws, size_t have, size_t need) {
+    return need == 0 || (ws && have >= need && aligned16(ws));
+}
+
 // ------------------------------------------------------------ device errors
 // Kernels report a bounded wait that gave up, or a bounds check that failed,
 // by OR-ing a bit into a per-translation-unit device word.  The host reads and

@@ -648,8 +648,8 @@ static int run_product(cudaStream_t st, const Product &P, void *ws, size_t ws_by
     if (skinny_ok(P) && P.T > 0) return skinny_product(st, P);
     ProductPlan q = plan_product(P);
     if (q.tc) {
-        if (q.bytes && (!ws || ws_bytes < q.bytes))
-            return fail(JLB_ERR_WORKSPACE, "the product needs %zu workspace bytes", q.bytes);
+        if (!workspace_ok(ws, ws_bytes, q.bytes))
+            return fail(JLB_ERR_WORKSPACE, "the product needs %zu workspace bytes, 16-byte aligned", q.bytes);
         const bool row = P.w_order == JLB_ROW_MAJOR;
         char *base = (char *)ws;
         Copy x{}, w{};
@@ -719,8 +719,8 @@ static GradientPlan plan_gradient(const Gradient &G) {
 static int run_gradient(cudaStream_t st, const Gradient &G, void *ws, size_t ws_bytes) {
     GradientPlan q = plan_gradient(G);
     if (q.tc) {
-        if (q.bytes && (!ws || ws_bytes < q.bytes))
-            return fail(JLB_ERR_WORKSPACE, "the gradient needs %zu workspace bytes", q.bytes);
+        if (!workspace_ok(ws, ws_bytes, q.bytes))
+            return fail(JLB_ERR_WORKSPACE, "the gradient needs %zu workspace bytes, 16-byte aligned", q.bytes);
         char *base = (char *)ws;
         Copy x{}, d{};
         if (q.copy_x) {
@@ -952,8 +952,8 @@ extern "C" JLB_API int jlb_act_backward(void *stream, int dtype, int idx_base, i
     if (N == 0 || E == 0 || (!dz && !db)) return ok();
     if (S > 0 && !dy) return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
     const size_t need = jlb_act_backward_workspace_size(E, S, N, db != nullptr);
-    if (need && (!workspace || workspace_bytes < need))
-        return fail(JLB_ERR_WORKSPACE, "act_backward needs %zu workspace bytes", need);
+    if (!workspace_ok(workspace, workspace_bytes, need))
+        return fail(JLB_ERR_WORKSPACE, "act_backward needs %zu workspace bytes, 16-byte aligned", need);
     if (act == JLB_ACT_NONE) z = nullptr;
     cudaStream_t st = as_stream(stream);
     const int64_t tiles = emm::row_tiles_bound(E, S, rowptr, emm::kSumRows);

@@ -433,8 +433,8 @@ extern "C" JLB_API int jlb_route(void *stream, int idx_base, int64_t T, int64_t 
         return fail(JLB_ERR_INVALID_ARGUMENT, "null buffer");
     const int chunks = (int)ceil_div(n > 0 ? n : 1, kChunk);
     const size_t need = jlb_route_workspace_size(T, k, E);
-    if (need && (!workspace || workspace_bytes < need))
-        return fail(JLB_ERR_WORKSPACE, "route needs %zu workspace bytes", need);
+    if (!workspace_ok(workspace, workspace_bytes, need))
+        return fail(JLB_ERR_WORKSPACE, "route needs %zu workspace bytes, 16-byte aligned", need);
     cudaStream_t st = as_stream(stream);
     int32_t *hist = need ? (int32_t *)workspace : nullptr, *at = nullptr;
     if (hist) {
