@@ -23,7 +23,9 @@ out of the assembled CSR and added by the patched SpMV kernel.
 """
 from __future__ import annotations
 
+import contextlib
 import gc
+import threading
 
 import numpy as np
 import torch
@@ -106,6 +108,33 @@ def _host_csr(b: USTensor):
     return rp, ci
 
 
+class _Collector:
+    """Python's cyclic collector, off while any thread captures a graph: a
+    collection that frees another graph resets it, which invalidates the capture.
+    The last of overlapping captures puts it back as the first found it."""
+
+    def __init__(self):
+        self._lock, self._captures, self._collects = threading.Lock(), 0, False
+
+    @contextlib.contextmanager
+    def paused(self):
+        with self._lock:
+            if self._captures == 0:
+                self._collects = gc.isenabled()
+                gc.disable()
+            self._captures += 1
+        try:
+            yield
+        finally:
+            with self._lock:
+                self._captures -= 1
+                if self._captures == 0 and self._collects:
+                    gc.enable()
+
+
+_collector = _Collector()
+
+
 class _Graphed:
     """Replays self.spmv(x, y) from a CUDA graph captured per (y, x) buffer
     pair; inside a capture the caller started, launches it directly."""
@@ -121,16 +150,8 @@ class _Graphed:
             self.spmv(x, y)          # first use outside the graph, then capture
             torch.cuda.current_stream(y.device).synchronize()
             g = torch.cuda.CUDAGraph()
-            # no cyclic collection meanwhile: one that frees another graph
-            # resets it, which invalidates the capture
-            collects = gc.isenabled()
-            gc.disable()
-            try:
-                with torch.cuda.graph(g):
-                    self.spmv(x, y)
-            finally:
-                if collects:
-                    gc.enable()
+            with _collector.paused(), torch.cuda.graph(g):
+                self.spmv(x, y)
             self.graphs[key] = g
         g.replay()
 
