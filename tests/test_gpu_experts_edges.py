@@ -201,3 +201,25 @@ def test_products_without_an_inner_dimension_of_many_rows(dtype):
     y = J.fused_matmul(torch.empty(S, 0, dtype=dtype, device=DEV), torch.empty(0, N, dtype=dtype, device=DEV), bias=b)
     J.device_status()
     assert torch.equal(y, b.expand(S, N))
+
+
+# ------------------------------------------------------------ entry points
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["row", "col"])
+def test_execute_grouped_in_place(dtype, order):
+    """execute(GroupedMMOp, x, w, rowptr, y, ...) writes y as grouped_matmul
+    returns it."""
+    E, K, N, sizes, base = 3, 72, 136, [40, 0, 25], 1
+    ptr, S = dev_i32(np.concatenate([[0], np.cumsum(sizes)]) + base), sum(sizes)
+    w = randn((E, K, N), dtype, 2) if order == "row" else randn((E, N, K), dtype, 2).transpose(1, 2)
+    x, b = randn((S, K), dtype, 1), randn((E, N), dtype, 3)
+    rows = dev_i32(np.random.default_rng(4).integers(0, S, S) + base)
+    y = torch.full((S, N), float("nan"), dtype=dtype, device=DEV)
+    J.execute(J.GroupedMMOp, x, w, ptr, y, bias=b, act="silu", rows=rows, origin=base)
+    J.device_status()
+    assert torch.equal(y, J.grouped_matmul(x, w, ptr, bias=b, act="silu", rows=rows, origin=base))
+    with pytest.raises(J.IncompatibleExtents):
+        J.execute(J.GroupedMMOp, x, w, ptr, y[:-1], origin=base)
+    with pytest.raises(J.UnsupportedIndexType):
+        J.execute(J.GroupedMMOp, x, w, ptr.long(), y, origin=base)
