@@ -15,16 +15,17 @@ constexpr int kWarps = kThreads / kWarp;
 constexpr int kPer = 4;                       // entries a thread
 constexpr int kChunk = kThreads * kPer;       // entries a CTA
 constexpr int kMaxE = 2048;
-// Chunks whose counts are scanned by kernels of their own (three launches
-// more) instead of being added up by every CTA (chunks x E loads each).
-// Measured in a graph, scanned against added up: 64 experts, 128 chunks 14.6
-// against 11.2 us and 256 chunks 20.8 against 21.5; 256 experts, 128 chunks
-// 15.9 against 17.6 and 256 chunks 25 against 46; 2,048 experts, 16 chunks
-// 26.7 against 28.4, 64 chunks 29 against 49, 512 chunks 97 against 852.  Among
-// other work, with the counts' way cold, the launches cost more: 256 experts,
-// 118 chunks 23.8 against 18.5 us.
+// Whether the chunks' counts are scanned by kernels of their own (three launches
+// more) instead of being added up by every CTA: each adds chunks x E counts, in as
+// many rounds as the SMs, one CTA each, need for the chunks.  A call among other
+// work, caches cold, added up against scanned: one round, 64 x 256 17 against
+// 28 us, 118 x 256 24 against 28, 128 x 512 32 against 30, 64 x 1,024 32 against
+// 34, 128 x 1,024 48 against 34, 32 x 2,048 38 against 42, 64 x 2,048 52 against
+// 42; two, 192 x 128 34 against 34, 256 x 64 30 against 34, 256 x 128 38 against
+// 34, 160 x 256 42 against 36; three and four, 384 x 64 46 against 44, 512 x 16
+// 42 against 46, 512 x 64 65 against 48, 512 x 2,048 861 against 112.
 __host__ __device__ constexpr bool scans_counts(int64_t chunks, int64_t E) {
-    return chunks > 192 || chunks * E > 49152;
+    return (chunks + 147) / 148 * chunks * E >= 65536;
 }
 
 // The expert of entry i, or -1 when it is dropped (outside 0 .. E-1).

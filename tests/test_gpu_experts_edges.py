@@ -203,6 +203,29 @@ def test_products_without_an_inner_dimension_of_many_rows(dtype):
     assert torch.equal(y, b.expand(S, N))
 
 
+# ------------------------------------------- routing around its two ways
+
+@pytest.mark.parametrize("E,chunks", [(512, 127), (512, 128), (16, 512), (64, 341), (64, 342), (128, 255), (128, 256),
+                                      (2048, 31), (2048, 32), (1, 600)])
+def test_route_on_both_sides_of_scanning_its_counts(E, chunks):
+    """4096 entries a chunk, the last one short."""
+    n = chunks * 4096 - 1000
+    ids = torch.randint(-1, E + 1, (n, 1), generator=torch.Generator().manual_seed(E + chunks), dtype=torch.int32)
+    r = J.route(ids.to(DEV), E)
+    J.device_status()
+    flat = ids.view(-1).long()
+    key = torch.where((flat < 0) | (flat >= E), E, flat)
+    order = torch.sort(key, stable=True).indices
+    counts = torch.bincount(key, minlength=E + 1)[:E]
+    live = int(counts.sum())
+    assert torch.equal(r.rowptr.cpu().long(), torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]))
+    slot = torch.full((n,), -1, dtype=torch.long)
+    slot[order[:live]] = torch.arange(live)
+    source = torch.full((n,), -1, dtype=torch.long)
+    source[:live] = order[:live]
+    assert torch.equal(r.slot.cpu().long().view(-1), slot) and torch.equal(r.source.cpu().long(), source)
+
+
 # ------------------------------------------------------------ entry points
 
 @pytest.mark.parametrize("dtype", TYPES)
