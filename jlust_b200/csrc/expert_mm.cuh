@@ -80,9 +80,9 @@ __device__ __forceinline__ bool group_bad(const int32_t *__restrict__ rowptr, in
 
 // ------------------------------------------------------------ activations
 // relu keeps NaN.  silu = z / (1 + e^-z); gelu = z Phi(z).  For BF16 results the
-// exponential and the quotients are cheaper; relative to the result, silu's
-// error is a few units of 2^-22 and gelu's below 1e-4 down to z = -10, and the
-// rounding to 8 bits is 2^-8.  silu is 0 where e^-z or its sum leaves the
+// exponential and the quotients are cheaper; relative to the result, silu's and
+// gelu's errors stay below 1e-4 down to z = -10 (the exponential's grows with its
+// argument), and the rounding to 8 bits is 2^-8.  silu is 0 where e^-z or its sum leaves the
 // quotient's range, below z = -87.3 (BF16) and -88.7 (F32): there its size is
 // under 1.1e-36.
 
